@@ -39,6 +39,7 @@ GP_BF16 = 1
 
 ACT_NONE, ACT_RELU, ACT_GELU_TANH, ACT_SILU, ACT_SIGMOID = 0, 1, 2, 3, 4
 TAIL_NONE, TAIL_LAYERNORM, TAIL_RESIDUAL_LN = 0, 1, 2
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 
 # every symbol include/gpipes.h declares
 EXPORTED_SYMBOLS = (
@@ -60,6 +61,15 @@ EXPORTED_SYMBOLS = (
     "gp_mgn_edge_update_out",
     "gp_mgn_node_update_out",
     "gp_gc_edges_bf16_noalloc_out",
+    "gp_block_norm_out",
+    "gp_w4_packed_bytes",
+    "gp_w4_quantize_out",
+    "gp_w4_pack_out",
+    "gp_w4_unpack_out",
+    "gp_w4_dequantize_out",
+    "gp_w4_linear_out",
+    "gp_w4_mlp_out",
+    "gp_w4_mlp_workspace_bytes",
     "gp_last_error",
     "gp_device_status",
     "gp_set_timeout_ns",
@@ -87,6 +97,32 @@ class GpSpec(ctypes.Structure):
         ("dtype", ctypes.c_int),
         ("ln_eps", ctypes.c_float),
         ("skip_layer", ctypes.c_int),
+    ]
+
+
+class GpBlockNormSpec(ctypes.Structure):
+    _fields_ = [
+        ("width", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+        ("stream_f32", ctypes.c_int),
+        ("y_f32", ctypes.c_int),
+        ("post", ctypes.c_int),
+        ("pre", ctypes.c_int),
+        ("post_eps", ctypes.c_float),
+        ("pre_eps", ctypes.c_float),
+        ("x_scale", ctypes.c_float),
+        ("y_scale", ctypes.c_float),
+        ("gate_rows", ctypes.c_int64),
+    ]
+
+
+class GpW4Spec(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("group", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+        ("zero_points", ctypes.c_int),
     ]
 
 
@@ -136,6 +172,26 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.gp_dlrm_topmlp_out.restype = _INT
     lib.gp_gc_edges_bf16_noalloc_out.argtypes = [_I64, _INT] + [_P] * 9
     lib.gp_gc_edges_bf16_noalloc_out.restype = _INT
+    lib.gp_block_norm_out.argtypes = [ctypes.POINTER(GpBlockNormSpec), _I64] + [_P] * 10
+    lib.gp_block_norm_out.restype = _INT
+    w4 = ctypes.POINTER(GpW4Spec)
+    lib.gp_w4_packed_bytes.argtypes = [w4]
+    lib.gp_w4_packed_bytes.restype = _I64
+    lib.gp_w4_quantize_out.argtypes = [w4, _P, _P, _P]
+    lib.gp_w4_quantize_out.restype = _INT
+    lib.gp_w4_pack_out.argtypes = [w4, _P, _P, _P, _P, _P]
+    lib.gp_w4_pack_out.restype = _INT
+    lib.gp_w4_unpack_out.argtypes = [w4, _P, _P, _P, _P, _P]
+    lib.gp_w4_unpack_out.restype = _INT
+    lib.gp_w4_dequantize_out.argtypes = [w4, _P, _P, _P]
+    lib.gp_w4_dequantize_out.restype = _INT
+    lib.gp_w4_linear_out.argtypes = [w4, _I64, _INT, _P, _P, _P, _P, _P]
+    lib.gp_w4_linear_out.restype = _INT
+    lib.gp_w4_mlp_out.argtypes = [ctypes.POINTER(GpSpec), _INT, _INT, _I64, _P, ctypes.POINTER(_P),
+                                  ctypes.POINTER(_P), _P, _P, _P, _P, _I64, _P]
+    lib.gp_w4_mlp_out.restype = _INT
+    lib.gp_w4_mlp_workspace_bytes.argtypes = [ctypes.POINTER(GpSpec), _I64]
+    lib.gp_w4_mlp_workspace_bytes.restype = _I64
     lib.gp_last_error.argtypes = []
     lib.gp_last_error.restype = ctypes.c_char_p
     lib.gp_device_status.argtypes = [_INT, _INT, ctypes.POINTER(_INT)]

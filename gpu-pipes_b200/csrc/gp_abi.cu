@@ -21,8 +21,10 @@
 #include <vector>
 
 #include "../../include/gpipes.h"
+#include "block_norm.cuh"
 #include "chain_common.cuh"
 #include "chain_registry.h"
+#include "w4.cuh"
 
 namespace gp {
 
@@ -330,10 +332,10 @@ static int validate(const gp_mlp_spec* spec, int64_t m, const void* x, const voi
   return GP_OK;
 }
 
-int finish_launch(cudaStream_t stream, int dev_status_check) {
+int finish_launch(cudaStream_t stream, int dev_status_check, int launches) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(GP_ERR_CUDA, "launch: %s", cudaGetErrorString(e));
-  g_launches.fetch_add(1, std::memory_order_relaxed);
+  count_launches(launches);
   if (dev_status_check && sync_check_enabled()) {
     e = cudaStreamSynchronize(stream);
     if (e != cudaSuccess) return set_error(GP_ERR_CUDA, "sync: %s", cudaGetErrorString(e));
@@ -346,6 +348,13 @@ int finish_launch(cudaStream_t stream, int dev_status_check) {
     if (h != 0) return set_error(GP_ERR_TIMEOUT, "device wait ran out (status 0x%x)", h);
   }
   return GP_OK;
+}
+
+int device_sm_count(int* sm_count) {
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc == GP_OK) *sm_count = st->sm_count;
+  return rc;
 }
 
 // resid: residual rows of a GP_TAIL_RESIDUAL_LN chain ([m, N_last]); null means x itself.
@@ -504,6 +513,231 @@ int fused_mlp_host(const gp_mlp_spec* spec, int64_t m, const void* x_host, const
   if (rc != GP_OK) return rc;
   if (e != cudaSuccess) return set_error(GP_ERR_CUDA, "host pipeline: %s", cudaGetErrorString(e));
   return GP_OK;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Block norms and 4-bit weights
+// ------------------------------------------------------------------------------------------------
+// Whether two buffers share a byte (null ones do not).
+static bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && x < y + nb && y < x + na;
+}
+
+static int block_norm(const gp_block_norm_spec* s, int64_t m, const void* x, const void* y, const void* gate,
+                      const void* post_gamma, const void* post_beta, const void* pre_gamma,
+                      const void* pre_beta, void* r, void* h, cudaStream_t stream) {
+  clear_error();
+  if (s == nullptr) return set_error(GP_ERR_ARG, "spec is NULL");
+  if (s->dtype != GP_F16 && s->dtype != GP_BF16) return set_error(GP_ERR_ARG, "dtype %d unknown", s->dtype);
+  if (m < 0) return set_error(GP_ERR_ARG, "m = %lld is negative", (long long)m);
+  if (m >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "m = %lld exceeds 2^31-1", (long long)m);
+  if (s->width <= 0 || s->width % 8 != 0 || s->width > kBlockNormMaxWidth)
+    return set_error(GP_ERR_SHAPE, "width %d must be a multiple of 8 up to %d", s->width, kBlockNormMaxWidth);
+  if (s->post < GP_NORM_NONE || s->post > GP_NORM_RMS || s->pre < GP_NORM_NONE || s->pre > GP_NORM_RMS)
+    return set_error(GP_ERR_ARG, "norms %d, %d unknown", s->post, s->pre);
+  if (s->gate_rows < 0) return set_error(GP_ERR_ARG, "gate_rows = %lld is negative", (long long)s->gate_rows);
+  if (m == 0) return GP_OK;  // empty tensors may come as NULL
+  if (x == nullptr && y == nullptr) return set_error(GP_ERR_ARG, "x and y are both NULL");
+  if (r == nullptr && h == nullptr) return set_error(GP_ERR_ARG, "r and h are both NULL");
+  if (y == nullptr && (s->post != GP_NORM_NONE || gate != nullptr))
+    return set_error(GP_ERR_ARG, "a norm or a gate of the block's output needs y");
+  const void* ptrs[9] = {x, y, gate, post_gamma, post_beta, pre_gamma, pre_beta, r, h};
+  for (const void* p : ptrs)
+    if (!aligned(p, 16)) return set_error(GP_ERR_ALIGN, "buffers must be 16-byte aligned");
+  const uint64_t n = static_cast<uint64_t>(m) * static_cast<uint64_t>(s->width);
+  const uint64_t sb = s->stream_f32 ? 4 : 2, yb = s->y_f32 ? 4 : 2, row = static_cast<uint64_t>(s->width) * 2;
+  const uint64_t gr = s->gate_rows > 0 ? (static_cast<uint64_t>(m) + s->gate_rows - 1) / s->gate_rows : 1;
+  // an output may replace an input element for element (same address, same element size)
+  auto clash = [&](const void* o, uint64_t ob, const void* i, uint64_t ib) {
+    return overlap(o, n * ob, i, n * ib) && !(o == i && ob == ib);
+  };
+  if (overlap(r, n * sb, h, n * 2)) return set_error(GP_ERR_ARG, "r and h overlap");
+  if (clash(r, sb, x, sb) || clash(r, sb, y, yb) || clash(h, 2, x, sb) || clash(h, 2, y, yb))
+    return set_error(GP_ERR_ARG, "an output overlaps an input without replacing it element for element");
+  for (int i = 2; i < 7; ++i)
+    if (overlap(r, n * sb, ptrs[i], i == 2 ? gr * row : row) || overlap(h, n * 2, ptrs[i], i == 2 ? gr * row : row))
+      return set_error(GP_ERR_ARG, "an output overlaps the gate or a norm's parameters");
+  int sms = 0;
+  int rc = device_sm_count(&sms);
+  if (rc != GP_OK) return rc;
+  BlockNormArgs a;
+  a.m = m;
+  a.gate_rows = s->gate_rows;
+  a.width = s->width;
+  a.post = s->post;
+  a.pre = s->pre;
+  a.x_scale = s->x_scale;
+  a.y_scale = s->y_scale;
+  a.post_eps = s->post_eps;
+  a.pre_eps = s->pre_eps;
+  a.x = x;
+  a.y = y;
+  a.gate = gate;
+  a.post_gamma = post_gamma;
+  a.post_beta = post_beta;
+  a.pre_gamma = pre_gamma;
+  a.pre_beta = pre_beta;
+  a.r = r;
+  a.h = h;
+  rc = launch_block_norm(a, s->dtype, s->stream_f32 != 0, s->y_f32 != 0, stream);
+  return rc == GP_OK ? finish_launch(stream, 1) : rc;
+}
+
+static int w4_layout(const gp_w4_spec* s, W4Layout* l) {
+  if (s == nullptr) return set_error(GP_ERR_ARG, "spec is NULL");
+  if (s->dtype != GP_F16 && s->dtype != GP_BF16) return set_error(GP_ERR_ARG, "dtype %d unknown", s->dtype);
+  if (s->k <= 0 || s->k % 8 != 0 || s->k > kW4MaxK)
+    return set_error(GP_ERR_SHAPE, "K = %lld must be a multiple of 8 up to %lld", (long long)s->k, (long long)kW4MaxK);
+  if (s->n <= 0 || s->n > kW4MaxN)
+    return set_error(GP_ERR_SHAPE, "N = %lld out of range [1, %lld]", (long long)s->n, (long long)kW4MaxN);
+  if (s->group != 32 && s->group != 64 && s->group != 128)
+    return set_error(GP_ERR_UNSUPPORTED, "group %d (32, 64 or 128)", s->group);
+  *l = W4Layout::make(s->k, s->n, s->group, s->zero_points);
+  return GP_OK;
+}
+
+// The checks of the kernels that turn weights into the packed form or back: `packed` and one
+// [K, N] matrix of eb-byte elements, the other side's buffers in others.
+struct W4Buf {
+  const void* p;
+  uint64_t bytes;
+  int align;
+  const char* name;
+};
+
+static int w4_check(const W4Layout& l, const void* packed, const W4Buf* bufs, int n) {
+  if (packed == nullptr) return set_error(GP_ERR_ARG, "packed is NULL");
+  if (!aligned(packed, 16)) return set_error(GP_ERR_ALIGN, "packed must be 16-byte aligned");
+  for (int i = 0; i < n; ++i) {
+    if (!aligned(bufs[i].p, bufs[i].align))
+      return set_error(GP_ERR_ALIGN, "%s must be %d-byte aligned", bufs[i].name, bufs[i].align);
+    if (overlap(packed, l.bytes, bufs[i].p, bufs[i].bytes))
+      return set_error(GP_ERR_ARG, "%s overlaps packed", bufs[i].name);
+    for (int j = 0; j < i; ++j)
+      if (overlap(bufs[j].p, bufs[j].bytes, bufs[i].p, bufs[i].bytes))
+        return set_error(GP_ERR_ARG, "%s overlaps %s", bufs[i].name, bufs[j].name);
+  }
+  return GP_OK;
+}
+
+// One layer; the launcher counts its launches.
+static int w4_linear(const W4Layout& l, int dtype, int64_t m, int act, const void* x, const void* packed,
+                     const void* bias, void* out, bool out_f32, cudaStream_t stream) {
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != GP_OK) return rc;
+  return launch_w4_linear(l, dtype, m, x, packed, bias, act, out, out_f32, stream, sms);
+}
+
+static uint64_t align256(uint64_t b) { return (b + 255) / 256 * 256; }
+
+// Two buffers of hidden activations (layers alternate), and the fp32 rows before a tail.
+struct W4MlpPlan {
+  uint64_t hidden = 0, pre = 0, total = 0;
+  int buffers = 0;
+};
+
+static int w4_mlp_plan(const gp_mlp_spec* s, int64_t m, W4MlpPlan* p) {
+  if (s == nullptr) return set_error(GP_ERR_ARG, "spec is NULL");
+  if (s->n_layers < 1 || s->n_layers > GP_MAX_LAYERS)
+    return set_error(GP_ERR_SHAPE, "n_layers %d out of range [1, %d]", s->n_layers, GP_MAX_LAYERS);
+  if (s->dtype != GP_F16 && s->dtype != GP_BF16) return set_error(GP_ERR_ARG, "dtype %d unknown", s->dtype);
+  if (m < 0) return set_error(GP_ERR_ARG, "m = %lld is negative", (long long)m);
+  if (m >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "m = %lld exceeds 2^31-1", (long long)m);
+  if (s->skip_layer != 0) return set_error(GP_ERR_UNSUPPORTED, "skip_layer %d on 4-bit weights", s->skip_layer);
+  if (s->tail < GP_TAIL_NONE || s->tail > GP_TAIL_RESIDUAL_LN) return set_error(GP_ERR_ARG, "tail %d unknown", s->tail);
+  const int nl = s->n_layers, last = s->widths[nl];
+  for (int i = 0; i < nl; ++i)
+    if (s->widths[i] <= 0 || s->widths[i] % 8 != 0 || s->widths[i] > kW4MaxK)
+      return set_error(GP_ERR_SHAPE, "width[%d] = %d must be a multiple of 8 up to %lld", i, s->widths[i], (long long)kW4MaxK);
+  if (last <= 0 || last > kW4MaxN) return set_error(GP_ERR_SHAPE, "width[%d] = %d", nl, last);
+  for (int i = 0; i < nl; ++i)
+    if ((i + 1 < nl || s->tail == GP_TAIL_NONE) && (s->act[i] < GP_ACT_NONE || s->act[i] > GP_ACT_SIGMOID))
+      return set_error(GP_ERR_ARG, "act[%d] = %d unknown", i, s->act[i]);
+  if (s->tail != GP_TAIL_NONE && (last % 8 != 0 || last > kBlockNormMaxWidth))
+    return set_error(GP_ERR_SHAPE, "a LayerNorm tail needs a last width that is a multiple of 8 up to %d (%d)",
+                     kBlockNormMaxWidth, last);
+  if (s->tail == GP_TAIL_RESIDUAL_LN && s->widths[0] != last)
+    return set_error(GP_ERR_SHAPE, "residual tail needs K0 == N_last (%d vs %d)", s->widths[0], last);
+  int widest = 0;
+  for (int i = 1; i < nl; ++i) widest = s->widths[i] > widest ? s->widths[i] : widest;
+  p->buffers = nl > 2 ? 2 : nl - 1;
+  p->hidden = align256(static_cast<uint64_t>(m) * widest * 2);
+  p->pre = s->tail != GP_TAIL_NONE ? align256(static_cast<uint64_t>(m) * last * 4) : 0;
+  p->total = p->buffers * p->hidden + p->pre;
+  return GP_OK;
+}
+
+static int w4_mlp(const gp_mlp_spec* s, int group, int zero_points, int64_t m, const void* x,
+                  const void* const* packed, const void* const* b, const void* gamma, const void* beta,
+                  void* out, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  clear_error();
+  W4MlpPlan plan;
+  int rc = w4_mlp_plan(s, m, &plan);
+  if (rc != GP_OK) return rc;
+  if (m == 0) return GP_OK;  // empty tensors may come as NULL
+  const int nl = s->n_layers;
+  if (x == nullptr || out == nullptr || packed == nullptr)
+    return set_error(GP_ERR_ARG, "x, packed and out must not be NULL");
+  const bool normed = s->tail != GP_TAIL_NONE;
+  if (!aligned(x, 16) || !aligned(out, normed ? 16 : 2))
+    return set_error(GP_ERR_ALIGN, "x must be 16-byte aligned, out %d-byte", normed ? 16 : 2);
+  if (!aligned(gamma, 16) || !aligned(beta, 16)) return set_error(GP_ERR_ALIGN, "gamma and beta must be 16-byte aligned");
+  W4Layout l[GP_MAX_LAYERS];
+  const uint64_t xn = static_cast<uint64_t>(m) * s->widths[0] * 2, on = static_cast<uint64_t>(m) * s->widths[nl] * 2;
+  const uint64_t wn = static_cast<uint64_t>(workspace_bytes < 0 ? 0 : workspace_bytes);
+  for (int i = 0; i < nl; ++i) {
+    const gp_w4_spec w = {s->widths[i], s->widths[i + 1], group, s->dtype, zero_points};
+    rc = w4_layout(&w, &l[i]);
+    if (rc != GP_OK) return rc;
+    if (packed[i] == nullptr) return set_error(GP_ERR_ARG, "packed[%d] is NULL", i);
+    if (!aligned(packed[i], 16)) return set_error(GP_ERR_ALIGN, "packed[%d] must be 16-byte aligned", i);
+    const void* bi = b != nullptr ? b[i] : nullptr;
+    if (!aligned(bi, 2)) return set_error(GP_ERR_ALIGN, "b[%d] must be 2-byte aligned", i);
+    const uint64_t bn = static_cast<uint64_t>(s->widths[i + 1]) * 2;
+    if (overlap(out, on, packed[i], l[i].bytes) || overlap(out, on, bi, bn) ||
+        overlap(workspace, wn, packed[i], l[i].bytes) || overlap(workspace, wn, bi, bn))
+      return set_error(GP_ERR_ARG, "out or workspace overlaps layer %d's weights", i);
+  }
+  if (workspace_bytes < 0 || static_cast<uint64_t>(workspace_bytes) < plan.total || (plan.total > 0 && workspace == nullptr))
+    return set_error(GP_ERR_ARG, "workspace of %lld bytes, %llu needed", (long long)workspace_bytes,
+                     (unsigned long long)plan.total);
+  if (!aligned(workspace, 16)) return set_error(GP_ERR_ALIGN, "workspace must be 16-byte aligned");
+  // out may be x where the norm of the tail replaces it row by row
+  const bool in_place = normed && out == x && s->widths[0] == s->widths[nl];
+  const uint64_t gn = static_cast<uint64_t>(s->widths[nl]) * 2;
+  if ((overlap(out, on, x, xn) && !in_place) || overlap(workspace, wn, x, xn) || overlap(workspace, wn, out, on) ||
+      (normed && (overlap(out, on, gamma, gn) || overlap(out, on, beta, gn) || overlap(workspace, wn, gamma, gn) ||
+                  overlap(workspace, wn, beta, gn))))
+    return set_error(GP_ERR_ARG, "x, out, workspace, gamma and beta must not overlap");
+  char* ws = static_cast<char*>(workspace);
+  const void* in = x;
+  for (int i = 0; i < nl; ++i) {
+    const bool last = i + 1 == nl;
+    void* to = last ? (normed ? static_cast<void*>(ws + plan.buffers * plan.hidden) : out)
+                    : static_cast<void*>(ws + (plan.buffers == 2 ? (i & 1) : 0) * plan.hidden);
+    rc = w4_linear(l[i], s->dtype, m, last && normed ? GP_ACT_NONE : s->act[i], in, packed[i],
+                   b != nullptr ? b[i] : nullptr, to, last && normed, stream);
+    if (rc != GP_OK) return rc;
+    in = to;
+  }
+  if (!normed) return finish_launch(stream, 1, 0);
+  BlockNormArgs a{};
+  a.m = m;
+  a.width = s->widths[nl];
+  a.post = GP_NORM_NONE;
+  a.pre = GP_NORM_LAYER;
+  a.x_scale = a.y_scale = 1.0f;
+  a.pre_eps = s->ln_eps;
+  a.x = s->tail == GP_TAIL_RESIDUAL_LN ? x : nullptr;
+  a.y = in;
+  a.pre_gamma = gamma;
+  a.pre_beta = beta;
+  a.h = out;
+  rc = launch_block_norm(a, s->dtype, false, true, stream);
+  if (rc != GP_OK) return rc;
+  return finish_launch(stream, 1);
 }
 
 }  // namespace gp
@@ -846,6 +1080,122 @@ int gp_testmlp_out(int64_t m, const void* x, const void* w1, const void* b1, con
   const void* w[3] = {w1, w2, w3};
   const void* b[3] = {b1, b2, b3};
   return fused_mlp(&s, m, x, w, b, nullptr, nullptr, out, static_cast<cudaStream_t>(stream));
+}
+
+int gp_block_norm_out(const gp_block_norm_spec* spec, int64_t m, const void* x, const void* y,
+                      const void* gate, const void* post_gamma, const void* post_beta,
+                      const void* pre_gamma, const void* pre_beta, void* r, void* h, void* stream) {
+  return block_norm(spec, m, x, y, gate, post_gamma, post_beta, pre_gamma, pre_beta, r, h,
+                    static_cast<cudaStream_t>(stream));
+}
+
+int64_t gp_w4_packed_bytes(const gp_w4_spec* spec) {
+  clear_error();
+  W4Layout l;
+  const int rc = w4_layout(spec, &l);
+  return rc == GP_OK ? l.bytes : rc;
+}
+
+static uint64_t w4_groups(const W4Layout& l) { return static_cast<uint64_t>((l.k + l.group - 1) / l.group) * l.n; }
+
+int gp_w4_quantize_out(const gp_w4_spec* spec, const void* w, void* packed, void* stream) {
+  clear_error();
+  W4Layout l;
+  int rc = w4_layout(spec, &l);
+  if (rc != GP_OK) return rc;
+  if (w == nullptr) return set_error(GP_ERR_ARG, "w is NULL");
+  const W4Buf bufs[1] = {{w, static_cast<uint64_t>(l.k) * l.n * 2, 2, "w"}};
+  rc = w4_check(l, packed, bufs, 1);
+  if (rc != GP_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = launch_w4_quantize(l, spec->dtype, w, packed, s);
+  return rc == GP_OK ? finish_launch(s, 1) : rc;
+}
+
+int gp_w4_pack_out(const gp_w4_spec* spec, const uint8_t* codes, const void* scales, const uint8_t* zeros,
+                   void* packed, void* stream) {
+  clear_error();
+  W4Layout l;
+  int rc = w4_layout(spec, &l);
+  if (rc != GP_OK) return rc;
+  if (codes == nullptr || scales == nullptr) return set_error(GP_ERR_ARG, "codes and scales must not be NULL");
+  if ((zeros != nullptr) != (l.zeros != 0)) return set_error(GP_ERR_ARG, "zeros goes with zero_points");
+  const W4Buf bufs[3] = {{codes, static_cast<uint64_t>(l.k) * l.n, 1, "codes"},
+                         {scales, w4_groups(l) * 2, 2, "scales"},
+                         {zeros, w4_groups(l), 1, "zeros"}};
+  rc = w4_check(l, packed, bufs, 3);
+  if (rc != GP_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = launch_w4_pack(l, spec->dtype, codes, scales, zeros, packed, s);
+  return rc == GP_OK ? finish_launch(s, 1) : rc;
+}
+
+int gp_w4_unpack_out(const gp_w4_spec* spec, const void* packed, uint8_t* codes, void* scales, uint8_t* zeros,
+                     void* stream) {
+  clear_error();
+  W4Layout l;
+  int rc = w4_layout(spec, &l);
+  if (rc != GP_OK) return rc;
+  if (codes == nullptr && scales == nullptr && zeros == nullptr)
+    return set_error(GP_ERR_ARG, "codes, scales and zeros are all NULL");
+  if (zeros != nullptr && !l.zeros) return set_error(GP_ERR_ARG, "weights without zero points");
+  const W4Buf bufs[3] = {{codes, static_cast<uint64_t>(l.k) * l.n, 1, "codes"},
+                         {scales, w4_groups(l) * 2, 2, "scales"},
+                         {zeros, w4_groups(l), 1, "zeros"}};
+  rc = w4_check(l, packed, bufs, 3);
+  if (rc != GP_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = launch_w4_unpack(l, spec->dtype, packed, codes, scales, zeros, s);
+  return rc == GP_OK ? finish_launch(s, 1) : rc;
+}
+
+int gp_w4_dequantize_out(const gp_w4_spec* spec, const void* packed, void* w, void* stream) {
+  clear_error();
+  W4Layout l;
+  int rc = w4_layout(spec, &l);
+  if (rc != GP_OK) return rc;
+  if (w == nullptr) return set_error(GP_ERR_ARG, "w is NULL");
+  const W4Buf bufs[1] = {{w, static_cast<uint64_t>(l.k) * l.n * 2, 2, "w"}};
+  rc = w4_check(l, packed, bufs, 1);
+  if (rc != GP_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = launch_w4_dequantize(l, spec->dtype, packed, w, s);
+  return rc == GP_OK ? finish_launch(s, 1) : rc;
+}
+
+int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, const void* packed,
+                     const void* bias, void* out, void* stream) {
+  clear_error();
+  W4Layout l;
+  int rc = w4_layout(spec, &l);
+  if (rc != GP_OK) return rc;
+  if (m < 0) return set_error(GP_ERR_ARG, "m = %lld is negative", (long long)m);
+  if (m >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "m = %lld exceeds 2^31-1", (long long)m);
+  if (act < GP_ACT_NONE || act > GP_ACT_SIGMOID) return set_error(GP_ERR_ARG, "act %d unknown", act);
+  if (m == 0) return GP_OK;  // empty tensors may come as NULL
+  if (x == nullptr || out == nullptr) return set_error(GP_ERR_ARG, "x and out must not be NULL");
+  const W4Buf bufs[3] = {{x, static_cast<uint64_t>(m) * l.k * 2, 16, "x"},
+                         {out, static_cast<uint64_t>(m) * l.n * 2, 2, "out"},
+                         {bias, static_cast<uint64_t>(l.n) * 2, 2, "bias"}};
+  rc = w4_check(l, packed, bufs, 3);
+  if (rc != GP_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = w4_linear(l, spec->dtype, m, act, x, packed, bias, out, false, s);
+  return rc == GP_OK ? finish_launch(s, 1, 0) : rc;
+}
+
+int gp_w4_mlp_out(const gp_mlp_spec* spec, int group, int zero_points, int64_t m, const void* x,
+                  const void* const* packed, const void* const* b, const void* gamma, const void* beta,
+                  void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+  return w4_mlp(spec, group, zero_points, m, x, packed, b, gamma, beta, out, workspace, workspace_bytes,
+                static_cast<cudaStream_t>(stream));
+}
+
+int64_t gp_w4_mlp_workspace_bytes(const gp_mlp_spec* spec, int64_t m) {
+  clear_error();
+  W4MlpPlan p;
+  const int rc = w4_mlp_plan(spec, m, &p);
+  return rc == GP_OK ? static_cast<int64_t>(p.total) : rc;
 }
 
 const char* gp_last_error(void) { return t_last_error.c_str(); }

@@ -254,6 +254,94 @@ GP_API int gp_fused_mlp_host(const gp_mlp_spec* spec, int64_t m, const void* x_h
                       const void* beta, void* out_host, int64_t chunk_rows, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Norms around a block, and layers with 4-bit weights, for serving transformer blocks next to the
+ * chains above. No reference counterpart.
+ *   Shared rules: every buffer is contiguous; sums, statistics and activations are fp32 and each
+ *   output is rounded once; nothing is allocated and no library workspace is used, so a call may be
+ *   captured into a CUDA graph without an eager call before it, and calls on different streams or
+ *   replays of different graphs may overlap as long as their own buffers do not. Inputs and outputs
+ *   that overlap without being named as allowed return GP_ERR_ARG.
+ * ------------------------------------------------------------------------------------------- */
+typedef enum gp_norm {
+  GP_NORM_NONE = 0,
+  GP_NORM_LAYER = 1,  /* (v - mean) / sqrt(mean((v - mean)^2) + eps) * gamma + beta */
+  GP_NORM_RMS = 2     /* v / sqrt(mean(v^2) + eps) * gamma + beta */
+} gp_norm;
+
+/* r = x_scale x + y_scale gate (.) Npost(y),  h = Npre(r), row by row. */
+typedef struct gp_block_norm_spec {
+  int width;          /* H: a multiple of 8, at most 32768 */
+  int dtype;          /* gp_dtype T of h, gate, gammas, betas, and of x / r / y unless fp32 */
+  int stream_f32;     /* x and r are fp32 (a residual stream kept in 32 bits) */
+  int y_f32;          /* y is fp32 */
+  int post;           /* gp_norm of the block's output y */
+  int pre;            /* gp_norm of the new stream, before the next block */
+  float post_eps, pre_eps;
+  float x_scale, y_scale;
+  int64_t gate_rows;  /* rows that share a row of gate: row i uses gate row i / gate_rows; 0: one
+                         gate row for all */
+} gp_block_norm_spec;
+
+/* x [m, H] (the stream; NULL: r = y_scale gate Npost(y)), y [m, H] (the block's output; NULL: r =
+ * x_scale x, and then post must be GP_NORM_NONE and gate NULL), gate [ceil(m / gate_rows), H] or NULL,
+ * gammas and betas [H] or NULL (1 / 0), r [m, H] or NULL (not stored), h [m, H] or NULL (not computed;
+ * with pre GP_NORM_NONE it is r in T). h is computed from the unrounded r.
+ * r may be x (in place) or y, h may be x or y, where the element types match; r and h are distinct.
+ * All pointers 16-byte aligned. */
+GP_API int gp_block_norm_out(const gp_block_norm_spec* spec, int64_t m, const void* x, const void* y,
+                             const void* gate, const void* post_gamma, const void* post_beta,
+                             const void* pre_gamma, const void* pre_beta, void* r, void* h, void* stream);
+
+/* Weights [K, N] (row-major, as for the chains) in 4 bits with group scales along K:
+ *   W[k][n] = s[k / G][n] (q[k][n] - z[k / G][n]),  q in 0..15,  s in T,  z in 0..15 (8 without zero points).
+ * K is a multiple of 8 up to 65536, N is 1 .. 2^24, G is 32, 64 or 128 (the last group may be short). */
+typedef struct gp_w4_spec {
+  int64_t k, n;
+  int group;       /* G */
+  int dtype;       /* gp_dtype T: the type of the scales, and of what the weights multiply */
+  int zero_points; /* nonzero: z is stored per group and column */
+} gp_w4_spec;
+
+/* Bytes of the packed form (codes in the products' order, then scales); negative: gp_status. */
+GP_API int64_t gp_w4_packed_bytes(const gp_w4_spec* spec);
+
+/* Quantises w [K, N] (T). Without zero points s = T(max|w| / 7) and q = clamp(rint(w / s), -8, 7) + 8;
+ * with them, lo = min(w, 0), hi = max(w, 0), s = T((hi - lo) / 15), z = clamp(rint(-lo / s), 0, 15) and
+ * q = clamp(rint(w / s) + z, 0, 15). rint rounds half to even. A group whose s rounds to 0 stands for
+ * zeros; one with a NaN or an infinity gets a scale that is not finite. packed: 16-byte aligned,
+ * gp_w4_packed_bytes(spec) long. w: 2-byte aligned. */
+GP_API int gp_w4_quantize_out(const gp_w4_spec* spec, const void* w, void* packed, void* stream);
+
+/* Packs weights quantised elsewhere: codes [K, N] (one per byte, the low four bits count), scales
+ * [ceil(K / G), N] (T), zeros [ceil(K / G), N] (bytes 0..15; NULL without zero points). */
+GP_API int gp_w4_pack_out(const gp_w4_spec* spec, const uint8_t* codes, const void* scales,
+                          const uint8_t* zeros, void* packed, void* stream);
+
+/* The reverse of gp_w4_pack_out; each of codes, scales and zeros may be NULL (not wanted). */
+GP_API int gp_w4_unpack_out(const gp_w4_spec* spec, const void* packed, uint8_t* codes, void* scales,
+                            uint8_t* zeros, void* stream);
+
+/* w [K, N] (T) = s (q - z), rounded once. */
+GP_API int gp_w4_dequantize_out(const gp_w4_spec* spec, const void* packed, void* w, void* stream);
+
+/* out [m, N] = act(x [m, K] W + bias) on packed weights, T; bias [N] or NULL; act a gp_act. Made for
+ * few rows, where the weights' bytes are the time; any m works. x 16-byte, out and bias 2-byte aligned. */
+GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, const void* packed,
+                            const void* bias, void* out, void* stream);
+
+/* A chain of layers (gp_mlp_spec) on packed weights: widths of any multiple of 8 (the last one any
+ * N without a tail), every activation and tail, no skip layer. Layer l is packed[l], a gp_w4_spec of
+ * widths[l] x widths[l + 1], the group and zero_points given here and the spec's dtype. Hidden
+ * activations are rounded to T; the last layer goes into a LayerNorm tail in fp32. workspace: caller's,
+ * 16-byte aligned, at least gp_w4_mlp_workspace_bytes(spec, m) long (0 bytes: NULL is fine), free for
+ * other use once the call's work has run. gamma and beta 16-byte aligned. */
+GP_API int gp_w4_mlp_out(const gp_mlp_spec* spec, int group, int zero_points, int64_t m, const void* x,
+                         const void* const* packed, const void* const* b, const void* gamma,
+                         const void* beta, void* out, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+GP_API int64_t gp_w4_mlp_workspace_bytes(const gp_mlp_spec* spec, int64_t m);
+
+/* ---------------------------------------------------------------------------------------------
  * Diagnostics and control (no reference counterpart: the reference has no error reporting).
  * ------------------------------------------------------------------------------------------- */
 /* Message describing the last error on this thread ("" if none). */
