@@ -1,20 +1,23 @@
 // Products with 4-bit weights for few rows: out [m, N] = act(x [m, K] W + b), W = s (q - z) (w4.cuh).
 //
-// With few rows the time is the weights' bytes (half a byte each), so the kernel is a stream over
-// the packed codes. The matrix instruction is mma.sync m16n8k16 with the WEIGHTS as its 16-row
-// operand (16 columns of W) and up to 8 rows of x as its 8-column operand: a warp turns 1,024
-// weights into instruction operands with about 1.3 integer and half instructions each, one to
-// eight rows cost the same, and the sums are fp32. (tcgen05 takes its weights from shared memory,
-// which for so few rows only adds a store and a load per weight.) The codes enter as the exact
-// integers q - z; the group's scale multiplies the fp32 sum of its 32 or 64 products, so no weight
-// is rounded.
+// With few rows the time is the weights' bytes (half a byte each), and what stands between them and
+// the memory's rate is the number of instructions per weight. So:
+//   - The matrix instruction is mma.sync m16n8k16 with the WEIGHTS as its 16-row operand (16 columns
+//     of W) and up to 8 rows of x as its 8-column operand; one to eight rows cost the same and the
+//     sums are fp32. (tcgen05 takes 16-bit weights from shared memory, which for so few rows only
+//     adds a store and a load per weight.)
+//   - A code becomes an operand with one mask (w4.cuh): the operand is q plus a constant, scaled by a
+//     power of two. sum_k x (q - z) = sum_k x (q + c) - (c + z) sum_k x, and the second term starts
+//     the accumulator; the sums of x over each group are taken once per CTA. The group's scale
+//     multiplies the fp32 sum, so no weight is rounded. A first form that subtracted z from each
+//     weight, took codes through a cp.async ring and divided to find the group ran 174 instructions
+//     per 1,024 weights and 57 us at 1 x 8192 x 28672.
 //
 //   - A CTA of 16 warps owns a slice of K (one of `ck` CTAs of a cluster does; ck = 1: all of it),
 //     keeps its part of the x rows in shared memory and goes over column tiles of 16. `ws` warps
-//     share a tile, each taking every ws-th 64-row block, so together they read whole stretches.
-//   - Every lane copies its own 16 bytes of codes (and its scales) into a private ring of kDepth
-//     slots with cp.async and reads back only what it copied: the ring needs no barrier, and the
-//     loads of the next tiles are in flight while the sums of this one are joined.
+//     share a tile, each taking every ws-th 128-row block, so together they read whole stretches.
+//   - The codes of the next few blocks are in flight in registers, across tiles: the loads go on
+//     while the warps' sums are joined.
 //   - The warps' sums are joined in shared memory, the CTAs' through distributed shared memory,
 //     both in a fixed order: results do not depend on timing.
 #include <climits>
@@ -28,9 +31,9 @@ namespace {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kDepth = 8;           // ring slots per warp
 constexpr int kPartStride = 20;     // floats per row of a warp's 16 x rows sums: conflict-free float2 stores
 constexpr int kMaxCluster = 8;
+constexpr int kZeroBytes = 256;     // zeros in shared memory, read in place of absent x rows
 
 struct W4RowsArgs {
   W4Layout l;
@@ -41,7 +44,7 @@ struct W4RowsArgs {
   int64_t m;
   int act;
   int ck;            // CTAs of a cluster, along K
-  int slice;         // 64-row blocks of a CTA
+  int slice;         // k-blocks of a CTA
   int ws;            // warps that share a column tile
   int iters;         // column tile groups per cluster
   int rows;          // x rows of a pass (at most 8 TT)
@@ -73,35 +76,48 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+// Codes and scales are read once: past L1.
+__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int W>
+__device__ __forceinline__ void ldg_words(const void* p, uint32_t (&v)[W]) {
+  if constexpr (W == 1) {
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+  } else if constexpr (W == 2) {
+    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+      asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+                   : "l"(static_cast<const uint32_t*>(p) + i));
+  }
+}
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-// TT: tiles of 8 x rows. UNIT: rows of W per scale step (32 or 64; groups of 128 use 64).
-template <typename T, int TT, int UNIT, bool ZP, typename OutT>
+// TT: tiles of 8 x rows. UNITS: groups per k-block of 128.
+template <typename T, int TT, int UNITS, bool ZP, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_constant__ W4RowsArgs a) {
-  constexpr int kUnits = 64 / UNIT;
-  constexpr int kScale = ZP ? 8 : 4;                          // bytes of scales per lane and unit
-  constexpr int kSlot = 32 * (16 + kUnits * kScale);          // bytes of a ring slot
+  constexpr int kWords = UNITS * (ZP ? 2 : 1);                // scale words of a lane per block
   constexpr int kPart = TT * 8 * kPartStride;                 // floats of a warp's sums
+  constexpr int kDepth = kWords >= 8 ? 3 : 4;                 // blocks in flight per warp (registers)
+  constexpr float kUnit0 = W4Deq<T>::unit(0), kUnit1 = W4Deq<T>::unit(1);
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* ring = smem;                                       // [kWarps][kDepth][kSlot]
-  float* part = reinterpret_cast<float*>(ring + kWarps * kDepth * kSlot);  // [2][kWarps][kPart]
-  float* red = part + 2 * kWarps * kPart;                     // [2][TT * 128 * kWarps / ws] at most, clusters only
+  float* part = reinterpret_cast<float*>(smem);               // [2][kWarps][kPart]
   const int np = kWarps / a.ws;                               // tiles at a time
   const int outs = np * TT * 128;                             // sums of a tile group
-  uint8_t* xs = reinterpret_cast<uint8_t*>(red + (a.ck > 1 ? 2 * outs : 0));
+  float* red = part + 2 * kWarps * kPart;                     // [2][outs], clusters only
+  float* xsum = red + (a.ck > 1 ? 2 * outs : 0);              // [slice * UNITS][8 TT]
+  uint8_t* zeros = reinterpret_cast<uint8_t*>(xsum + a.slice * UNITS * 8 * TT);
+  uint8_t* xs = zeros + kZeroBytes;                           // [rows][x_stride]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = a.ck > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -109,143 +125,155 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * a.rows;
   const int rows = static_cast<int>(a.m - row0 < a.rows ? a.m - row0 : a.rows);
   const int b0 = rank * a.slice;
-  const int nb = min(a.slice, a.l.k_blocks - b0);             // blocks of this CTA (may be <= 0)
+  const int nb = min(a.slice, a.l.blocks - b0);               // blocks of this CTA
   const int sub = warp % a.ws, slot_tile = warp / a.ws;
   const int steps = (a.slice + a.ws - 1) / a.ws;              // blocks of a warp per tile
 
-  const uint8_t* codes = static_cast<const uint8_t*>(a.packed);
-  const uint8_t* scales = codes + a.l.scale_off;
-  const uint32_t my_ring = smem_u32(ring) + warp * (kDepth * kSlot);
-
-  // the step that is loaded next: tile group it_i, block b_i of this warp's
-  int it_i = 0, b_i = 0;
-  auto src = [&](int it, int b, const uint8_t*& c, const uint8_t*& s) {
-    const int tile = (cluster + it * clusters) * np + slot_tile;
-    const int rel = sub + b * a.ws;
-    if (it >= a.iters || tile >= a.l.n_tiles || rel >= nb) return false;
-    const int blk = b0 + rel;
-    c = codes + (static_cast<int64_t>(tile) * a.l.k_blocks + blk) * 512 + lane * 16;
-    s = scales + (static_cast<int64_t>(tile) * a.l.groups + blk * 64 / a.l.group) * (8 * kScale) + g * kScale;
-    return true;
-  };
-  auto issue = [&](int slot) {
-    const uint8_t *c, *s;
-    if (src(it_i, b_i, c, s)) {
-      const uint32_t d = my_ring + slot * kSlot;
-      cp_async<16>(d + lane * 16, c);
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) cp_async<kScale>(d + 512 + (u * 32 + lane) * kScale, s + u * 8 * kScale);
+  // the block that is loaded next: tile and block (relative to the slice) of this warp's
+  int ld_tile = cluster * np + slot_tile, ld_rel = sub, ld_b = 0;
+  const int tile_step = clusters * np;
+  const uint8_t* codes = static_cast<const uint8_t*>(a.packed) +
+                         (static_cast<int64_t>(ld_tile) * a.l.blocks + b0 + sub) * kW4BlockBytes + lane * 16;
+  const uint8_t* scales = static_cast<const uint8_t*>(a.packed) + a.l.scale_off +
+                          (static_cast<int64_t>(ld_tile) * a.l.blocks + b0 + sub) * (32 * kWords) + g * (4 * kWords);
+  const int64_t back = static_cast<int64_t>(tile_step) * a.l.blocks - static_cast<int64_t>(steps) * a.ws;
+  auto advance = [&] {
+    codes += a.ws * kW4BlockBytes;
+    scales += a.ws * (32 * kWords);
+    ld_rel += a.ws;
+    if (++ld_b == steps) {
+      ld_b = 0;
+      ld_rel = sub;
+      ld_tile += tile_step;
+      codes += back * kW4BlockBytes;
+      scales += back * (32 * kWords);
     }
-    cp_commit();
-    if (++b_i == steps) b_i = 0, ++it_i;
   };
 
   // The first codes go into L2 while the previous kernel of the stream drains (a hint: nothing is
   // read into the program before the wait).
-  {
-    const uint8_t *c, *s;
-    for (int i = 0, it = 0, b = 0; i < kDepth; ++i) {
-      if ((lane & 7) == 0 && src(it, b, c, s)) asm volatile("prefetch.global.L2 [%0];" ::"l"(c));
-      if (++b == steps) b = 0, ++it;
-    }
-  }
+  if (ld_tile < a.l.n_tiles)
+    for (int i = 0; i < kDepth && i < steps && sub + i * a.ws < nb; ++i)
+      if ((lane & 7) == 0) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes + i * a.ws * kW4BlockBytes));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes + i * a.ws * kW4BlockBytes + kW4BlockBytes / 2));
+      }
   pdl_wait_prior();
   pdl_launch_dependents();
-#pragma unroll
-  for (int i = 0; i < kDepth - 1; ++i) issue(i);
 
-  // x rows of this CTA's slice; zero past K
+  uint4 cbuf[kDepth][2];
+  uint32_t sbuf[kDepth][kWords];
+  auto load = [&](int p) {
+    if (ld_tile < a.l.n_tiles && ld_rel < nb) {
+      cbuf[p][0] = ldg_stream(codes);
+      cbuf[p][1] = ldg_stream(codes + kW4BlockBytes / 2);
+      ldg_words<kWords>(scales, sbuf[p]);
+    }
+    advance();
+  };
+#pragma unroll
+  for (int p = 0; p < kDepth; ++p) load(p);
+
+  // x rows of this CTA's slice (zero past K) and their sums over each group. Sixteen lanes hold a
+  // block of a row; absent rows have sums of zero and are read from the zeros.
+  if (threadIdx.x < kZeroBytes / 16) reinterpret_cast<uint4*>(zeros)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   {
-    const int chunks = a.slice * 8;  // 16-byte pieces of a row
-    for (int i = threadIdx.x; i < rows * chunks; i += kThreads) {
-      const int r = i / chunks, c = i % chunks;
-      const int k = b0 * 64 + c * 8;
+    const int pieces = a.slice * 16;  // 16-byte pieces of a row
+    for (int i = threadIdx.x; i < (8 * TT - rows) * a.slice * UNITS; i += kThreads) {
+      const int dead = 8 * TT - rows;
+      xsum[i / dead * (8 * TT) + rows + i % dead] = 0.0f;
+    }
+    for (int i0 = 0; i0 < rows * pieces; i0 += kThreads) {
+      const int i = i0 + threadIdx.x;
+      const int r = i / pieces, c = i % pieces;
+      const int k = b0 * kW4Block + c * 8;
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (k < a.l.k) v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (row0 + r) * a.l.k + k);
-      *reinterpret_cast<uint4*>(xs + r * a.x_stride + c * 16) = v;
+      if (r < rows && k < a.l.k) v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (row0 + r) * a.l.k + k);
+      if (r < rows) *reinterpret_cast<uint4*>(xs + r * a.x_stride + c * 16) = v;
+      const float2 f0 = Elem<T>::unpack(v.x), f1 = Elem<T>::unpack(v.y), f2 = Elem<T>::unpack(v.z), f3 = Elem<T>::unpack(v.w);
+      float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+#pragma unroll
+      for (int o = 1; o < 16 / UNITS; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (r < rows && c % (16 / UNITS) == 0) xsum[(c / (16 / UNITS)) * (8 * TT) + r] = sum;
     }
   }
   __syncthreads();
   // every CTA of the cluster runs before one writes into another's shared memory
   if (a.ck > 1) cluster_sync_all();
 
-  const uint8_t* xr[TT];
-  bool live[TT];
+  uint32_t xr[TT], xmask[TT];
 #pragma unroll
   for (int i = 0; i < TT; ++i) {
-    live[i] = i * 8 + g < rows;
-    xr[i] = xs + (live[i] ? i * 8 + g : 0) * a.x_stride + t * 16;
+    const bool live = i * 8 + g < rows;
+    xr[i] = smem_u32(live ? xs + (i * 8 + g) * a.x_stride : zeros) + t * 16;
+    xmask[i] = live ? 0xffffffffu : 0u;
   }
 
-  int slot = 0;
-  for (int it = 0; it < a.iters; ++it) {
-    float acc[TT][4];
+  float acc[TT][4];
+  auto compute = [&](int p, int rel) {
 #pragma unroll
-    for (int i = 0; i < TT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-    const int tile0 = (cluster + it * clusters) * np;
-    const bool has_tile = tile0 + slot_tile < a.l.n_tiles;
-    for (int b = 0; b < steps; ++b) {
-      issue((slot + kDepth - 1) % kDepth);
-      cp_wait<kDepth - 1>();
-      const int rel = sub + b * a.ws;
-      if (has_tile && rel < nb) {
-        const uint32_t d = my_ring + slot * kSlot;
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(d + lane * 16) : "memory");
-        float sum[TT][4];
+    for (int u = 0; u < UNITS; ++u) {
+      float sum[TT][4];
+      const float2 s = Elem<T>::unpack(sbuf[p][ZP ? 2 * u : u]);
+      float2 z = make_float2(-8.0f - W4Deq<T>::kOffset, -8.0f - W4Deq<T>::kOffset);
+      if constexpr (ZP) {
+        z = Elem<T>::unpack(sbuf[p][2 * u + 1]);
+        z.x = -W4Deq<T>::kOffset - z.x;
+        z.y = -W4Deq<T>::kOffset - z.y;
+      }
+      z.x *= kUnit0;
+      z.y *= kUnit1;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int u = h * kUnits / 2;
-          uint32_t s01, z01 = 0, c0 = W4Deq<T>::kC0, c1 = W4Deq<T>::kC1;
-          if constexpr (ZP) {
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(s01), "=r"(z01)
-                         : "r"(d + 512 + (u * 32 + lane) * kScale) : "memory");
-            W4Deq<T>::consts(z01, c0, c1);
-          } else {
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(s01) : "r"(d + 512 + (u * 32 + lane) * kScale) : "memory");
-          }
-          if (kUnits == 2 || h == 0)
+      for (int i = 0; i < TT; ++i) {
+        const float2 xv = *reinterpret_cast<const float2*>(xsum + (rel * UNITS + u) * (8 * TT) + i * 8 + 2 * t);
+        sum[i][0] = z.x * xv.x;
+        sum[i][1] = z.x * xv.y;
+        sum[i][2] = z.y * xv.x;
+        sum[i][3] = z.y * xv.y;
+      }
 #pragma unroll
-            for (int i = 0; i < TT; ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.0f;
-          uint32_t p0[4], p1[4];
-          W4Deq<T>::pairs(w[2 * h], c0, c1, p0);
-          W4Deq<T>::pairs(w[2 * h + 1], c0, c1, p1);
+      for (int h = u * (4 / UNITS); h < (u + 1) * (4 / UNITS); ++h) {  // 32 rows at a time
+        const uint4 c = cbuf[p][h >> 1];
+        uint32_t p0[4], p1[4];
+        W4Deq<T>::pairs((h & 1) ? c.z : c.x, p0);
+        W4Deq<T>::pairs((h & 1) ? c.w : c.y, p1);
 #pragma unroll
-          for (int i = 0; i < TT; ++i) {
-            uint4 xv = make_uint4(0, 0, 0, 0);
-            if (live[i]) xv = *reinterpret_cast<const uint4*>(xr[i] + rel * 128 + h * 64);
-            mma16816<T>(sum[i], p0, xv.x, xv.y);
-            mma16816<T>(sum[i], p1, xv.z, xv.w);
-          }
-          if (kUnits == 2 || h == 1) {
-            const float2 s = Elem<T>::unpack(s01);
-#pragma unroll
-            for (int i = 0; i < TT; ++i) {
-              acc[i][0] = fmaf(s.x, sum[i][0], acc[i][0]);
-              acc[i][1] = fmaf(s.x, sum[i][1], acc[i][1]);
-              acc[i][2] = fmaf(s.y, sum[i][2], acc[i][2]);
-              acc[i][3] = fmaf(s.y, sum[i][3], acc[i][3]);
-            }
-          }
+        for (int i = 0; i < TT; ++i) {
+          uint32_t x0, x1, x2, x3;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x0), "=r"(x1), "=r"(x2), "=r"(x3)
+                       : "r"(xr[i] + (static_cast<uint32_t>(rel * (kW4Block * 2)) & xmask[i]) + h * 64) : "memory");
+          mma16816<T>(sum[i], p0, x0, x1);
+          mma16816<T>(sum[i], p1, x2, x3);
         }
       }
-      slot = slot + 1 == kDepth ? 0 : slot + 1;
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        acc[i][0] = fmaf(s.x, sum[i][0], acc[i][0]);
+        acc[i][1] = fmaf(s.x, sum[i][1], acc[i][1]);
+        acc[i][2] = fmaf(s.y, sum[i][2], acc[i][2]);
+        acc[i][3] = fmaf(s.y, sum[i][3], acc[i][3]);
+      }
     }
+  };
+
+  auto join = [&](int it) {
+    const int tile0 = (cluster + it * clusters) * np;
     // join: part[warp][row][column]; a buffer is written again two groups on, after the next
     // group's barrier, when everyone has read it
     float* pb = part + (it & 1) * (kWarps * kPart);
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
       float* p = pb + warp * kPart + (i * 8 + 2 * t) * kPartStride + 2 * g;
-      *reinterpret_cast<float2*>(p) = make_float2(acc[i][0], acc[i][2]);
-      *reinterpret_cast<float2*>(p + kPartStride) = make_float2(acc[i][1], acc[i][3]);
+      *reinterpret_cast<float2*>(p) = make_float2(acc[i][0] * (1.0f / kUnit0), acc[i][2] * (1.0f / kUnit1));
+      *reinterpret_cast<float2*>(p + kPartStride) = make_float2(acc[i][1] * (1.0f / kUnit0), acc[i][3] * (1.0f / kUnit1));
     }
     __syncthreads();
     auto warps_sum = [&](int o) {
       const int tl = o / (TT * 128), r = (o >> 4) % (TT * 8), n = o & 15;
       const float* p = pb + tl * a.ws * kPart + r * kPartStride + n;
       float v = 0.0f;
+#pragma unroll 4
       for (int i = 0; i < a.ws; ++i) v += p[i * kPart];
       return v;
     };
@@ -283,23 +311,47 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
         finish(oo, v);
       }
     }
+  };
+
+  auto clear = [&] {
+#pragma unroll
+    for (int i = 0; i < TT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+  };
+  clear();
+  int it = 0, b = 0, rel = sub, tile = cluster * np + slot_tile;
+  while (it < a.iters) {
+#pragma unroll
+    for (int p = 0; p < kDepth; ++p) {
+      if (it < a.iters) {
+        if (tile < a.l.n_tiles && rel < nb) compute(p, rel);
+        load(p);
+        rel += a.ws;
+        if (++b == steps) {
+          join(it);
+          clear();
+          b = 0;
+          rel = sub;
+          tile += tile_step;
+          ++it;
+        }
+      }
+    }
   }
-  // cp.async copies still in flight are none: every group past the last step is empty
 }
 
-constexpr int rows_slot(int units, bool zp) { return 32 * (16 + units * (zp ? 8 : 4)); }
+int rows_x_stride(int slice) { return slice * (kW4Block * 2) + 64; }  // conflict-free: 64 past a multiple of 128
 
-// Shared memory of a CTA: ring, warps' sums, clusters' sums, x rows
-int64_t rows_smem(int tt, int units, bool zp, int ck, int ws, int rows, int x_stride) {
+// Shared memory of a CTA: warps' sums, clusters' sums, group sums of x, zeros, x rows
+int64_t rows_smem(int tt, int units, int ck, int ws, int slice, int rows) {
   const int64_t outs = static_cast<int64_t>(kWarps / ws) * tt * 128;
-  return static_cast<int64_t>(kWarps) * kDepth * rows_slot(units, zp) + 2ll * kWarps * tt * 8 * kPartStride * 4 +
-         (ck > 1 ? 2 * outs * 4 : 0) + static_cast<int64_t>(rows) * x_stride;
+  return 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) + 32ll * slice * units * tt +
+         kZeroBytes + static_cast<int64_t>(rows) * rows_x_stride(slice);
 }
 
-template <typename T, int TT, int UNIT, bool ZP, typename OutT>
+template <typename T, int TT, int UNITS, bool ZP, typename OutT>
 int rows_launch(const W4RowsArgs& a, int smem, int clusters, int64_t row_tiles, cudaStream_t s, const PdlIo& io) {
   static unsigned long long done_mask = 0;
-  auto kern = &w4_rows_kernel<T, TT, UNIT, ZP, OutT>;
+  auto kern = &w4_rows_kernel<T, TT, UNITS, ZP, OutT>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kSmemLimit, &done_mask);
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -330,13 +382,17 @@ int rows_launch(const W4RowsArgs& a, int smem, int clusters, int64_t row_tiles, 
   return e == cudaSuccess ? GP_OK : set_error(GP_ERR_CUDA, "w4 linear launch: %s", cudaGetErrorString(e));
 }
 
+template <typename T, int TT, int UNITS, typename OutT>
+int rows_zeros(const W4RowsArgs& a, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return a.l.zeros ? rows_launch<T, TT, UNITS, true, OutT>(a, smem, clusters, rt, s, io)
+                   : rows_launch<T, TT, UNITS, false, OutT>(a, smem, clusters, rt, s, io);
+}
+
 template <typename T, int TT, typename OutT>
 int rows_dispatch(const W4RowsArgs& a, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  if (a.l.group == 32)
-    return a.l.zeros ? rows_launch<T, TT, 32, true, OutT>(a, smem, clusters, rt, s, io)
-                     : rows_launch<T, TT, 32, false, OutT>(a, smem, clusters, rt, s, io);
-  return a.l.zeros ? rows_launch<T, TT, 64, true, OutT>(a, smem, clusters, rt, s, io)
-                   : rows_launch<T, TT, 64, false, OutT>(a, smem, clusters, rt, s, io);
+  return a.l.units == 1   ? rows_zeros<T, TT, 1, OutT>(a, smem, clusters, rt, s, io)
+         : a.l.units == 2 ? rows_zeros<T, TT, 2, OutT>(a, smem, clusters, rt, s, io)
+                          : rows_zeros<T, TT, 4, OutT>(a, smem, clusters, rt, s, io);
 }
 
 template <typename T, typename OutT>
@@ -356,7 +412,6 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
   a.bias = bias;
   a.out = out;
   a.act = act;
-  const int units = l.group == 32 ? 2 : 1;
   // Split of the work: ck CTAs of a cluster along K, ws warps per column tile. A tile group costs
   // its warps' blocks plus a join (about one block's time within a CTA, about three more across a
   // cluster); the fewest rounds of that over the GPU's SMs win. A pass takes up to 16 rows, fewer
@@ -366,11 +421,11 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
     const int rows = static_cast<int>(m < per_pass ? m : per_pass), tt = per_pass > 8 ? 2 : 1;
     int64_t best = LLONG_MAX;
     for (int ck = 1; ck <= kMaxCluster; ck *= 2) {
-      const int slice = (l.k_blocks + ck - 1) / ck;
-      if (ck > 1 && (ck - 1) * slice >= l.k_blocks) break;  // a CTA without work
+      const int slice = (l.blocks + ck - 1) / ck;
+      if (ck > 1 && (ck - 1) * slice >= l.blocks) break;  // a CTA without work
       for (int ws = 1; ws <= kWarps; ws *= 2) {
         if (ws > 1 && ws / 2 >= slice) break;
-        if (rows_smem(tt, units, l.zeros != 0, ck, ws, rows, slice * 128 + 64) > kSmemLimit) continue;
+        if (rows_smem(tt, l.units, ck, ws, slice, rows) > kSmemLimit) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
         const int clusters = groups < sm_count / ck ? groups : sm_count / ck;
         const int64_t iters = (groups + clusters - 1) / clusters;
@@ -387,10 +442,10 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
     if (per_pass == 1) return set_error(GP_ERR_UNSUPPORTED, "w4 linear: K = %d", l.k);
   }
   a.rows = per_pass;
-  a.x_stride = a.slice * 128 + 64;
+  a.x_stride = rows_x_stride(a.slice);
   const int tt = per_pass > 8 ? 2 : 1;
-  const int smem = static_cast<int>(rows_smem(tt, units, l.zeros != 0, a.ck, a.ws,
-                                              static_cast<int>(m < per_pass ? m : per_pass), a.x_stride));
+  const int smem = static_cast<int>(rows_smem(tt, l.units, a.ck, a.ws, a.slice,
+                                              static_cast<int>(m < per_pass ? m : per_pass)));
   const int groups = (l.n_tiles + kWarps / a.ws - 1) / (kWarps / a.ws);
   const int clusters = groups < sm_count / a.ck ? groups : sm_count / a.ck;
   PdlIo io;

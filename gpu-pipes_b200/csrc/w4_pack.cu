@@ -51,19 +51,21 @@ __device__ __forceinline__ Where where(const W4Layout& l) {
   return w;
 }
 
-__device__ __forceinline__ uint4* code_ptr(const W4Layout& l, void* packed, int tile, int block, int g) {
+// part: 64-row part of the whole matrix (block = part / 2)
+__device__ __forceinline__ uint4* code_ptr(const W4Layout& l, void* packed, int tile, int part, int g) {
   return reinterpret_cast<uint4*>(static_cast<char*>(packed) +
-                                  ((static_cast<int64_t>(tile) * l.k_blocks + block) * 512 + g * 64));
+                                  ((static_cast<int64_t>(tile) * l.blocks * 2 + part) * (kW4BlockBytes / 2) + g * 64));
 }
 
 __device__ __forceinline__ uint32_t* scale_ptr(const W4Layout& l, void* packed, int tile, int group, int g) {
-  const int64_t i = (static_cast<int64_t>(tile) * l.groups + group) * 8 + g;
+  const int64_t cell = static_cast<int64_t>(tile) * l.blocks + group / l.units;
+  const int64_t i = (cell * 8 + g) * l.units + group % l.units;
   return reinterpret_cast<uint32_t*>(static_cast<char*>(packed) + l.scale_off) + (l.zeros ? 2 * i : i);
 }
 
 // Codes of one 32-row half of a block for a column pair: q(r, k) gives the code of row k (0..31) of
 // the half. Word 2 h + j of lane 4 g + t.
-template <class F>
+template <typename T, class F>
 __device__ __forceinline__ void put_half(uint4* block_pair, int h, F&& q) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
@@ -76,7 +78,7 @@ __device__ __forceinline__ void put_half(uint4* block_pair, int h, F&& q) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) w[j] |= q(r, 8 * t + 4 * j + i) << (4 * w4_nibble(r, i));
     }
-    reinterpret_cast<uint2*>(block_pair + t)[h] = make_uint2(w[0], w[1]);
+    reinterpret_cast<uint2*>(block_pair + t)[h] = make_uint2(w4_store_word<T>(w[0]), w4_store_word<T>(w[1]));
   }
 }
 
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_
   pdl_launch_dependents();
   const Where at = where(l);
   if (!at.in) return;
-  for (int64_t grp = blockIdx.y; grp < l.groups; grp += gridDim.y) {
+  for (int64_t grp = blockIdx.y; grp < l.blocks * l.units; grp += gridDim.y) {
     const int k0 = static_cast<int>(grp) * G;
     uint32_t v[G];
 #pragma unroll
@@ -128,8 +130,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_
 #pragma unroll
     for (int hh = 0; hh < G / 32; ++hh) {
       const int k = k0 + hh * 32;
-      if (k / 64 >= l.k_blocks) break;  // a group of 128 may reach past the last block
-      put_half(code_ptr(l, packed, at.tile, k / 64, at.g), (k / 32) & 1, [&](int r, int kk) {
+      put_half<T>(code_ptr(l, packed, at.tile, k / 64, at.g), (k / 32) & 1, [&](int r, int kk) {
         const float2 f = Elem<T>::unpack(v[hh * 32 + kk]);
         const float x = r == 0 ? f.x : f.y;
         float q = z[r];
@@ -150,11 +151,11 @@ __global__ void __launch_bounds__(kPackThreads) w4_pack_kernel(const __grid_cons
   pdl_launch_dependents();
   const Where at = where(l);
   if (!at.in) return;
-  for (int64_t b = blockIdx.y; b < l.k_blocks; b += gridDim.y) {
+  for (int64_t b = blockIdx.y; b < l.blocks * 2; b += gridDim.y) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = static_cast<int>(b) * 64 + h * 32;
-      put_half(code_ptr(l, packed, at.tile, static_cast<int>(b), at.g), h, [&](int r, int kk) {
+      put_half<T>(code_ptr(l, packed, at.tile, static_cast<int>(b), at.g), h, [&](int r, int kk) {
         const bool pad = k + kk >= l.k || at.c + r >= l.n;
         return pad ? 0u : static_cast<uint32_t>(codes[static_cast<int64_t>(k + kk) * l.n + at.c + r]) & 15u;
       });
@@ -184,13 +185,13 @@ __global__ void __launch_bounds__(kPackThreads) w4_unpack_kernel(const __grid_co
   pdl_launch_dependents();
   const Where at = where(l);
   if (!at.in || at.c >= l.n) return;
-  for (int64_t b = blockIdx.y; b < l.k_blocks; b += gridDim.y) {
+  for (int64_t b = blockIdx.y; b < l.blocks * 2; b += gridDim.y) {
     if (codes != nullptr) {
       const uint4* p = code_ptr(l, packed, at.tile, static_cast<int>(b), at.g);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const uint4 u = p[t];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t w[4] = {w4_load_word<T>(u.x), w4_load_word<T>(u.y), w4_load_word<T>(u.z), w4_load_word<T>(u.w)};
 #pragma unroll
         for (int e = 0; e < 16; ++e) {  // word 2 h + j, row i of it
           const int wi = e >> 2, i = e & 3;
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_dequantize_kernel(const __gri
   pdl_launch_dependents();
   const Where at = where(l);
   if (!at.in || at.c >= l.n) return;
-  for (int64_t b = blockIdx.y; b < l.k_blocks; b += gridDim.y) {
+  for (int64_t b = blockIdx.y; b < l.blocks * 2; b += gridDim.y) {
     const uint4* p = code_ptr(l, packed, at.tile, static_cast<int>(b), at.g);
     uint4 u[4];
 #pragma unroll
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_dequantize_kernel(const __gri
       if (l.zeros) z = Elem<T>::unpack(sp[1]);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const uint32_t wd[2] = {h == 0 ? u[t].x : u[t].z, h == 0 ? u[t].y : u[t].w};
+        const uint32_t wd[2] = {w4_load_word<T>(h == 0 ? u[t].x : u[t].z), w4_load_word<T>(h == 0 ? u[t].y : u[t].w)};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = e >> 2, i = e & 3, k = k0 + 8 * t + e;
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_dequantize_kernel(const __gri
   }
 }
 
-// Launch over column pairs (x) and row blocks or groups (y, with a stride past the grid's limit).
+// Launch over column pairs (x) and 64-row parts or groups (y, with a stride past the grid's limit).
 // `out` / `bytes`: what the launch writes.
 template <typename... KArgs, typename... Args>
 int launch_pack(void (*kern)(KArgs...), const W4Layout& l, int rows, cudaStream_t s, const PdlIo& io, Args... args) {
@@ -281,7 +282,7 @@ int quantize_g(const W4Layout& l, const T* w, void* packed, cudaStream_t s) {
   const bool vec = even_rows(l, w);
   auto kern = l.zeros ? (vec ? &w4_quantize_kernel<T, G, true, true> : &w4_quantize_kernel<T, G, true, false>)
                       : (vec ? &w4_quantize_kernel<T, G, false, true> : &w4_quantize_kernel<T, G, false, false>);
-  return launch_pack(kern, l, l.groups, s, io, w, packed);
+  return launch_pack(kern, l, l.blocks * l.units, s, io, w, packed);
 }
 
 template <typename T>
@@ -298,7 +299,7 @@ int pack_t(const W4Layout& l, const uint8_t* codes, const void* scales, const ui
   PdlIo io;
   io.add(PdlIo::kWrite, packed, static_cast<uint64_t>(l.bytes));
   auto kern = even_rows(l, scales) ? &w4_pack_kernel<T, true> : &w4_pack_kernel<T, false>;
-  return launch_pack(kern, l, l.k_blocks, s, io, codes, static_cast<const T*>(scales), zeros, packed);
+  return launch_pack(kern, l, l.blocks * 2, s, io, codes, static_cast<const T*>(scales), zeros, packed);
 }
 
 template <typename T>
@@ -309,7 +310,7 @@ int unpack_t(const W4Layout& l, const void* packed, uint8_t* codes, void* scales
   io.add(PdlIo::kWrite, scales, ng * 2);
   io.add(PdlIo::kWrite, zeros, ng);
   auto kern = scales != nullptr && even_rows(l, scales) ? &w4_unpack_kernel<T, true> : &w4_unpack_kernel<T, false>;
-  return launch_pack(kern, l, l.k_blocks, s, io, const_cast<void*>(packed), codes, static_cast<T*>(scales), zeros);
+  return launch_pack(kern, l, l.blocks * 2, s, io, const_cast<void*>(packed), codes, static_cast<T*>(scales), zeros);
 }
 
 template <typename T>
@@ -317,7 +318,7 @@ int dequantize_t(const W4Layout& l, const void* packed, void* w, cudaStream_t s)
   PdlIo io;
   io.add(PdlIo::kWrite, w, static_cast<uint64_t>(l.k) * l.n * 2);
   auto kern = even_rows(l, w) ? &w4_dequantize_kernel<T, true> : &w4_dequantize_kernel<T, false>;
-  return launch_pack(kern, l, l.k_blocks, s, io, const_cast<void*>(packed), static_cast<T*>(w));
+  return launch_pack(kern, l, l.blocks * 2, s, io, const_cast<void*>(packed), static_cast<T*>(w));
 }
 
 }  // namespace

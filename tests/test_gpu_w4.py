@@ -228,10 +228,10 @@ def test_linear_large_offsets(cuda_dev):
     tail = 48
     codes, scales, _ = make(k, tail, torch.bfloat16, 128, False)
     t4 = cuda_ext.w4_pack(codes, scales, None, group=128)
-    tiles = (n - tail) // 16  # ... but for the last 48 columns
-    w4.packed[tiles * (k // 64) * 512:(tiles + 3) * (k // 64) * 512] = t4.packed[:3 * (k // 64) * 512]
-    so, to = (n // 16) * (k // 64) * 512, 3 * (k // 64) * 512
-    w4.packed[so + tiles * (k // 128) * 32:so + (tiles + 3) * (k // 128) * 32] = t4.packed[to:to + 3 * (k // 128) * 32]
+    cells = k // 128  # of a 16-column tile: 1,024 bytes of codes each, then 32 of scales
+    at, so, to = (n - tail) // 16 * cells, n // 16 * cells * 1024, tail // 16 * cells * 1024
+    w4.packed[at * 1024:so] = t4.packed[:to]
+    w4.packed[so + at * 32:] = t4.packed[to:]
     x = rows(m, k, torch.bfloat16)
     out = cuda_ext.w4_linear(x, w4)
     assert torch.equal(out[:, -tail:], cuda_ext.w4_linear(x, t4))

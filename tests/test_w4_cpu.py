@@ -23,9 +23,8 @@ def nbytes(*a, **kw):
 @pytest.mark.parametrize("k,n,group,zeros", [(8, 1, 32, 0), (64, 16, 64, 1), (1000, 17, 128, 0),
                                              (1024, 4096, 128, 0), (5128, 11003, 32, 1), (65536, 3, 64, 1)])
 def test_packed_bytes(k, n, group, zeros):
-    tiles, blocks = -(-n // 16), -(-k // 64)
-    groups = -(-blocks * 64 // group)
-    want = tiles * blocks * 512 + tiles * groups * 16 * (4 if zeros else 2)
+    cells = -(-n // 16) * -(-k // 128)  # 16 columns x 128 rows
+    want = cells * (1024 + 16 * (128 // group) * (4 if zeros else 2))
     assert nbytes(k, n, group, L.GP_F16, zeros) == want
 
 
