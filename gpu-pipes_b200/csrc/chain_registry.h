@@ -83,8 +83,12 @@ void workspace_release(cudaStream_t stream);
 unsigned long long current_timeout_ns();
 int current_fault_injection();
 void count_launches(int n);
-// SM count of the current device (its per-device state is created on first use).
-int device_sm_count(int* sm_count);
+// The current device (its per-device state is created on first use).
+struct DeviceInfo {
+  int sm_count;
+  int* status;  // device status word
+};
+int device_info(DeviceInfo* info);
 // After the last launch of a call: its launch error, the launch count (`launches` more) and, with
 // GP_SYNC_CHECK=1, the stream's completion and the device status word.
 int finish_launch(cudaStream_t stream, int dev_status_check, int launches = 1);

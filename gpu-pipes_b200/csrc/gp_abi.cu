@@ -350,10 +350,10 @@ int finish_launch(cudaStream_t stream, int dev_status_check, int launches) {
   return GP_OK;
 }
 
-int device_sm_count(int* sm_count) {
+int device_info(DeviceInfo* info) {
   DeviceState* st = nullptr;
   const int rc = get_device_state(&st);
-  if (rc == GP_OK) *sm_count = st->sm_count;
+  if (rc == GP_OK) *info = {st->sm_count, st->status};
   return rc;
 }
 
@@ -558,8 +558,8 @@ static int block_norm(const gp_block_norm_spec* s, int64_t m, const void* x, con
   for (int i = 2; i < 7; ++i)
     if (overlap(r, n * sb, ptrs[i], i == 2 ? gr * row : row) || overlap(h, n * 2, ptrs[i], i == 2 ? gr * row : row))
       return set_error(GP_ERR_ARG, "an output overlaps the gate or a norm's parameters");
-  int sms = 0;
-  int rc = device_sm_count(&sms);
+  DeviceInfo dev;
+  int rc = device_info(&dev);
   if (rc != GP_OK) return rc;
   BlockNormArgs a;
   a.m = m;
@@ -624,10 +624,10 @@ static int w4_check(const W4Layout& l, const void* packed, const W4Buf* bufs, in
 // One layer; the launcher counts its launches.
 static int w4_linear(const W4Layout& l, int dtype, int64_t m, int act, const void* x, const void* packed,
                      const void* bias, void* out, bool out_f32, cudaStream_t stream) {
-  int sms = 0;
-  const int rc = device_sm_count(&sms);
+  DeviceInfo dev;
+  const int rc = device_info(&dev);
   if (rc != GP_OK) return rc;
-  return launch_w4_linear(l, dtype, m, x, packed, bias, act, out, out_f32, stream, sms);
+  return launch_w4_linear(l, dtype, m, x, packed, bias, act, out, out_f32, stream, dev);
 }
 
 static uint64_t align256(uint64_t b) { return (b + 255) / 256 * 256; }

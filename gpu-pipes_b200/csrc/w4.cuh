@@ -18,6 +18,7 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "chain_registry.h"
 #include "gp_ptx.cuh"
 
 namespace gp {
@@ -115,6 +116,6 @@ int launch_w4_dequantize(const W4Layout& l, int dtype, const void* packed, void*
 
 // out [m, n] = act(x [m, k] W + bias), out in T or fp32 (out_f32); x rows are read 16 bytes at a time
 int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, const void* packed, const void* bias,
-                     int act, void* out, bool out_f32, cudaStream_t s, int sm_count);
+                     int act, void* out, bool out_f32, cudaStream_t s, const DeviceInfo& dev);
 
 }  // namespace gp

@@ -16,8 +16,11 @@
 //   - A CTA of 16 warps owns a slice of K (one of `ck` CTAs of a cluster does; ck = 1: all of it),
 //     keeps its part of the x rows in shared memory and goes over column tiles of 16. `ws` warps
 //     share a tile, each taking every ws-th 128-row block, so together they read whole stretches.
-//   - The codes of the next few blocks are in flight in registers, across tiles: the loads go on
-//     while the warps' sums are joined.
+//   - Every warp streams its blocks through a ring of its own in shared memory: one lane starts the
+//     bulk copies (a block's codes and its scales, contiguous both), the warp waits on the slot's
+//     mbarrier, takes the slot into registers and hands it back at once. The loads of the next tiles
+//     go on while the sums of this one are joined. (Loads straight to registers, four blocks ahead,
+//     ended up waiting for one another: 40 us at 1 x 8192 x 28672.)
 //   - The warps' sums are joined in shared memory, the CTAs' through distributed shared memory,
 //     both in a fixed order: results do not depend on timing.
 #include <climits>
@@ -33,6 +36,9 @@ constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kPartStride = 20;     // floats per row of a warp's 16 x rows sums: conflict-free float2 stores
 constexpr int kMaxCluster = 8;
+constexpr int kMaxDepth = 8;        // ring slots per warp
+constexpr int kMinDepth = 3;
+constexpr int kRowsSmem = kSmemLimit - 2048;  // dynamic: the barriers are static
 constexpr int kZeroBytes = 256;     // zeros in shared memory, read in place of absent x rows
 
 struct W4RowsArgs {
@@ -49,6 +55,10 @@ struct W4RowsArgs {
   int iters;         // column tile groups per cluster
   int rows;          // x rows of a pass (at most 8 TT)
   int x_stride;      // bytes between x rows in shared memory
+  int depth;         // ring slots per warp
+  int* status;
+  unsigned long long timeout_ns;
+  int inject;        // fault injection: 1 = no block is ever loaded
 };
 
 // exact forms: with few rows the epilogue costs nothing, so nothing is approximated
@@ -76,26 +86,30 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes and scales are read once: past L1.
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
   return v;
 }
 
 template <int W>
-__device__ __forceinline__ void ldg_words(const void* p, uint32_t (&v)[W]) {
+__device__ __forceinline__ void lds_words(uint32_t p, uint32_t (&v)[W]) {
   if constexpr (W == 1) {
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(p) : "memory");
   } else if constexpr (W == 2) {
-    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(p) : "memory");
   } else {
 #pragma unroll
-    for (int i = 0; i < W; i += 4)
-      asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
-                   : "l"(static_cast<const uint32_t*>(p) + i));
+    for (int i = 0; i < W; i += 4) {
+      const uint4 u = lds128(p + 4 * i);
+      v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
+    }
   }
 }
 
@@ -108,10 +122,13 @@ template <typename T, int TT, int UNITS, bool ZP, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_constant__ W4RowsArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);                // scale words of a lane per block
   constexpr int kPart = TT * 8 * kPartStride;                 // floats of a warp's sums
-  constexpr int kDepth = kWords >= 8 ? 3 : 4;                 // blocks in flight per warp (registers)
+  constexpr int kScaleBytes = 32 * kWords;                    // scales of a block
+  constexpr int kSlot = kW4BlockBytes + kScaleBytes;
   constexpr float kUnit0 = W4Deq<T>::unit(0), kUnit1 = W4Deq<T>::unit(1);
   extern __shared__ __align__(128) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem);               // [2][kWarps][kPart]
+  __shared__ __align__(8) uint64_t full[kWarps][kMaxDepth];
+  __shared__ int abort_flag;
+  float* part = reinterpret_cast<float*>(smem + kWarps * a.depth * kSlot);  // [2][kWarps][kPart]
   const int np = kWarps / a.ws;                               // tiles at a time
   const int outs = np * TT * 128;                             // sums of a tile group
   float* red = part + 2 * kWarps * kPart;                     // [2][outs], clusters only
@@ -127,52 +144,50 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   const int b0 = rank * a.slice;
   const int nb = min(a.slice, a.l.blocks - b0);               // blocks of this CTA
   const int sub = warp % a.ws, slot_tile = warp / a.ws;
-  const int steps = (a.slice + a.ws - 1) / a.ws;              // blocks of a warp per tile
 
-  // the block that is loaded next: tile and block (relative to the slice) of this warp's
-  int ld_tile = cluster * np + slot_tile, ld_rel = sub, ld_b = 0;
+  // the block that is loaded next: tile and block (relative to the slice) of this warp's; a warp
+  // without a block in the slice loads nothing
   const int tile_step = clusters * np;
-  const uint8_t* codes = static_cast<const uint8_t*>(a.packed) +
-                         (static_cast<int64_t>(ld_tile) * a.l.blocks + b0 + sub) * kW4BlockBytes + lane * 16;
-  const uint8_t* scales = static_cast<const uint8_t*>(a.packed) + a.l.scale_off +
-                          (static_cast<int64_t>(ld_tile) * a.l.blocks + b0 + sub) * (32 * kWords) + g * (4 * kWords);
-  const int64_t back = static_cast<int64_t>(tile_step) * a.l.blocks - static_cast<int64_t>(steps) * a.ws;
-  auto advance = [&] {
+  int ld_tile = sub < nb ? cluster * np + slot_tile : INT_MAX, ld_rel = sub, ld_slot = 0;
+  const uint32_t ring = smem_u32(smem) + warp * a.depth * kSlot, bars = smem_u32(full[warp]);
+  const uint8_t* const codes0 = static_cast<const uint8_t*>(a.packed) + (b0 + sub) * kW4BlockBytes;
+  const uint8_t* const scales0 = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + (b0 + sub) * kScaleBytes;
+  const int64_t first = static_cast<int64_t>(cluster * np + slot_tile) * a.l.blocks;
+  const uint8_t *codes = codes0 + first * kW4BlockBytes, *scales = scales0 + first * kScaleBytes;
+  // one lane: the next block of the warp's sequence into the next slot
+  auto load = [&] {
+    if (ld_tile >= a.l.n_tiles || a.inject != 0) return;
+    const uint32_t bar = bars + ld_slot * 8, dst = ring + ld_slot * kSlot;
+    mbar_arrive_expect_tx(bar, kSlot);
+    bulk_load(dst, codes, kW4BlockBytes, bar);
+    bulk_load(dst + kW4BlockBytes, scales, kScaleBytes, bar);
+    ld_slot = ld_slot + 1 == a.depth ? 0 : ld_slot + 1;
     codes += a.ws * kW4BlockBytes;
-    scales += a.ws * (32 * kWords);
+    scales += a.ws * kScaleBytes;
     ld_rel += a.ws;
-    if (++ld_b == steps) {
-      ld_b = 0;
+    if (ld_rel >= nb) {
       ld_rel = sub;
-      ld_tile += tile_step;
-      codes += back * kW4BlockBytes;
-      scales += back * (32 * kWords);
+      ld_tile = tile_step < a.l.n_tiles - ld_tile ? ld_tile + tile_step : INT_MAX;
+      const int64_t at = static_cast<int64_t>(ld_tile) * a.l.blocks;
+      codes = codes0 + at * kW4BlockBytes;
+      scales = scales0 + at * kScaleBytes;
     }
   };
 
   // The first codes go into L2 while the previous kernel of the stream drains (a hint: nothing is
   // read into the program before the wait).
-  if (ld_tile < a.l.n_tiles)
-    for (int i = 0; i < kDepth && i < steps && sub + i * a.ws < nb; ++i)
-      if ((lane & 7) == 0) {
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes + i * a.ws * kW4BlockBytes));
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes + i * a.ws * kW4BlockBytes + kW4BlockBytes / 2));
-      }
+  if (ld_tile < a.l.n_tiles && lane < 8)
+    for (int i = 0; i < a.depth && sub + i * a.ws < nb; ++i)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(codes + i * a.ws * kW4BlockBytes + lane * 128));
+  if (lane == 0) {
+    for (int i = 0; i < a.depth; ++i) mbar_init(bars + i * 8, 1);
+    fence_mbar_init();
+    if (warp == 0) abort_flag = 0;
+  }
   pdl_wait_prior();
   pdl_launch_dependents();
-
-  uint4 cbuf[kDepth][2];
-  uint32_t sbuf[kDepth][kWords];
-  auto load = [&](int p) {
-    if (ld_tile < a.l.n_tiles && ld_rel < nb) {
-      cbuf[p][0] = ldg_stream(codes);
-      cbuf[p][1] = ldg_stream(codes + kW4BlockBytes / 2);
-      ldg_words<kWords>(scales, sbuf[p]);
-    }
-    advance();
-  };
-#pragma unroll
-  for (int p = 0; p < kDepth; ++p) load(p);
+  if (lane == 0)
+    for (int i = 0; i < a.depth; ++i) load();
 
   // x rows of this CTA's slice (zero past K) and their sums over each group. Sixteen lanes hold a
   // block of a row; absent rows have sums of zero and are read from the zeros.
@@ -210,14 +225,31 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   }
 
   float acc[TT][4];
-  auto compute = [&](int p, int rel) {
+  const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
+  int slot = 0, phase = 0;
+  bool ok = true;
+  auto compute = [&](int rel) {
+    if (!mbar_wait(bars + slot * 8, phase, wctx, kDevTimeoutProducer)) ok = false;
+    if (!__all_sync(0xffffffffu, ok)) {  // nothing is read; the joins go on, so no barrier is missed
+      ok = false;
+      return;
+    }
+    uint4 cbuf[2];
+    uint32_t sbuf[kWords];
+    const uint32_t d = ring + slot * kSlot;
+    cbuf[0] = lds128(d + lane * 16);
+    cbuf[1] = lds128(d + kW4BlockBytes / 2 + lane * 16);
+    lds_words<kWords>(d + kW4BlockBytes + g * (4 * kWords), sbuf);
+    if (++slot == a.depth) slot = 0, phase ^= 1;
+    __syncwarp();
+    if (lane == 0) load();
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       float sum[TT][4];
-      const float2 s = Elem<T>::unpack(sbuf[p][ZP ? 2 * u : u]);
+      const float2 s = Elem<T>::unpack(sbuf[ZP ? 2 * u : u]);
       float2 z = make_float2(-8.0f - W4Deq<T>::kOffset, -8.0f - W4Deq<T>::kOffset);
       if constexpr (ZP) {
-        z = Elem<T>::unpack(sbuf[p][2 * u + 1]);
+        z = Elem<T>::unpack(sbuf[2 * u + 1]);
         z.x = -W4Deq<T>::kOffset - z.x;
         z.y = -W4Deq<T>::kOffset - z.y;
       }
@@ -233,18 +265,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       }
 #pragma unroll
       for (int h = u * (4 / UNITS); h < (u + 1) * (4 / UNITS); ++h) {  // 32 rows at a time
-        const uint4 c = cbuf[p][h >> 1];
+        const uint4 c = cbuf[h >> 1];
         uint32_t p0[4], p1[4];
         W4Deq<T>::pairs((h & 1) ? c.z : c.x, p0);
         W4Deq<T>::pairs((h & 1) ? c.w : c.y, p1);
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-          uint32_t x0, x1, x2, x3;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(x0), "=r"(x1), "=r"(x2), "=r"(x3)
-                       : "r"(xr[i] + (static_cast<uint32_t>(rel * (kW4Block * 2)) & xmask[i]) + h * 64) : "memory");
-          mma16816<T>(sum[i], p0, x0, x1);
-          mma16816<T>(sum[i], p1, x2, x3);
+          const uint4 xv = lds128(xr[i] + (static_cast<uint32_t>(rel * (kW4Block * 2)) & xmask[i]) + h * 64);
+          mma16816<T>(sum[i], p0, xv.x, xv.y);
+          mma16816<T>(sum[i], p1, xv.z, xv.w);
         }
       }
 #pragma unroll
@@ -317,34 +346,30 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < TT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
   };
-  clear();
-  int it = 0, b = 0, rel = sub, tile = cluster * np + slot_tile;
-  while (it < a.iters) {
-#pragma unroll
-    for (int p = 0; p < kDepth; ++p) {
-      if (it < a.iters) {
-        if (tile < a.l.n_tiles && rel < nb) compute(p, rel);
-        load(p);
-        rel += a.ws;
-        if (++b == steps) {
-          join(it);
-          clear();
-          b = 0;
-          rel = sub;
-          tile += tile_step;
-          ++it;
-        }
+  for (int it = 0, tile = cluster * np + slot_tile; it < a.iters; ++it, tile += tile_step) {
+    clear();
+    if (tile < a.l.n_tiles)
+      for (int rel = sub; rel < nb; rel += a.ws) compute(rel);
+    join(it);
+  }
+  // After a wait that ran out, the copies that were started are waited for (again with a limit)
+  // before the CTA's shared memory goes away; otherwise every copy has been taken above.
+  if (!ok && lane == 0 && a.inject == 0) {
+    for (int i = 0; i < a.depth; ++i) {
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(bars + slot * 8, phase) && globaltimer_ns() - t0 < a.timeout_ns) {
       }
+      if (++slot == a.depth) slot = 0, phase ^= 1;
     }
   }
 }
 
 int rows_x_stride(int slice) { return slice * (kW4Block * 2) + 64; }  // conflict-free: 64 past a multiple of 128
 
-// Shared memory of a CTA: warps' sums, clusters' sums, group sums of x, zeros, x rows
-int64_t rows_smem(int tt, int units, int ck, int ws, int slice, int rows) {
+// Shared memory of a CTA: rings, warps' sums, clusters' sums, group sums of x, zeros, x rows
+int64_t rows_smem(const W4Layout& l, int tt, int ck, int ws, int slice, int rows, int depth) {
   const int64_t outs = static_cast<int64_t>(kWarps / ws) * tt * 128;
-  return 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) + 32ll * slice * units * tt +
+  return static_cast<int64_t>(kWarps) * depth * (kW4BlockBytes + l.scale_bytes()) + 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) + 32ll * slice * l.units * tt +
          kZeroBytes + static_cast<int64_t>(rows) * rows_x_stride(slice);
 }
 
@@ -352,7 +377,7 @@ template <typename T, int TT, int UNITS, bool ZP, typename OutT>
 int rows_launch(const W4RowsArgs& a, int smem, int clusters, int64_t row_tiles, cudaStream_t s, const PdlIo& io) {
   static unsigned long long done_mask = 0;
   auto kern = &w4_rows_kernel<T, TT, UNITS, ZP, OutT>;
-  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kSmemLimit, &done_mask);
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kRowsSmem, &done_mask);
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * a.ck), static_cast<unsigned>(row_tiles), 1);
@@ -404,8 +429,12 @@ int rows_tt(const W4RowsArgs& a, int tt, int smem, int clusters, int64_t rt, cud
 }  // namespace
 
 int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, const void* packed, const void* bias,
-                     int act, void* out, bool out_f32, cudaStream_t s, int sm_count) {
+                     int act, void* out, bool out_f32, cudaStream_t s, const DeviceInfo& dev) {
+  const int sm_count = dev.sm_count;
   W4RowsArgs a;
+  a.status = dev.status;
+  a.timeout_ns = current_timeout_ns();
+  a.inject = current_fault_injection();
   a.l = l;
   a.x = x;
   a.packed = packed;
@@ -425,7 +454,7 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
       if (ck > 1 && (ck - 1) * slice >= l.blocks) break;  // a CTA without work
       for (int ws = 1; ws <= kWarps; ws *= 2) {
         if (ws > 1 && ws / 2 >= slice) break;
-        if (rows_smem(tt, l.units, ck, ws, slice, rows) > kSmemLimit) continue;
+        if (rows_smem(l, tt, ck, ws, slice, rows, kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
         const int clusters = groups < sm_count / ck ? groups : sm_count / ck;
         const int64_t iters = (groups + clusters - 1) / clusters;
@@ -444,8 +473,10 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
   a.rows = per_pass;
   a.x_stride = rows_x_stride(a.slice);
   const int tt = per_pass > 8 ? 2 : 1;
-  const int smem = static_cast<int>(rows_smem(tt, l.units, a.ck, a.ws, a.slice,
-                                              static_cast<int>(m < per_pass ? m : per_pass)));
+  const int rows = static_cast<int>(m < per_pass ? m : per_pass);
+  a.depth = kMaxDepth;
+  while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.depth) > kRowsSmem) --a.depth;
+  const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.depth));
   const int groups = (l.n_tiles + kWarps / a.ws - 1) / (kWarps / a.ws);
   const int clusters = groups < sm_count / a.ck ? groups : sm_count / a.ck;
   PdlIo io;

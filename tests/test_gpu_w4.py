@@ -507,3 +507,25 @@ def test_device_refusals(cuda_dev):
         cuda_ext.w4_mlp(x, [w4, other], [None, None], acts=[0, 0])
     empty = cuda_ext.w4_linear(x[:0], w4)
     assert empty.shape == (0, 32)
+
+
+def test_missing_codes_time_out_and_the_next_call_is_right(cuda_dev):
+    """With host-side fault injection no block of codes is ever loaded: every wait runs out after
+    5 ms, the kernel ends, the status word says so, and the context stays usable."""
+    for m, k, n in ((1, 256, 64), (3, 4096, 48)):  # one CTA per tile, and a cluster along K
+        codes, scales, z = make(k, n, torch.float16, 64, True)
+        w4 = cuda_ext.w4_pack(codes, scales, z, group=64)
+        x = rows(m, k, torch.float16)
+        want = cuda_ext.w4_linear(x, w4)
+        assert L.device_status(0, clear=True) == 0
+        try:
+            L.set_timeout_ns(5_000_000)
+            L.set_fault_injection(1)
+            cuda_ext.w4_linear(x, w4)
+            torch.cuda.synchronize()
+        finally:
+            L.set_fault_injection(0)
+            L.set_timeout_ns(0)
+        assert L.device_status(0, clear=True) == 0x100
+        assert torch.equal(cuda_ext.w4_linear(x, w4), want)
+        assert L.device_status(0) == 0
