@@ -32,13 +32,16 @@
 namespace gp {
 namespace {
 
+// Warps of a CTA (one CTA per SM): kWarps turn codes into sums, kJoinWarps add the sums up and store.
 constexpr int kWarps = 16;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kJoinWarps = 4;
+constexpr int kJoiners = 32 * kJoinWarps;
+constexpr int kThreads = 32 * (kWarps + kJoinWarps);
 constexpr int kPartStride = 20;     // floats per row of a warp's 16 x rows sums: conflict-free float2 stores
 constexpr int kMaxCluster = 8;
 constexpr int kMaxDepth = 8;        // ring slots per warp
 constexpr int kMinDepth = 3;
-constexpr int kRowsSmem = kSmemLimit - 2048;  // dynamic: the barriers are static
+constexpr int kRowsSmem = kSmemLimit - 3072;  // dynamic: the barriers are static
 constexpr int kZeroBytes = 256;     // zeros in shared memory, read in place of absent x rows
 
 struct W4RowsArgs {
@@ -51,6 +54,7 @@ struct W4RowsArgs {
   int act;
   int ck;            // CTAs of a cluster, along K
   int slice;         // k-blocks of a CTA
+  int run;           // k-blocks of a ring slot (1 or 2), neighbours in the packed codes
   int ws;            // warps that share a column tile
   int iters;         // column tile groups per cluster
   int rows;          // x rows of a pass (at most 8 TT)
@@ -113,8 +117,23 @@ __device__ __forceinline__ void lds_words(uint32_t p, uint32_t (&v)[W]) {
   }
 }
 
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+// Named barriers of the CTA (0 is __syncthreads): waiting, and arriving without waiting.
+__device__ __forceinline__ void bar_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id) {
+  __syncwarp();
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+}
+constexpr int kBarFull = 1, kBarFree = 3;  // + buffer 0 / 1 of the warps' sums
+
+// 16 bytes into the shared memory of a CTA of the cluster, counted on that CTA's mbarrier: the
+// reader needs no other signal and the writer no fence.
+__device__ __forceinline__ void st_async_f32x4(uint32_t addr, uint32_t bar, float4 v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%2, %3, %4, %5}, [%1];" ::"r"(addr),
+               "r"(bar), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
 }
 
 // TT: tiles of 8 x rows. UNITS: groups per k-block of 128.
@@ -126,9 +145,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   constexpr int kSlot = kW4BlockBytes + kScaleBytes;
   constexpr float kUnit0 = W4Deq<T>::unit(0), kUnit1 = W4Deq<T>::unit(1);
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kWarps][kMaxDepth];
-  __shared__ int abort_flag;
-  float* part = reinterpret_cast<float*>(smem + kWarps * a.depth * kSlot);  // [2][kWarps][kPart]
+  __shared__ __align__(8) uint64_t full[kWarps + kJoinWarps][kMaxDepth];
+  __shared__ __align__(8) uint64_t red_full[2];
+  __shared__ int abort_flag, join_abort;
+  float* part = reinterpret_cast<float*>(smem + kWarps * a.depth * a.run * kSlot);  // [2][kWarps][kPart]
   const int np = kWarps / a.ws;                               // tiles at a time
   const int outs = np * TT * 128;                             // sums of a tile group
   float* red = part + 2 * kWarps * kPart;                     // [2][outs], clusters only
@@ -145,45 +165,47 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   const int nb = min(a.slice, a.l.blocks - b0);               // blocks of this CTA
   const int sub = warp % a.ws, slot_tile = warp / a.ws;
 
-  // the block that is loaded next: tile and block (relative to the slice) of this warp's; a warp
-  // without a block in the slice loads nothing
-  const int tile_step = clusters * np;
-  int ld_tile = sub < nb ? cluster * np + slot_tile : INT_MAX, ld_rel = sub, ld_slot = 0;
-  const uint32_t ring = smem_u32(smem) + warp * a.depth * kSlot, bars = smem_u32(full[warp]);
-  const uint8_t* const codes0 = static_cast<const uint8_t*>(a.packed) + (b0 + sub) * kW4BlockBytes;
-  const uint8_t* const scales0 = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + (b0 + sub) * kScaleBytes;
-  const int64_t first = static_cast<int64_t>(cluster * np + slot_tile) * a.l.blocks;
-  const uint8_t *codes = codes0 + first * kW4BlockBytes, *scales = scales0 + first * kScaleBytes;
-  // one lane: the next block of the warp's sequence into the next slot
+  // the run of blocks that is loaded next: tile and first block (relative to the slice) of this
+  // warp's; a warp without a block in the slice (and a joining one) loads nothing
+  const int tile_step = clusters * np, lead = sub * a.run, stride = a.ws * a.run, slot_bytes = a.run * kSlot;
+  int ld_tile = warp < kWarps && lead < nb ? cluster * np + slot_tile : INT_MAX, ld_rel = lead, ld_slot = 0;
+  const uint32_t ring = smem_u32(smem) + warp * a.depth * slot_bytes, bars = smem_u32(full[warp]);
+  const uint8_t* const codes0 = static_cast<const uint8_t*>(a.packed) + static_cast<int64_t>(b0) * kW4BlockBytes;
+  const uint8_t* const scales0 = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + static_cast<int64_t>(b0) * kScaleBytes;
+  int64_t ld_cell = static_cast<int64_t>(cluster * np + slot_tile) * a.l.blocks;
+  // one lane: the next run of the warp's sequence into the next slot
   auto load = [&] {
     if (ld_tile >= a.l.n_tiles || a.inject != 0) return;
-    const uint32_t bar = bars + ld_slot * 8, dst = ring + ld_slot * kSlot;
-    mbar_arrive_expect_tx(bar, kSlot);
-    bulk_load(dst, codes, kW4BlockBytes, bar);
-    bulk_load(dst + kW4BlockBytes, scales, kScaleBytes, bar);
+    const uint32_t bar = bars + ld_slot * 8, dst = ring + ld_slot * slot_bytes;
+    const int n = min(a.run, nb - ld_rel);
+    mbar_arrive_expect_tx(bar, n * kSlot);
+    bulk_load(dst, codes0 + (ld_cell + ld_rel) * kW4BlockBytes, n * kW4BlockBytes, bar);
+    bulk_load(dst + a.run * kW4BlockBytes, scales0 + (ld_cell + ld_rel) * kScaleBytes, n * kScaleBytes, bar);
     ld_slot = ld_slot + 1 == a.depth ? 0 : ld_slot + 1;
-    codes += a.ws * kW4BlockBytes;
-    scales += a.ws * kScaleBytes;
-    ld_rel += a.ws;
+    ld_rel += stride;
     if (ld_rel >= nb) {
-      ld_rel = sub;
+      ld_rel = lead;
       ld_tile = tile_step < a.l.n_tiles - ld_tile ? ld_tile + tile_step : INT_MAX;
-      const int64_t at = static_cast<int64_t>(ld_tile) * a.l.blocks;
-      codes = codes0 + at * kW4BlockBytes;
-      scales = scales0 + at * kScaleBytes;
+      ld_cell += static_cast<int64_t>(tile_step) * a.l.blocks;
     }
   };
 
   // The first codes go into L2 while the previous kernel of the stream drains (a hint: nothing is
   // read into the program before the wait).
-  if (ld_tile < a.l.n_tiles && lane < 8)
-    for (int i = 0; i < a.depth && sub + i * a.ws < nb; ++i)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(codes + i * a.ws * kW4BlockBytes + lane * 128));
-  if (lane == 0) {
+  if (ld_tile < a.l.n_tiles)
+    for (int i = 0; i < a.depth && lead + i * stride < nb; ++i) {
+      const int n = min(a.run, nb - lead - i * stride);
+      if (lane < 8 * n)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes0 + (ld_cell + lead + i * stride) * kW4BlockBytes + lane * 128));
+    }
+  if (lane == 0 && warp < kWarps)
     for (int i = 0; i < a.depth; ++i) mbar_init(bars + i * 8, 1);
-    fence_mbar_init();
-    if (warp == 0) abort_flag = 0;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&red_full[0]), 1);
+    mbar_init(smem_u32(&red_full[1]), 1);
+    abort_flag = join_abort = 0;
   }
+  if (lane == 0) fence_mbar_init();
   pdl_wait_prior();
   pdl_launch_dependents();
   if (lane == 0)
@@ -216,141 +238,175 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   // every CTA of the cluster runs before one writes into another's shared memory
   if (a.ck > 1) cluster_sync_all();
 
-  uint32_t xr[TT], xmask[TT];
-#pragma unroll
-  for (int i = 0; i < TT; ++i) {
-    const bool live = i * 8 + g < rows;
-    xr[i] = smem_u32(live ? xs + (i * 8 + g) * a.x_stride : zeros) + t * 16;
-    xmask[i] = live ? 0xffffffffu : 0u;
-  }
-
-  float acc[TT][4];
   const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
   int slot = 0, phase = 0;
   bool ok = true;
-  auto compute = [&](int rel) {
-    if (!mbar_wait(bars + slot * 8, phase, wctx, kDevTimeoutProducer)) ok = false;
-    if (!__all_sync(0xffffffffu, ok)) {  // nothing is read; the joins go on, so no barrier is missed
-      ok = false;
-      return;
-    }
-    uint4 cbuf[2];
-    uint32_t sbuf[kWords];
-    const uint32_t d = ring + slot * kSlot;
-    cbuf[0] = lds128(d + lane * 16);
-    cbuf[1] = lds128(d + kW4BlockBytes / 2 + lane * 16);
-    lds_words<kWords>(d + kW4BlockBytes + g * (4 * kWords), sbuf);
-    if (++slot == a.depth) slot = 0, phase ^= 1;
-    __syncwarp();
-    if (lane == 0) load();
+  if (warp >= kWarps) {
+    // ---- joining: part[warp][row][column] of a tile group, summed over its warps (and CTAs)
+    const int j = threadIdx.x - 32 * kWarps;
+    // Sums go four neighbouring columns at a time: quad q is tile q / (32 TT), row (q / 4) % (8 TT),
+    // columns 4 (q % 4) .. + 3. CTA r of a cluster finishes quads [r own, (r + 1) own).
+    // The wait for another CTA has its own abort flag: a lost copy of codes ends no join, whose sums
+    // are all sent and so arrive before any CTA leaves.
+    const WaitCtx jctx{a.status, &join_abort, a.timeout_ns};
+    const int quads = outs / 4, own = quads / a.ck;
+    const bool vec = a.l.n % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(OutT)) == 0;
+    for (int it = 0; it < a.iters; ++it) {
+      const int tile0 = (cluster + it * clusters) * np, buf = it & 1;
+      const float* pb = part + buf * (kWarps * kPart);
+      auto row_of = [&](int q) { return (q >> 2) % (TT * 8); };
+      auto warps_sum = [&](int q) {
+        const float* p = pb + q / (TT * 32) * a.ws * kPart + row_of(q) * kPartStride + 4 * (q & 3);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int i = 0; i < a.ws; ++i) {
+          const float4 u = *reinterpret_cast<const float4*>(p + i * kPart);
+          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        return v;
+      };
+      auto finish = [&](int q, float4 u) {
+        const int64_t n = static_cast<int64_t>(tile0 + q / (TT * 32)) * 16 + 4 * (q & 3);
+        if (n >= a.l.n) return;
+        float v[4] = {u.x, u.y, u.z, u.w};
+        const int live = a.l.n - n < 4 ? static_cast<int>(a.l.n - n) : 4;
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      float sum[TT][4];
-      const float2 s = Elem<T>::unpack(sbuf[ZP ? 2 * u : u]);
-      float2 z = make_float2(-8.0f - W4Deq<T>::kOffset, -8.0f - W4Deq<T>::kOffset);
-      if constexpr (ZP) {
-        z = Elem<T>::unpack(sbuf[2 * u + 1]);
-        z.x = -W4Deq<T>::kOffset - z.x;
-        z.y = -W4Deq<T>::kOffset - z.y;
-      }
-      z.x *= kUnit0;
-      z.y *= kUnit1;
+        for (int i = 0; i < 4; ++i) {
+          if (a.bias != nullptr && i < live) v[i] += Elem<T>::to_f(static_cast<const T*>(a.bias)[n + i]);
+          v[i] = act_exact(a.act, v[i]);
+        }
+        OutT* to = static_cast<OutT*>(a.out) + (row0 + row_of(q)) * a.l.n + n;
+        if constexpr (sizeof(OutT) == 4) {
+          if (vec) {
+            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+          } else {
+            for (int i = 0; i < live; ++i) to[i] = v[i];
+          }
+        } else {
+          const uint32_t lo = Elem<T>::pack(v[0], v[1]), hi = Elem<T>::pack(v[2], v[3]);
+          if (vec) {
+            *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+          } else {
+            uint16_t* h = reinterpret_cast<uint16_t*>(to);
+            const uint16_t e[4] = {static_cast<uint16_t>(lo), static_cast<uint16_t>(lo >> 16), static_cast<uint16_t>(hi),
+                                   static_cast<uint16_t>(hi >> 16)};
 #pragma unroll
-      for (int i = 0; i < TT; ++i) {
-        const float2 xv = *reinterpret_cast<const float2*>(xsum + (rel * UNITS + u) * (8 * TT) + i * 8 + 2 * t);
-        sum[i][0] = z.x * xv.x;
-        sum[i][1] = z.x * xv.y;
-        sum[i][2] = z.y * xv.x;
-        sum[i][3] = z.y * xv.y;
-      }
-#pragma unroll
-      for (int h = u * (4 / UNITS); h < (u + 1) * (4 / UNITS); ++h) {  // 32 rows at a time
-        const uint4 c = cbuf[h >> 1];
-        uint32_t p0[4], p1[4];
-        W4Deq<T>::pairs((h & 1) ? c.z : c.x, p0);
-        W4Deq<T>::pairs((h & 1) ? c.w : c.y, p1);
-#pragma unroll
-        for (int i = 0; i < TT; ++i) {
-          const uint4 xv = lds128(xr[i] + (static_cast<uint32_t>(rel * (kW4Block * 2)) & xmask[i]) + h * 64);
-          mma16816<T>(sum[i], p0, xv.x, xv.y);
-          mma16816<T>(sum[i], p1, xv.z, xv.w);
+            for (int i = 0; i < 4; ++i)
+              if (i < live) h[i] = e[i];
+          }
+        }
+      };
+      bar_sync(kBarFull + buf);
+      if (a.ck == 1) {
+        for (int q = j; q < quads; q += kJoiners)
+          if (row_of(q) < rows) finish(q, warps_sum(q));
+        if (it + 2 < a.iters) bar_arrive(kBarFree + buf);
+      } else {
+        // A buffer of sums is written again two groups on. The sender has then received the group in
+        // between from the buffer's reader, whose threads all passed a barrier after their reads.
+        const uint32_t bar = smem_u32(&red_full[buf]), to = smem_u32(red + buf * outs) + rank * own * 16;
+        if (j == 0) mbar_arrive_expect_tx(bar, outs * 4);
+        for (int q = j; q < quads; q += kJoiners) {
+          const uint32_t dst = static_cast<uint32_t>(q / own);
+          st_async_f32x4(mapa_shared(to + q % own * 16, dst), mapa_shared(bar, dst), warps_sum(q));
+        }
+        if (it + 2 < a.iters) bar_arrive(kBarFree + buf);
+        if (!mbar_wait<true>(bar, (it >> 1) & 1, jctx, kDevTimeoutEpilogue)) continue;
+        for (int o = j; o < own; o += kJoiners) {
+          if (row_of(rank * own + o) >= rows) continue;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int i = 0; i < a.ck; ++i) {
+            const float4 u = *reinterpret_cast<const float4*>(red + buf * outs + (i * own + o) * 4);
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+          }
+          finish(rank * own + o, v);
         }
       }
-#pragma unroll
-      for (int i = 0; i < TT; ++i) {
-        acc[i][0] = fmaf(s.x, sum[i][0], acc[i][0]);
-        acc[i][1] = fmaf(s.x, sum[i][1], acc[i][1]);
-        acc[i][2] = fmaf(s.y, sum[i][2], acc[i][2]);
-        acc[i][3] = fmaf(s.y, sum[i][3], acc[i][3]);
-      }
     }
-  };
-
-  auto join = [&](int it) {
-    const int tile0 = (cluster + it * clusters) * np;
-    // join: part[warp][row][column]; a buffer is written again two groups on, after the next
-    // group's barrier, when everyone has read it
-    float* pb = part + (it & 1) * (kWarps * kPart);
+  } else {
+    // ---- codes to sums
+    uint32_t xr[TT], xmask[TT];
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
-      float* p = pb + warp * kPart + (i * 8 + 2 * t) * kPartStride + 2 * g;
-      *reinterpret_cast<float2*>(p) = make_float2(acc[i][0] * (1.0f / kUnit0), acc[i][2] * (1.0f / kUnit1));
-      *reinterpret_cast<float2*>(p + kPartStride) = make_float2(acc[i][1] * (1.0f / kUnit0), acc[i][3] * (1.0f / kUnit1));
+      const bool live = i * 8 + g < rows;
+      xr[i] = smem_u32(live ? xs + (i * 8 + g) * a.x_stride : zeros) + t * 16;
+      xmask[i] = live ? 0xffffffffu : 0u;
     }
-    __syncthreads();
-    auto warps_sum = [&](int o) {
-      const int tl = o / (TT * 128), r = (o >> 4) % (TT * 8), n = o & 15;
-      const float* p = pb + tl * a.ws * kPart + r * kPartStride + n;
-      float v = 0.0f;
-#pragma unroll 4
-      for (int i = 0; i < a.ws; ++i) v += p[i * kPart];
-      return v;
-    };
-    auto finish = [&](int o, float v) {
-      const int tl = o / (TT * 128), r = (o >> 4) % (TT * 8);
-      const int64_t n = static_cast<int64_t>(tile0 + tl) * 16 + (o & 15);
-      if (r >= rows || n >= a.l.n) return;
-      if (a.bias != nullptr) v += Elem<T>::to_f(static_cast<const T*>(a.bias)[n]);
-      v = act_exact(a.act, v);
-      const int64_t at = (row0 + r) * a.l.n + n;
-      if constexpr (sizeof(OutT) == 4) {
-        static_cast<float*>(a.out)[at] = v;
-      } else {
-        const uint32_t u = Elem<T>::pack(v, 0.0f);
-        static_cast<uint16_t*>(a.out)[at] = static_cast<uint16_t>(u);
-      }
-    };
-    if (a.ck == 1) {
-      for (int o = threadIdx.x; o < outs; o += kThreads)
-        if ((o >> 4) % (TT * 8) < rows) finish(o, warps_sum(o));
-    } else {
-      // CTA r of the cluster finishes outputs [r outs / ck, (r + 1) outs / ck): the others send
-      // their sums there; the buffer alternates like part, with the cluster's barrier in between
-      const int own = outs / a.ck;
-      float* rb = red + (it & 1) * outs;
-      for (int o = threadIdx.x; o < outs; o += kThreads)
-        if ((o >> 4) % (TT * 8) < rows)
-          st_cluster_f32(mapa_shared(smem_u32(rb + rank * own + o % own), static_cast<uint32_t>(o / own)), warps_sum(o));
-      cluster_sync_all();
-      for (int o = threadIdx.x; o < own; o += kThreads) {
-        const int oo = rank * own + o;
-        if ((oo >> 4) % (TT * 8) >= rows) continue;
-        float v = 0.0f;
-        for (int i = 0; i < a.ck; ++i) v += rb[i * own + o];
-        finish(oo, v);
-      }
-    }
-  };
-
-  auto clear = [&] {
+    float acc[TT][4];
+    // block `i` of the run in ring slot d; rel: its place in the slice
+    auto block = [&](uint32_t d, int i, int rel) {
+      const uint4 cbuf[2] = {lds128(d + i * kW4BlockBytes + lane * 16),
+                             lds128(d + i * kW4BlockBytes + kW4BlockBytes / 2 + lane * 16)};
+      uint32_t sbuf[kWords];
+      lds_words<kWords>(d + a.run * kW4BlockBytes + i * kScaleBytes + g * (4 * kWords), sbuf);
 #pragma unroll
-    for (int i = 0; i < TT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-  };
-  for (int it = 0, tile = cluster * np + slot_tile; it < a.iters; ++it, tile += tile_step) {
-    clear();
-    if (tile < a.l.n_tiles)
-      for (int rel = sub; rel < nb; rel += a.ws) compute(rel);
-    join(it);
+      for (int u = 0; u < UNITS; ++u) {
+        float sum[TT][4];
+        const float2 s = Elem<T>::unpack(sbuf[ZP ? 2 * u : u]);
+        float2 z = make_float2(-8.0f - W4Deq<T>::kOffset, -8.0f - W4Deq<T>::kOffset);
+        if constexpr (ZP) {
+          z = Elem<T>::unpack(sbuf[2 * u + 1]);
+          z.x = -W4Deq<T>::kOffset - z.x;
+          z.y = -W4Deq<T>::kOffset - z.y;
+        }
+        z.x *= kUnit0;
+        z.y *= kUnit1;
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          const float2 xv = *reinterpret_cast<const float2*>(xsum + (rel * UNITS + u) * (8 * TT) + i * 8 + 2 * t);
+          sum[i][0] = z.x * xv.x;
+          sum[i][1] = z.x * xv.y;
+          sum[i][2] = z.y * xv.x;
+          sum[i][3] = z.y * xv.y;
+        }
+#pragma unroll
+        for (int h = u * (4 / UNITS); h < (u + 1) * (4 / UNITS); ++h) {  // 32 rows at a time
+          const uint4 c = cbuf[h >> 1];
+          uint32_t p0[4], p1[4];
+          W4Deq<T>::pairs((h & 1) ? c.z : c.x, p0);
+          W4Deq<T>::pairs((h & 1) ? c.w : c.y, p1);
+#pragma unroll
+          for (int i = 0; i < TT; ++i) {
+            const uint4 xv = lds128(xr[i] + (static_cast<uint32_t>(rel * (kW4Block * 2)) & xmask[i]) + h * 64);
+            mma16816<T>(sum[i], p0, xv.x, xv.y);
+            mma16816<T>(sum[i], p1, xv.z, xv.w);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+          acc[i][0] = fmaf(s.x, sum[i][0], acc[i][0]);
+          acc[i][1] = fmaf(s.x, sum[i][1], acc[i][1]);
+          acc[i][2] = fmaf(s.y, sum[i][2], acc[i][2]);
+          acc[i][3] = fmaf(s.y, sum[i][3], acc[i][3]);
+        }
+      }
+    };
+    for (int it = 0, tile = cluster * np + slot_tile; it < a.iters; ++it, tile += tile_step) {
+#pragma unroll
+      for (int i = 0; i < TT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+      if (tile < a.l.n_tiles)
+        for (int rel = lead; rel < nb; rel += stride) {
+          if (!mbar_wait(bars + slot * 8, phase, wctx, kDevTimeoutProducer)) ok = false;
+          ok = __all_sync(0xffffffffu, ok) != 0;
+          if (!ok) break;  // nothing is read; the joins go on, so no barrier is missed
+          const uint32_t d = ring + slot * slot_bytes;
+          block(d, 0, rel);
+          if (a.run == 2 && rel + 1 < nb) block(d, 1, rel + 1);
+          if (++slot == a.depth) slot = 0, phase ^= 1;
+          __syncwarp();
+          if (lane == 0) load();
+        }
+      const int buf = it & 1;
+      float* pb = part + buf * (kWarps * kPart) + warp * kPart;
+      if (it >= 2) bar_sync(kBarFree + buf);
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        float* p = pb + (i * 8 + 2 * t) * kPartStride + 2 * g;
+        *reinterpret_cast<float2*>(p) = make_float2(acc[i][0] * (1.0f / kUnit0), acc[i][2] * (1.0f / kUnit1));
+        *reinterpret_cast<float2*>(p + kPartStride) = make_float2(acc[i][1] * (1.0f / kUnit0), acc[i][3] * (1.0f / kUnit1));
+      }
+      bar_arrive(kBarFull + buf);
+    }
   }
   // After a wait that ran out, the copies that were started are waited for (again with a limit)
   // before the CTA's shared memory goes away; otherwise every copy has been taken above.
@@ -362,14 +418,19 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       if (++slot == a.depth) slot = 0, phase ^= 1;
     }
   }
+  // no CTA leaves while another may still write into its shared memory
+  if (a.ck > 1) {
+    __syncwarp();
+    cluster_sync_all();
+  }
 }
 
 int rows_x_stride(int slice) { return slice * (kW4Block * 2) + 64; }  // conflict-free: 64 past a multiple of 128
 
 // Shared memory of a CTA: rings, warps' sums, clusters' sums, group sums of x, zeros, x rows
-int64_t rows_smem(const W4Layout& l, int tt, int ck, int ws, int slice, int rows, int depth) {
+int64_t rows_smem(const W4Layout& l, int tt, int ck, int ws, int slice, int rows, int slots) {
   const int64_t outs = static_cast<int64_t>(kWarps / ws) * tt * 128;
-  return static_cast<int64_t>(kWarps) * depth * (kW4BlockBytes + l.scale_bytes()) + 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) + 32ll * slice * l.units * tt +
+  return static_cast<int64_t>(kWarps) * slots * (kW4BlockBytes + l.scale_bytes()) + 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) + 32ll * slice * l.units * tt +
          kZeroBytes + static_cast<int64_t>(rows) * rows_x_stride(slice);
 }
 
@@ -448,13 +509,14 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
   int per_pass = m > 8 ? 16 : 8;
   for (;; per_pass /= 2) {
     const int rows = static_cast<int>(m < per_pass ? m : per_pass), tt = per_pass > 8 ? 2 : 1;
-    int64_t best = LLONG_MAX;
+      int64_t best = LLONG_MAX;
     for (int ck = 1; ck <= kMaxCluster; ck *= 2) {
       const int slice = (l.blocks + ck - 1) / ck;
       if (ck > 1 && (ck - 1) * slice >= l.blocks) break;  // a CTA without work
       for (int ws = 1; ws <= kWarps; ws *= 2) {
         if (ws > 1 && ws / 2 >= slice) break;
-        if (rows_smem(l, tt, ck, ws, slice, rows, kMinDepth) > kRowsSmem) continue;
+        const int run = slice >= 4 * ws ? 2 : 1;
+        if (rows_smem(l, tt, ck, ws, slice, rows, run * kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
         const int clusters = groups < sm_count / ck ? groups : sm_count / ck;
         const int64_t iters = (groups + clusters - 1) / clusters;
@@ -463,6 +525,7 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
         best = cost;
         a.ck = ck;
         a.slice = slice;
+        a.run = run;
         a.ws = ws;
         a.iters = static_cast<int>(iters);
       }
@@ -475,8 +538,8 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
   const int tt = per_pass > 8 ? 2 : 1;
   const int rows = static_cast<int>(m < per_pass ? m : per_pass);
   a.depth = kMaxDepth;
-  while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.depth) > kRowsSmem) --a.depth;
-  const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.depth));
+  while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.run * a.depth) > kRowsSmem) --a.depth;
+  const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.run * a.depth));
   const int groups = (l.n_tiles + kWarps / a.ws - 1) / (kWarps / a.ws);
   const int clusters = groups < sm_count / a.ck ? groups : sm_count / a.ck;
   PdlIo io;
