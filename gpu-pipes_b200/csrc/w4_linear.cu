@@ -16,11 +16,13 @@
 //   - A CTA of 16 warps owns a slice of K (one of `ck` CTAs of a cluster does; ck = 1: all of it),
 //     keeps its part of the x rows in shared memory and goes over column tiles of 16. `ws` warps
 //     share a tile, each taking every ws-th 128-row block, so together they read whole stretches.
-//   - Every warp streams its blocks through a ring of its own in shared memory: one lane starts the
-//     bulk copies (a block's codes and its scales, contiguous both), the warp waits on the slot's
-//     mbarrier, takes the slot into registers and hands it back at once. The loads of the next tiles
-//     go on while the sums of this one are joined. (Loads straight to registers, four blocks ahead,
-//     ended up waiting for one another: 40 us at 1 x 8192 x 28672.)
+//   - A producing thread streams the codes and scales through a ring of stages in shared memory. A
+//     stage is what the 16 warps take next: for each tile one stretch of ws * RUN neighbouring
+//     blocks, one bulk copy each for codes and scales. Waiting and loading stay out of the
+//     computing warps, whose loop is bound by its integer instructions (148 per block of 2,048 weights
+//     with a ring per warp that the warp itself fed, 101 without).
+//   - The codes of the next tiles are in flight while the sums of this one are joined by warps of
+//     their own.
 //   - The warps' sums are joined in shared memory, the CTAs' through distributed shared memory,
 //     both in a fixed order: results do not depend on timing.
 #include <climits>
@@ -32,15 +34,16 @@
 namespace gp {
 namespace {
 
-// Warps of a CTA (one CTA per SM): kWarps turn codes into sums, kJoinWarps add the sums up and store.
+// Warps of a CTA (one CTA per SM): kWarps turn codes into sums, kJoinWarps add the sums up and store,
+// one more loads.
 constexpr int kWarps = 16;
-constexpr int kJoinWarps = 4;
+constexpr int kJoinWarps = 3;
 constexpr int kJoiners = 32 * kJoinWarps;
-constexpr int kThreads = 32 * (kWarps + kJoinWarps);
+constexpr int kThreads = 32 * (kWarps + kJoinWarps + 1);
 constexpr int kPartStride = 20;     // floats per row of a warp's 16 x rows sums: conflict-free float2 stores
 constexpr int kMaxCluster = 8;
-constexpr int kMaxDepth = 8;        // ring slots per warp
-constexpr int kMinDepth = 3;
+constexpr int kMaxDepth = 8;        // ring stages
+constexpr int kMinDepth = 2;
 constexpr int kRowsSmem = kSmemLimit - 3072;  // dynamic: the barriers are static
 constexpr int kZeroBytes = 256;     // zeros in shared memory, read in place of absent x rows
 
@@ -51,15 +54,15 @@ struct W4RowsArgs {
   const void* bias;
   void* out;
   int64_t m;
+  int out_f32;
   int act;
   int ck;            // CTAs of a cluster, along K
   int slice;         // k-blocks of a CTA
-  int run;           // k-blocks of a ring slot (1 or 2), neighbours in the packed codes
   int ws;            // warps that share a column tile
   int iters;         // column tile groups per cluster
   int rows;          // x rows of a pass (at most 8 TT)
   int x_stride;      // bytes between x rows in shared memory
-  int depth;         // ring slots per warp
+  int depth;         // ring stages
   int* status;
   unsigned long long timeout_ns;
   int inject;        // fault injection: 1 = no block is ever loaded
@@ -120,11 +123,11 @@ __device__ __forceinline__ void lds_words(uint32_t p, uint32_t (&v)[W]) {
 // Named barriers of the CTA (0 is __syncthreads): waiting, and arriving without waiting.
 __device__ __forceinline__ void bar_sync(int id) {
   __syncwarp();
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(32 * (kWarps + kJoinWarps)) : "memory");
 }
 __device__ __forceinline__ void bar_arrive(int id) {
   __syncwarp();
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(32 * (kWarps + kJoinWarps)) : "memory");
 }
 constexpr int kBarFull = 1, kBarFree = 3;  // + buffer 0 / 1 of the warps' sums
 
@@ -136,19 +139,21 @@ __device__ __forceinline__ void st_async_f32x4(uint32_t addr, uint32_t bar, floa
                : "memory");
 }
 
-// TT: tiles of 8 x rows. UNITS: groups per k-block of 128.
-template <typename T, int TT, int UNITS, bool ZP, typename OutT>
+// TT: tiles of 8 x rows. UNITS: groups per k-block of 128. RUN: k-blocks of a ring slot, neighbours in the
+// packed codes.
+template <typename T, int TT, int UNITS, bool ZP, int RUN>
 __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_constant__ W4RowsArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);                // scale words of a lane per block
   constexpr int kPart = TT * 8 * kPartStride;                 // floats of a warp's sums
   constexpr int kScaleBytes = 32 * kWords;                    // scales of a block
-  constexpr int kSlot = kW4BlockBytes + kScaleBytes;
+  constexpr int kStageCodes = kWarps * RUN * kW4BlockBytes;   // a stage: codes of every warp, then scales
+  constexpr int kStage = kWarps * RUN * (kW4BlockBytes + kScaleBytes);
   constexpr float kUnit0 = W4Deq<T>::unit(0), kUnit1 = W4Deq<T>::unit(1);
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kWarps + kJoinWarps][kMaxDepth];
+  __shared__ __align__(8) uint64_t full[kMaxDepth], empty[kMaxDepth];
   __shared__ __align__(8) uint64_t red_full[2];
   __shared__ int abort_flag, join_abort;
-  float* part = reinterpret_cast<float*>(smem + kWarps * a.depth * a.run * kSlot);  // [2][kWarps][kPart]
+  float* part = reinterpret_cast<float*>(smem + a.depth * kStage);  // [2][kWarps][kPart]
   const int np = kWarps / a.ws;                               // tiles at a time
   const int outs = np * TT * 128;                             // sums of a tile group
   float* red = part + 2 * kWarps * kPart;                     // [2][outs], clusters only
@@ -165,62 +170,82 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   const int nb = min(a.slice, a.l.blocks - b0);               // blocks of this CTA
   const int sub = warp % a.ws, slot_tile = warp / a.ws;
 
-  // the run of blocks that is loaded next: tile and first block (relative to the slice) of this
-  // warp's; a warp without a block in the slice (and a joining one) loads nothing
-  const int tile_step = clusters * np, lead = sub * a.run, stride = a.ws * a.run, slot_bytes = a.run * kSlot;
-  int ld_tile = warp < kWarps && lead < nb ? cluster * np + slot_tile : INT_MAX, ld_rel = lead, ld_slot = 0;
-  const uint32_t ring = smem_u32(smem) + warp * a.depth * slot_bytes, bars = smem_u32(full[warp]);
-  const uint8_t* const codes0 = static_cast<const uint8_t*>(a.packed) + static_cast<int64_t>(b0) * kW4BlockBytes;
-  const uint8_t* const scales0 = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + static_cast<int64_t>(b0) * kScaleBytes;
-  int64_t ld_cell = static_cast<int64_t>(cluster * np + slot_tile) * a.l.blocks;
-  // one lane: the next run of the warp's sequence into the next slot
-  auto load = [&] {
-    if (ld_tile >= a.l.n_tiles || a.inject != 0) return;
-    const uint32_t bar = bars + ld_slot * 8, dst = ring + ld_slot * slot_bytes;
-    const int n = min(a.run, nb - ld_rel);
-    mbar_arrive_expect_tx(bar, n * kSlot);
-    bulk_load(dst, codes0 + (ld_cell + ld_rel) * kW4BlockBytes, n * kW4BlockBytes, bar);
-    bulk_load(dst + a.run * kW4BlockBytes, scales0 + (ld_cell + ld_rel) * kScaleBytes, n * kScaleBytes, bar);
-    ld_slot = ld_slot + 1 == a.depth ? 0 : ld_slot + 1;
-    ld_rel += stride;
-    if (ld_rel >= nb) {
-      ld_rel = lead;
-      ld_tile = tile_step < a.l.n_tiles - ld_tile ? ld_tile + tile_step : INT_MAX;
-      ld_cell += static_cast<int64_t>(tile_step) * a.l.blocks;
-    }
+  const int tile_step = clusters * np, lead = sub * RUN, stride = a.ws * RUN;
+  const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
+  bool ok = true;
+  // codes and scales of block `rel` of the slice in column tile `tile`
+  auto codes_at = [&](int tile, int rel) {
+    return static_cast<const uint8_t*>(a.packed) + (static_cast<int64_t>(tile) * a.l.blocks + b0 + rel) * kW4BlockBytes;
+  };
+  auto scales_at = [&](int tile, int rel) {
+    return static_cast<const uint8_t*>(a.packed) + a.l.scale_off +
+           (static_cast<int64_t>(tile) * a.l.blocks + b0 + rel) * kScaleBytes;
   };
 
-  // The first codes go into L2 while the previous kernel of the stream drains (a hint: nothing is
-  // read into the program before the wait).
-  if (ld_tile < a.l.n_tiles)
-    for (int i = 0; i < a.depth && lead + i * stride < nb; ++i) {
-      const int n = min(a.run, nb - lead - i * stride);
-      if (lane < 8 * n)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(codes0 + (ld_cell + lead + i * stride) * kW4BlockBytes + lane * 128));
-    }
-  if (lane == 0 && warp < kWarps)
-    for (int i = 0; i < a.depth; ++i) mbar_init(bars + i * 8, 1);
   if (threadIdx.x == 0) {
+    for (int i = 0; i < a.depth; ++i) {
+      mbar_init(smem_u32(&full[i]), 1);
+      mbar_init(smem_u32(&empty[i]), kWarps);
+    }
     mbar_init(smem_u32(&red_full[0]), 1);
     mbar_init(smem_u32(&red_full[1]), 1);
     abort_flag = join_abort = 0;
+    fence_mbar_init();
   }
-  if (lane == 0) fence_mbar_init();
+  // The first codes go into L2 while the previous kernel of the stream drains (a hint: nothing is
+  // read into the program before the wait).
+  if (warp < np && cluster * np + warp < a.l.n_tiles)
+    for (int i = lane; i < min(nb, a.depth * stride); i += 32)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(codes_at(cluster * np + warp, i)), "n"(kW4BlockBytes));
   pdl_wait_prior();
   pdl_launch_dependents();
-  if (lane == 0)
-    for (int i = 0; i < a.depth; ++i) load();
+  __syncthreads();  // barriers
+  // every CTA of the cluster runs before one writes into another's shared memory
+  if (a.ck > 1) cluster_sync_all();
 
+  if (warp == kWarps + kJoinWarps) {
+    // ---- loading, by one thread
+    if (lane == 0 && a.inject == 0) {
+      int stage = 0, phase = 0, issued = 0;
+      for (int it = 0; it < a.iters && ok; ++it)
+        for (int rel = 0; rel < nb; rel += stride) {
+          if (issued >= a.depth && !mbar_wait(smem_u32(&empty[stage]), phase ^ 1, wctx, kDevTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const int n = min(stride, nb - rel);
+          const int tile0 = (cluster + it * clusters) * np, tiles = min(np, a.l.n_tiles - tile0);
+          const uint32_t bar = smem_u32(&full[stage]), dst = smem_u32(smem) + stage * kStage;
+          mbar_arrive_expect_tx(bar, max(tiles, 0) * n * (kW4BlockBytes + kScaleBytes));
+          for (int i = 0; i < tiles; ++i) {
+            bulk_load(dst + i * stride * kW4BlockBytes, codes_at(tile0 + i, rel), n * kW4BlockBytes, bar);
+            bulk_load(dst + kStageCodes + i * stride * kScaleBytes, scales_at(tile0 + i, rel), n * kScaleBytes, bar);
+          }
+          ++issued;
+          if (++stage == a.depth) stage = 0, phase ^= 1;
+        }
+      // After a wait that ran out somewhere, the copies under way are waited for (again with a limit)
+      // before the CTA's shared memory goes away; otherwise the computing warps take every stage.
+      if (!ok)
+        for (int i = 0; i < a.depth; ++i) {
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(smem_u32(&full[stage]), phase ^ 1) && globaltimer_ns() - t0 < a.timeout_ns) {
+          }
+          if (++stage == a.depth) stage = 0, phase ^= 1;
+        }
+    }
+  } else {
   // x rows of this CTA's slice (zero past K) and their sums over each group. Sixteen lanes hold a
   // block of a row; absent rows have sums of zero and are read from the zeros.
+  constexpr int kStagers = 32 * (kWarps + kJoinWarps);
   if (threadIdx.x < kZeroBytes / 16) reinterpret_cast<uint4*>(zeros)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   {
     const int pieces = a.slice * 16;  // 16-byte pieces of a row
-    for (int i = threadIdx.x; i < (8 * TT - rows) * a.slice * UNITS; i += kThreads) {
+    for (int i = threadIdx.x; i < (8 * TT - rows) * a.slice * UNITS; i += kStagers) {
       const int dead = 8 * TT - rows;
       xsum[i / dead * (8 * TT) + rows + i % dead] = 0.0f;
     }
-    for (int i0 = 0; i0 < rows * pieces; i0 += kThreads) {
+    for (int i0 = 0; i0 < rows * pieces; i0 += kStagers) {
       const int i = i0 + threadIdx.x;
       const int r = i / pieces, c = i % pieces;
       const int k = b0 * kW4Block + c * 8;
@@ -234,13 +259,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       if (r < rows && c % (16 / UNITS) == 0) xsum[(c / (16 / UNITS)) * (8 * TT) + r] = sum;
     }
   }
-  __syncthreads();
-  // every CTA of the cluster runs before one writes into another's shared memory
-  if (a.ck > 1) cluster_sync_all();
+  bar_sync(kBarFull);  // x is in place (this barrier's first use as a buffer's comes after)
 
-  const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
-  int slot = 0, phase = 0;
-  bool ok = true;
   if (warp >= kWarps) {
     // ---- joining: part[warp][row][column] of a tile group, summed over its warps (and CTAs)
     const int j = threadIdx.x - 32 * kWarps;
@@ -250,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
     // are all sent and so arrive before any CTA leaves.
     const WaitCtx jctx{a.status, &join_abort, a.timeout_ns};
     const int quads = outs / 4, own = quads / a.ck;
-    const bool vec = a.l.n % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(OutT)) == 0;
+    const bool vec = a.l.n % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (a.out_f32 ? 16 : 8) == 0;
     for (int it = 0; it < a.iters; ++it) {
       const int tile0 = (cluster + it * clusters) * np, buf = it & 1;
       const float* pb = part + buf * (kWarps * kPart);
@@ -275,24 +295,25 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
           if (a.bias != nullptr && i < live) v[i] += Elem<T>::to_f(static_cast<const T*>(a.bias)[n + i]);
           v[i] = act_exact(a.act, v[i]);
         }
-        OutT* to = static_cast<OutT*>(a.out) + (row0 + row_of(q)) * a.l.n + n;
-        if constexpr (sizeof(OutT) == 4) {
+        const int64_t at = (row0 + row_of(q)) * a.l.n + n;
+        if (a.out_f32) {
+          float* to = static_cast<float*>(a.out) + at;
           if (vec) {
             *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
           } else {
-            for (int i = 0; i < live; ++i) to[i] = v[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i < live) to[i] = v[i];
           }
         } else {
+          uint16_t* to = static_cast<uint16_t*>(a.out) + at;
           const uint32_t lo = Elem<T>::pack(v[0], v[1]), hi = Elem<T>::pack(v[2], v[3]);
           if (vec) {
             *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
           } else {
-            uint16_t* h = reinterpret_cast<uint16_t*>(to);
-            const uint16_t e[4] = {static_cast<uint16_t>(lo), static_cast<uint16_t>(lo >> 16), static_cast<uint16_t>(hi),
-                                   static_cast<uint16_t>(hi >> 16)};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (i < live) h[i] = e[i];
+              if (i < live) to[i] = static_cast<uint16_t>((i < 2 ? lo : hi) >> (16 * (i & 1)));
           }
         }
       };
@@ -324,25 +345,25 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       }
     }
   } else {
-    // ---- codes to sums
-    uint32_t xr[TT], xmask[TT];
+    // ---- codes to sums. Addresses run along: this loop is bound by its integer instructions.
+    uint32_t xa0[TT], xstep[TT];
 #pragma unroll
-    for (int i = 0; i < TT; ++i) {
+    for (int i = 0; i < TT; ++i) {  // absent rows read the zeros again and again
       const bool live = i * 8 + g < rows;
-      xr[i] = smem_u32(live ? xs + (i * 8 + g) * a.x_stride : zeros) + t * 16;
-      xmask[i] = live ? 0xffffffffu : 0u;
+      xa0[i] = smem_u32(live ? xs + (i * 8 + g) * a.x_stride + lead * (kW4Block * 2) : zeros) + t * 16;
+      xstep[i] = live ? kW4Block * 2 : 0;
     }
+    const uint32_t xsum0 = smem_u32(xsum) + (lead * UNITS * 8 * TT + 2 * t) * 4;
+    constexpr int kXsumBlock = UNITS * 8 * TT * 4;
     float acc[TT][4];
-    // block `i` of the run in ring slot d; rel: its place in the slice
-    auto block = [&](uint32_t d, int i, int rel) {
-      const uint4 cbuf[2] = {lds128(d + i * kW4BlockBytes + lane * 16),
-                             lds128(d + i * kW4BlockBytes + kW4BlockBytes / 2 + lane * 16)};
+    // a block: codes and scales at c and s, x rows at xa, their group sums at xg
+    auto block = [&](uint32_t c, uint32_t s, const uint32_t (&xa)[TT], uint32_t xg) {
+      const uint4 cbuf[2] = {lds128(c), lds128(c + kW4BlockBytes / 2)};
       uint32_t sbuf[kWords];
-      lds_words<kWords>(d + a.run * kW4BlockBytes + i * kScaleBytes + g * (4 * kWords), sbuf);
+      lds_words<kWords>(s, sbuf);
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
         float sum[TT][4];
-        const float2 s = Elem<T>::unpack(sbuf[ZP ? 2 * u : u]);
         float2 z = make_float2(-8.0f - W4Deq<T>::kOffset, -8.0f - W4Deq<T>::kOffset);
         if constexpr (ZP) {
           z = Elem<T>::unpack(sbuf[2 * u + 1]);
@@ -353,7 +374,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
         z.y *= kUnit1;
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-          const float2 xv = *reinterpret_cast<const float2*>(xsum + (rel * UNITS + u) * (8 * TT) + i * 8 + 2 * t);
+          uint32_t v[2];
+          lds_words<2>(xg + u * (8 * TT * 4) + i * 32, v);
+          const float2 xv = make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
           sum[i][0] = z.x * xv.x;
           sum[i][1] = z.x * xv.y;
           sum[i][2] = z.y * xv.x;
@@ -361,41 +384,65 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
         }
 #pragma unroll
         for (int h = u * (4 / UNITS); h < (u + 1) * (4 / UNITS); ++h) {  // 32 rows at a time
-          const uint4 c = cbuf[h >> 1];
+          const uint4 cw = cbuf[h >> 1];
           uint32_t p0[4], p1[4];
-          W4Deq<T>::pairs((h & 1) ? c.z : c.x, p0);
-          W4Deq<T>::pairs((h & 1) ? c.w : c.y, p1);
+          W4Deq<T>::pairs((h & 1) ? cw.z : cw.x, p0);
+          W4Deq<T>::pairs((h & 1) ? cw.w : cw.y, p1);
 #pragma unroll
           for (int i = 0; i < TT; ++i) {
-            const uint4 xv = lds128(xr[i] + (static_cast<uint32_t>(rel * (kW4Block * 2)) & xmask[i]) + h * 64);
+            const uint4 xv = lds128(xa[i] + h * 64);
             mma16816<T>(sum[i], p0, xv.x, xv.y);
             mma16816<T>(sum[i], p1, xv.z, xv.w);
           }
         }
+        const float2 sc = Elem<T>::unpack(sbuf[ZP ? 2 * u : u]);
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-          acc[i][0] = fmaf(s.x, sum[i][0], acc[i][0]);
-          acc[i][1] = fmaf(s.x, sum[i][1], acc[i][1]);
-          acc[i][2] = fmaf(s.y, sum[i][2], acc[i][2]);
-          acc[i][3] = fmaf(s.y, sum[i][3], acc[i][3]);
+          acc[i][0] = fmaf(sc.x, sum[i][0], acc[i][0]);
+          acc[i][1] = fmaf(sc.x, sum[i][1], acc[i][1]);
+          acc[i][2] = fmaf(sc.y, sum[i][2], acc[i][2]);
+          acc[i][3] = fmaf(sc.y, sum[i][3], acc[i][3]);
         }
       }
     };
+    // this warp's place in a stage
+    const uint32_t c0 = smem_u32(smem) + (slot_tile * stride + lead) * kW4BlockBytes + lane * 16;
+    const uint32_t to_scales = smem_u32(smem) + kStageCodes + (slot_tile * stride + lead) * kScaleBytes + g * (4 * kWords) - c0;
+    int stage = 0, phase = 0;
+    uint32_t cs = c0;
     for (int it = 0, tile = cluster * np + slot_tile; it < a.iters; ++it, tile += tile_step) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-      if (tile < a.l.n_tiles)
-        for (int rel = lead; rel < nb; rel += stride) {
-          if (!mbar_wait(bars + slot * 8, phase, wctx, kDevTimeoutProducer)) ok = false;
-          ok = __all_sync(0xffffffffu, ok) != 0;
-          if (!ok) break;  // nothing is read; the joins go on, so no barrier is missed
-          const uint32_t d = ring + slot * slot_bytes;
-          block(d, 0, rel);
-          if (a.run == 2 && rel + 1 < nb) block(d, 1, rel + 1);
-          if (++slot == a.depth) slot = 0, phase ^= 1;
-          __syncwarp();
-          if (lane == 0) load();
+      uint32_t xa[TT], xg = xsum0;
+#pragma unroll
+      for (int i = 0; i < TT; ++i) xa[i] = xa0[i];
+      // blocks left for this warp from `lead` on, run by run; every warp takes part in every stage
+      int left = tile < a.l.n_tiles ? nb - lead : 0;
+      for (int rel = 0; rel < nb && ok; rel += stride) {
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[stage]), phase, wctx, kDevTimeoutProducer))) {
+          ok = false;  // nothing is read; the joins go on, so no barrier is missed
+          break;
         }
+        const uint32_t s = cs + to_scales;
+        uint32_t xb[TT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) xb[i] = xa[i];
+#pragma unroll
+        for (int b = 0; b < RUN; ++b) {
+          if (b >= left) break;
+          block(cs + b * kW4BlockBytes, s + b * kScaleBytes, xb, xg + b * kXsumBlock);
+#pragma unroll
+          for (int i = 0; i < TT; ++i) xb[i] += xstep[i];
+        }
+        left -= stride;
+#pragma unroll
+        for (int i = 0; i < TT; ++i) xa[i] += stride * xstep[i];
+        xg += stride * kXsumBlock;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&empty[stage]));
+        cs += kStage;
+        if (++stage == a.depth) stage = 0, phase ^= 1, cs = c0;
+      }
       const int buf = it & 1;
       float* pb = part + buf * (kWarps * kPart) + warp * kPart;
       if (it >= 2) bar_sync(kBarFree + buf);
@@ -408,16 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       bar_arrive(kBarFull + buf);
     }
   }
-  // After a wait that ran out, the copies that were started are waited for (again with a limit)
-  // before the CTA's shared memory goes away; otherwise every copy has been taken above.
-  if (!ok && lane == 0 && a.inject == 0) {
-    for (int i = 0; i < a.depth; ++i) {
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(bars + slot * 8, phase) && globaltimer_ns() - t0 < a.timeout_ns) {
-      }
-      if (++slot == a.depth) slot = 0, phase ^= 1;
-    }
-  }
+  }  // not loading
   // no CTA leaves while another may still write into its shared memory
   if (a.ck > 1) {
     __syncwarp();
@@ -434,10 +472,10 @@ int64_t rows_smem(const W4Layout& l, int tt, int ck, int ws, int slice, int rows
          kZeroBytes + static_cast<int64_t>(rows) * rows_x_stride(slice);
 }
 
-template <typename T, int TT, int UNITS, bool ZP, typename OutT>
+template <typename T, int TT, int UNITS, bool ZP, int RUN>
 int rows_launch(const W4RowsArgs& a, int smem, int clusters, int64_t row_tiles, cudaStream_t s, const PdlIo& io) {
   static unsigned long long done_mask = 0;
-  auto kern = &w4_rows_kernel<T, TT, UNITS, ZP, OutT>;
+  auto kern = &w4_rows_kernel<T, TT, UNITS, ZP, RUN>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kRowsSmem, &done_mask);
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -468,23 +506,29 @@ int rows_launch(const W4RowsArgs& a, int smem, int clusters, int64_t row_tiles, 
   return e == cudaSuccess ? GP_OK : set_error(GP_ERR_CUDA, "w4 linear launch: %s", cudaGetErrorString(e));
 }
 
-template <typename T, int TT, int UNITS, typename OutT>
-int rows_zeros(const W4RowsArgs& a, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  return a.l.zeros ? rows_launch<T, TT, UNITS, true, OutT>(a, smem, clusters, rt, s, io)
-                   : rows_launch<T, TT, UNITS, false, OutT>(a, smem, clusters, rt, s, io);
+template <typename T, int TT, int UNITS, bool ZP>
+int rows_run(const W4RowsArgs& a, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return run == 4 ? rows_launch<T, TT, UNITS, ZP, 4>(a, smem, clusters, rt, s, io)
+                  : rows_launch<T, TT, UNITS, ZP, 2>(a, smem, clusters, rt, s, io);
 }
 
-template <typename T, int TT, typename OutT>
-int rows_dispatch(const W4RowsArgs& a, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  return a.l.units == 1   ? rows_zeros<T, TT, 1, OutT>(a, smem, clusters, rt, s, io)
-         : a.l.units == 2 ? rows_zeros<T, TT, 2, OutT>(a, smem, clusters, rt, s, io)
-                          : rows_zeros<T, TT, 4, OutT>(a, smem, clusters, rt, s, io);
+template <typename T, int TT, int UNITS>
+int rows_zeros(const W4RowsArgs& a, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return a.l.zeros ? rows_run<T, TT, UNITS, true>(a, run, smem, clusters, rt, s, io)
+                   : rows_run<T, TT, UNITS, false>(a, run, smem, clusters, rt, s, io);
 }
 
-template <typename T, typename OutT>
-int rows_tt(const W4RowsArgs& a, int tt, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  return tt == 1 ? rows_dispatch<T, 1, OutT>(a, smem, clusters, rt, s, io)
-                 : rows_dispatch<T, 2, OutT>(a, smem, clusters, rt, s, io);
+template <typename T, int TT>
+int rows_units(const W4RowsArgs& a, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return a.l.units == 1   ? rows_zeros<T, TT, 1>(a, run, smem, clusters, rt, s, io)
+         : a.l.units == 2 ? rows_zeros<T, TT, 2>(a, run, smem, clusters, rt, s, io)
+                          : rows_zeros<T, TT, 4>(a, run, smem, clusters, rt, s, io);
+}
+
+template <typename T>
+int rows_tt(const W4RowsArgs& a, int tt, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return tt == 1 ? rows_units<T, 1>(a, run, smem, clusters, rt, s, io)
+                 : rows_units<T, 2>(a, run, smem, clusters, rt, s, io);
 }
 
 }  // namespace
@@ -501,12 +545,13 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
   a.packed = packed;
   a.bias = bias;
   a.out = out;
+  a.out_f32 = out_f32;
   a.act = act;
   // Split of the work: ck CTAs of a cluster along K, ws warps per column tile. A tile group costs
   // its warps' blocks plus a join (about one block's time within a CTA, about three more across a
   // cluster); the fewest rounds of that over the GPU's SMs win. A pass takes up to 16 rows, fewer
   // where they would not fit in shared memory even spread over eight CTAs.
-  int per_pass = m > 8 ? 16 : 8;
+  int per_pass = m > 8 ? 16 : 8, run = 2;
   for (;; per_pass /= 2) {
     const int rows = static_cast<int>(m < per_pass ? m : per_pass), tt = per_pass > 8 ? 2 : 1;
       int64_t best = LLONG_MAX;
@@ -515,8 +560,8 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
       if (ck > 1 && (ck - 1) * slice >= l.blocks) break;  // a CTA without work
       for (int ws = 1; ws <= kWarps; ws *= 2) {
         if (ws > 1 && ws / 2 >= slice) break;
-        const int run = slice >= 4 * ws ? 2 : 1;
-        if (rows_smem(l, tt, ck, ws, slice, rows, run * kMinDepth) > kRowsSmem) continue;
+        const int r = slice >= 4 * ws && rows_smem(l, tt, ck, ws, slice, rows, 4 * 3) <= kRowsSmem ? 4 : 2;
+        if (rows_smem(l, tt, ck, ws, slice, rows, r * kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
         const int clusters = groups < sm_count / ck ? groups : sm_count / ck;
         const int64_t iters = (groups + clusters - 1) / clusters;
@@ -525,7 +570,7 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
         best = cost;
         a.ck = ck;
         a.slice = slice;
-        a.run = run;
+        run = r;
         a.ws = ws;
         a.iters = static_cast<int>(iters);
       }
@@ -538,8 +583,8 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
   const int tt = per_pass > 8 ? 2 : 1;
   const int rows = static_cast<int>(m < per_pass ? m : per_pass);
   a.depth = kMaxDepth;
-  while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.run * a.depth) > kRowsSmem) --a.depth;
-  const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, a.run * a.depth));
+  while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth) > kRowsSmem) --a.depth;
+  const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth));
   const int groups = (l.n_tiles + kWarps / a.ws - 1) / (kWarps / a.ws);
   const int clusters = groups < sm_count / a.ck ? groups : sm_count / a.ck;
   PdlIo io;
@@ -553,12 +598,8 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
     c.out = static_cast<char*>(out) + r0 * l.n * (out_f32 ? 4 : 2);
     const int64_t rt = (c.m + per_pass - 1) / per_pass;
     int rc;
-    if (dtype == GP_BF16)
-      rc = out_f32 ? rows_tt<__nv_bfloat16, float>(c, tt, smem, clusters, rt, s, io)
-                   : rows_tt<__nv_bfloat16, __nv_bfloat16>(c, tt, smem, clusters, rt, s, io);
-    else
-      rc = out_f32 ? rows_tt<__half, float>(c, tt, smem, clusters, rt, s, io)
-                   : rows_tt<__half, __half>(c, tt, smem, clusters, rt, s, io);
+    rc = dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(c, tt, run, smem, clusters, rt, s, io)
+                          : rows_tt<__half>(c, tt, run, smem, clusters, rt, s, io);
     if (rc != GP_OK) return rc;
     count_launches(1);
   }
