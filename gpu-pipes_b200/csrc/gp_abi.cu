@@ -627,7 +627,7 @@ static int w4_linear(const W4Layout& l, int dtype, int64_t m, int act, const voi
   DeviceInfo dev;
   const int rc = device_info(&dev);
   if (rc != GP_OK) return rc;
-  return launch_w4_linear(l, dtype, m, x, packed, bias, act, out, out_f32, stream, dev);
+  return launch_w4_linear({l, dtype, m, x, packed, bias, act, out, out_f32}, stream, dev);
 }
 
 static uint64_t align256(uint64_t b) { return (b + 255) / 256 * 256; }

@@ -5,7 +5,7 @@
 // instructions take them, so a product reads them in 16-byte pieces and rearranges nothing:
 //   codes   [n-tile of 16][k-block of 128][64-row part 2][lane 32][word 4]   1,024 bytes per block
 //     lane = 4 g + t holds columns n = 16 tile + 2 g + r (r = 0, 1) and, of each 32-row half h of a
-//     part, rows k = 32 h + 8 t + 4 j + i (word = 2 h + j, i = 0..3). The code of (r, i) is nibble
+//     part, rows k = 32 h + 16 j + 4 t + i (word = 2 h + j, i = 0..3). The code of (r, i) is nibble
 //     4 (i & 1) + 2 (i >> 1) + r of the word: rows i, i + 1 sit 16 bits apart, so one mask takes
 //     both values of a 16-bit pair. bf16 words are rotated left by 3 bits (see W4Deq).
 //   scales  [n-tile][k-block][g 8][group of the block][r 2] T; with zero points [..][group]{s0, s1, z0, z1}
@@ -106,6 +106,17 @@ __device__ __forceinline__ uint32_t w4_load_word(uint32_t v) {
   return __funnelshift_r(v, v, W4Deq<T>::kRotate);
 }
 
+// Activations of the epilogues, in fp32 and not approximated: next to the weights they cost nothing.
+__device__ __forceinline__ float w4_act(int act, float v) {
+  switch (act) {
+    case kActRelu: return v > 0.0f ? v : (v == v ? 0.0f : v);
+    case kActGeluTanh: return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * v, v * v, v)));
+    case kActSilu: return v / (1.0f + expf(-v));
+    case kActSigmoid: return 1.0f / (1.0f + expf(-v));
+    default: return v;
+  }
+}
+
 // ---- host interface (w4_pack.cu, w4_linear.cu); dtype is GP_F16 / GP_BF16
 int launch_w4_quantize(const W4Layout& l, int dtype, const void* w, void* packed, cudaStream_t s);
 int launch_w4_pack(const W4Layout& l, int dtype, const uint8_t* codes, const void* scales, const uint8_t* zeros,
@@ -115,7 +126,19 @@ int launch_w4_unpack(const W4Layout& l, int dtype, const void* packed, uint8_t* 
 int launch_w4_dequantize(const W4Layout& l, int dtype, const void* packed, void* w, cudaStream_t s);
 
 // out [m, n] = act(x [m, k] W + bias), out in T or fp32 (out_f32); x rows are read 16 bytes at a time
-int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, const void* packed, const void* bias,
-                     int act, void* out, bool out_f32, cudaStream_t s, const DeviceInfo& dev);
+struct W4LinearArgs {
+  W4Layout l;
+  int dtype;
+  int64_t m;
+  const void* x;
+  const void* packed;
+  const void* bias;
+  int act;
+  void* out;
+  bool out_f32;
+};
+int launch_w4_rows(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev);   // few rows (w4_linear.cu)
+int launch_w4_tiles(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev);  // more rows (w4_tiles.cu)
+int launch_w4_linear(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev);
 
 }  // namespace gp

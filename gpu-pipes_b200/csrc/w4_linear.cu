@@ -26,6 +26,7 @@
 //   - The warps' sums are joined in shared memory, the CTAs' through distributed shared memory,
 //     both in a fixed order: results do not depend on timing.
 #include <climits>
+#include <cstdlib>
 
 #include "../../include/gpipes.h"
 #include "chain_registry.h"
@@ -67,17 +68,6 @@ struct W4RowsArgs {
   unsigned long long timeout_ns;
   int inject;        // fault injection: 1 = no block is ever loaded
 };
-
-// exact forms: with few rows the epilogue costs nothing, so nothing is approximated
-__device__ __forceinline__ float act_exact(int act, float v) {
-  switch (act) {
-    case GP_ACT_RELU: return v > 0.0f ? v : (v == v ? 0.0f : v);
-    case GP_ACT_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * v, v * v, v)));
-    case GP_ACT_SILU: return v / (1.0f + expf(-v));
-    case GP_ACT_SIGMOID: return 1.0f / (1.0f + expf(-v));
-    default: return v;
-  }
-}
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -251,7 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       const int k = b0 * kW4Block + c * 8;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < rows && k < a.l.k) v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (row0 + r) * a.l.k + k);
-      if (r < rows) *reinterpret_cast<uint4*>(xs + r * a.x_stride + c * 16) = v;
+      if (r < rows) {  // rows 16 j + 4 t + i of a 32-row half where lane t reads them as 16 bytes, j by j
+        uint8_t* to = xs + r * a.x_stride + (c >> 2) * 64 + (c & 1) * 32 + ((c >> 1) & 1) * 8;
+        *reinterpret_cast<uint2*>(to) = make_uint2(v.x, v.y);
+        *reinterpret_cast<uint2*>(to + 16) = make_uint2(v.z, v.w);
+      }
       const float2 f0 = Elem<T>::unpack(v.x), f1 = Elem<T>::unpack(v.y), f2 = Elem<T>::unpack(v.z), f3 = Elem<T>::unpack(v.w);
       float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
 #pragma unroll
@@ -293,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (a.bias != nullptr && i < live) v[i] += Elem<T>::to_f(static_cast<const T*>(a.bias)[n + i]);
-          v[i] = act_exact(a.act, v[i]);
+          v[i] = w4_act(a.act, v[i]);
         }
         const int64_t at = (row0 + row_of(q)) * a.l.n + n;
         if (a.out_f32) {
@@ -533,20 +527,19 @@ int rows_tt(const W4RowsArgs& a, int tt, int run, int smem, int clusters, int64_
 
 }  // namespace
 
-int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, const void* packed, const void* bias,
-                     int act, void* out, bool out_f32, cudaStream_t s, const DeviceInfo& dev) {
+int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev) {
+  const W4Layout& l = in.l;
+  const int64_t m = in.m;
   const int sm_count = dev.sm_count;
   W4RowsArgs a;
   a.status = dev.status;
   a.timeout_ns = current_timeout_ns();
   a.inject = current_fault_injection();
   a.l = l;
-  a.x = x;
-  a.packed = packed;
-  a.bias = bias;
-  a.out = out;
-  a.out_f32 = out_f32;
-  a.act = act;
+  a.packed = in.packed;
+  a.bias = in.bias;
+  a.out_f32 = in.out_f32;
+  a.act = in.act;
   // Split of the work: ck CTAs of a cluster along K, ws warps per column tile. A tile group costs
   // its warps' blocks plus a join (about one block's time within a CTA, about three more across a
   // cluster); the fewest rounds of that over the GPU's SMs win. A pass takes up to 16 rows, fewer
@@ -558,14 +551,17 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
     for (int ck = 1; ck <= kMaxCluster; ck *= 2) {
       const int slice = (l.blocks + ck - 1) / ck;
       if (ck > 1 && (ck - 1) * slice >= l.blocks) break;  // a CTA without work
-      for (int ws = 1; ws <= kWarps; ws *= 2) {
-        if (ws > 1 && ws / 2 >= slice) break;
-        const int r = slice >= 4 * ws && rows_smem(l, tt, ck, ws, slice, rows, 4 * 3) <= kRowsSmem ? 4 : 2;
+      for (int ws = kWarps; ws >= 1; ws /= 2) {
+        if (ws > 1 && ws / 2 >= slice) continue;  // warps without a block
+        if (slice > 4 * ws && ws < kWarps) break; // more than four blocks a warp: rather more warps per tile
+        const int per_warp = (slice + ws - 1) / ws;
+        int r = per_warp > 2 ? 4 : 2;
+        if (rows_smem(l, tt, ck, ws, slice, rows, 4 * 3) > kRowsSmem) r = 2;
         if (rows_smem(l, tt, ck, ws, slice, rows, r * kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
         const int clusters = groups < sm_count / ck ? groups : sm_count / ck;
         const int64_t iters = (groups + clusters - 1) / clusters;
-        const int64_t cost = iters * ((slice + ws - 1) / ws + 1 + (ck > 1 ? 3 : 0));
+        const int64_t cost = iters * (2 * per_warp + 3) + (ck > 1 ? 6 : 0);
         if (cost >= best) continue;
         best = cost;
         a.ck = ck;
@@ -588,22 +584,28 @@ int launch_w4_linear(const W4Layout& l, int dtype, int64_t m, const void* x, con
   const int groups = (l.n_tiles + kWarps / a.ws - 1) / (kWarps / a.ws);
   const int clusters = groups < sm_count / a.ck ? groups : sm_count / a.ck;
   PdlIo io;
-  io.add(PdlIo::kWrite, out, static_cast<uint64_t>(m) * l.n * (out_f32 ? 4 : 2));
+  io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(m) * l.n * (in.out_f32 ? 4 : 2));
   // the grid's y dimension holds 65,535 row tiles; longer inputs go in several launches
   const int64_t step = 65535ll * per_pass;
   for (int64_t r0 = 0; r0 < m; r0 += step) {
     W4RowsArgs c = a;
     c.m = m - r0 < step ? m - r0 : step;
-    c.x = static_cast<const char*>(x) + r0 * l.k * 2;
-    c.out = static_cast<char*>(out) + r0 * l.n * (out_f32 ? 4 : 2);
+    c.x = static_cast<const char*>(in.x) + r0 * l.k * 2;
+    c.out = static_cast<char*>(in.out) + r0 * l.n * (in.out_f32 ? 4 : 2);
     const int64_t rt = (c.m + per_pass - 1) / per_pass;
     int rc;
-    rc = dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(c, tt, run, smem, clusters, rt, s, io)
+    rc = in.dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(c, tt, run, smem, clusters, rt, s, io)
                           : rows_tt<__half>(c, tt, run, smem, clusters, rt, s, io);
     if (rc != GP_OK) return rc;
     count_launches(1);
   }
   return GP_OK;
+}
+
+int launch_w4_linear(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev) {
+  static const int force = [] { const char* e = std::getenv("GP_W4_PATH"); return e ? std::atoi(e) : 0; }();
+  if (force) return force == 1 ? launch_w4_rows(a, s, dev) : launch_w4_tiles(a, s, dev);
+  return a.m <= 16 ? launch_w4_rows(a, s, dev) : launch_w4_tiles(a, s, dev);
 }
 
 }  // namespace gp

@@ -76,7 +76,7 @@ __device__ __forceinline__ void put_half(uint4* block_pair, int h, F&& q) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) w[j] |= q(r, 8 * t + 4 * j + i) << (4 * w4_nibble(r, i));
+        for (int r = 0; r < 2; ++r) w[j] |= q(r, 16 * j + 4 * t + i) << (4 * w4_nibble(r, i));
     }
     reinterpret_cast<uint2*>(block_pair + t)[h] = make_uint2(w4_store_word<T>(w[0]), w4_store_word<T>(w[1]));
   }
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_unpack_kernel(const __grid_co
 #pragma unroll
         for (int e = 0; e < 16; ++e) {  // word 2 h + j, row i of it
           const int wi = e >> 2, i = e & 3;
-          const int k = static_cast<int>(b) * 64 + (wi >> 1) * 32 + 8 * t + 4 * (wi & 1) + i;
+          const int k = static_cast<int>(b) * 64 + (wi >> 1) * 32 + 16 * (wi & 1) + 4 * t + i;
 #pragma unroll
           for (int r = 0; r < 2; ++r)
             if (k < l.k && at.c + r < l.n)
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_dequantize_kernel(const __gri
         const uint32_t wd[2] = {w4_load_word<T>(h == 0 ? u[t].x : u[t].z), w4_load_word<T>(h == 0 ? u[t].y : u[t].w)};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int j = e >> 2, i = e & 3, k = k0 + 8 * t + e;
+          const int j = e >> 2, i = e & 3, k = k0 + 16 * j + 4 * t + i;
           const float q0 = static_cast<float>((wd[j] >> (4 * w4_nibble(0, i))) & 15u);
           const float q1 = static_cast<float>((wd[j] >> (4 * w4_nibble(1, i))) & 15u);
           if (k < l.k) store_pair<VEC>(w, k, l.n, at.c, Elem<T>::pack(s.x * (q0 - z.x), s.y * (q1 - z.y)));

@@ -7,7 +7,7 @@ import torch
 
 from gpu_pipes_b200 import _lib as L
 from gpu_pipes_b200 import cuda_ext
-from tests._tol import U32, check, rounded
+from tests._tol import U32, check, half_step, rounded, tiny
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -56,16 +56,19 @@ def act64(a, v):
     return v
 
 
-def linear_ref(x, xerr, w, bias, act):
+def linear_ref(x, xerr, w, bias, act, dtype):
     """(act(x w + b), error bound before a store) for x within xerr. The sums: products of 16-bit
     values are exact in fp32; the matrix unit adds 16 at a time and may truncate, at most a step
     (2 U32) of the magnitudes per addition, K / 16 of them if none were independent, then at most
-    64 + 16 + 8 joins. An activation has slope at most 1.13 and costs a few half steps, tanh's
+    64 + 16 + 8 joins. More than 16 rows go to the kernel that rounds each weight to T, at most half a
+    step of it. An activation has slope at most 1.13 and costs a few half steps, tanh's
     cancellation among them (relative to |v|, not to the result)."""
     k = w.shape[0]
     v = x @ w
     mag = x.abs() @ w.abs()
     err = xerr @ w.abs() + 2 * U32 * (k / 16 + 96) * mag
+    if x.shape[0] > 16:
+        err = err + half_step(dtype) * (mag + xerr @ w.abs()) + tiny(dtype) * x.abs().sum(1, keepdim=True)
     if bias is not None:
         v, err = v + bias.double(), err + U32 * (v.abs() + bias.double().abs())
     if act not in (L.ACT_NONE, L.ACT_RELU):
@@ -186,7 +189,7 @@ def check_linear(m, k, n, dtype, group, zeros, act, bias, dev, seed=0):
     w4 = cuda_ext.w4_pack(codes, scales, z, group=group)
     buf = torch.full((m + 2, n), 7.0, dtype=dtype, device=dev)
     cuda_ext.w4_linear_out(x, w4, b, buf[:m], act=act)
-    ref, err = linear_ref(x.double(), torch.zeros_like(x, dtype=torch.float64), weights64(codes, scales, z, group), b, act)
+    ref, err = linear_ref(x.double(), torch.zeros_like(x, dtype=torch.float64), weights64(codes, scales, z, group), b, act, dtype)
     check(buf[:m], ref, rounded(ref, err, dtype), f"{m}x{k}x{n}")
     assert (buf[m:] == 7).all()  # rows behind the last stay
 
@@ -290,7 +293,7 @@ def mlp_ref(x, layers, biases, acts, tail, gamma, beta, eps, group, dtype):
     for i, (codes, scales, z) in enumerate(layers):
         last = i + 1 == len(layers)
         act = L.ACT_NONE if last and tail else acts[i]
-        v, err = linear_ref(v, err, weights64(codes, scales, z, group), biases[i], act)
+        v, err = linear_ref(v, err, weights64(codes, scales, z, group), biases[i], act, dtype)
         if not last:
             err = rounded(v, err, dtype)  # hidden activations are stored in 16 bits
     if not tail:
@@ -512,7 +515,7 @@ def test_device_refusals(cuda_dev):
 def test_missing_codes_time_out_and_the_next_call_is_right(cuda_dev):
     """With host-side fault injection no block of codes is ever loaded: every wait runs out after
     5 ms, the kernel ends, the status word says so, and the context stays usable."""
-    for m, k, n in ((1, 256, 64), (3, 4096, 48)):  # one CTA per tile, and a cluster along K
+    for m, k, n in ((1, 256, 64), (8, 16384, 48), (40, 256, 2000), (40, 4096, 48)):  # both kernels, alone and in clusters
         codes, scales, z = make(k, n, torch.float16, 64, True)
         w4 = cuda_ext.w4_pack(codes, scales, z, group=64)
         x = rows(m, k, torch.float16)
@@ -526,6 +529,6 @@ def test_missing_codes_time_out_and_the_next_call_is_right(cuda_dev):
         finally:
             L.set_fault_injection(0)
             L.set_timeout_ns(0)
-        assert L.device_status(0, clear=True) == 0x100
+        assert L.device_status(0, clear=True) in (0x100, 0x200, 0x300)  # whichever role gave up first
         assert torch.equal(cuda_ext.w4_linear(x, w4), want)
         assert L.device_status(0) == 0
