@@ -106,15 +106,36 @@ __device__ __forceinline__ uint32_t w4_load_word(uint32_t v) {
   return __funnelshift_r(v, v, W4Deq<T>::kRotate);
 }
 
-// Activations of the epilogues, in fp32 and not approximated: next to the weights they cost nothing.
-__device__ __forceinline__ float w4_act(int act, float v) {
-  switch (act) {
-    case kActRelu: return v > 0.0f ? v : (v == v ? 0.0f : v);
-    case kActGeluTanh: return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * v, v * v, v)));
-    case kActSilu: return v / (1.0f + expf(-v));
-    case kActSigmoid: return 1.0f / (1.0f + expf(-v));
-    default: return v;
+// W words from shared memory in one access (two for W = 8)
+template <int W>
+__device__ __forceinline__ void w4_lds(uint32_t p, uint32_t (&v)[W]) {
+  if constexpr (W == 1) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(p) : "memory");
+  } else if constexpr (W == 2) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(p) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+                   : "r"(p + 4 * i)
+                   : "memory");
   }
+}
+
+// Activations of the epilogues, in fp32 and not approximated: next to the weights they cost nothing.
+// The transcendental ones are a function call: they run once or twice per CTA, and copies of them in
+// an unrolled epilogue cost more in instruction fetches than the calls.
+static __device__ __noinline__ float w4_act_call(int act, float v) {
+  if (act == kActGeluTanh) return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * v, v * v, v)));
+  const float e = 1.0f + expf(-v);
+  return act == kActSilu ? v / e : 1.0f / e;
+}
+
+__device__ __forceinline__ float w4_act(int act, float v) {
+  if (act == kActNone) return v;
+  if (act == kActRelu) return v > 0.0f ? v : (v == v ? 0.0f : v);
+  return w4_act_call(act, v);
 }
 
 // ---- host interface (w4_pack.cu, w4_linear.cu); dtype is GP_F16 / GP_BF16

@@ -95,21 +95,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t p) {
   return v;
 }
 
-template <int W>
-__device__ __forceinline__ void lds_words(uint32_t p, uint32_t (&v)[W]) {
-  if constexpr (W == 1) {
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(p) : "memory");
-  } else if constexpr (W == 2) {
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(p) : "memory");
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; i += 4) {
-      const uint4 u = lds128(p + 4 * i);
-      v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
-    }
-  }
-}
-
 // Named barriers of the CTA (0 is __syncthreads): waiting, and arriving without waiting.
 __device__ __forceinline__ void bar_sync(int id) {
   __syncwarp();
@@ -354,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
     auto block = [&](uint32_t c, uint32_t s, const uint32_t (&xa)[TT], uint32_t xg) {
       const uint4 cbuf[2] = {lds128(c), lds128(c + kW4BlockBytes / 2)};
       uint32_t sbuf[kWords];
-      lds_words<kWords>(s, sbuf);
+      w4_lds<kWords>(s, sbuf);
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
         float sum[TT][4];
@@ -369,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
           uint32_t v[2];
-          lds_words<2>(xg + u * (8 * TT * 4) + i * 32, v);
+          w4_lds<2>(xg + u * (8 * TT * 4) + i * 32, v);
           const float2 xv = make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
           sum[i][0] = z.x * xv.x;
           sum[i][1] = z.x * xv.y;

@@ -12,10 +12,14 @@
 // w4_dequantize gives it; the sums are fp32. Scaling the sums instead, group by group, as the row
 // kernel does, would read the accumulator once per group: more time than the tile's product.
 //
-//   loader (1 warp)     x panels by TMA, codes and scales by bulk copies, a ring of 128-row stages
+//   loader (1 thread)   x panels of 64 columns by TMA into a ring of stages
 //   16 dequantising warps  four groups of four (one warp per TMEM lane quarter); a group takes every
-//                       fourth 64-row part: codes -> T -> its TMEM stage of 32 columns
-//   MMA issuer (1 thread) four K = 16 products per part; commits free the TMEM stage and the ring stage
+//                       fourth 64-row part. Each lane copies its own codes and scales with cp.async
+//                       into a private ring, four parts ahead, turns them into T in registers and
+//                       stores them to one of the group's two TMEM stages of 32 columns. (As bulk
+//                       copies, a part's codes are 16 pieces of 512 bytes and their scales: the copy
+//                       engine took about 1 us for a 128 x 128 block of them.)
+//   MMA issuer (1 thread) four K = 16 products per part; commits free the TMEM stage and the x stage
 //   epilogue            the dequantising warps: bias, activation, store
 // Where there are fewer tiles than SMs, a cluster of ck CTAs splits K and sums over distributed
 // shared memory in a fixed order.
@@ -31,8 +35,10 @@ constexpr int kDeqWarps = 4 * kDeqGroups;
 constexpr int kTileThreads = 32 * (2 + kDeqWarps);
 constexpr int kTileN = 128;        // columns of W per tile: the TMEM lanes
 constexpr int kTileTiles = kTileN / 16;
-constexpr int kAStages = kDeqGroups;  // TMEM stages of dequantised weights, 32 columns (64 rows of W) each
-constexpr int kMaxStages = 8;
+constexpr int kAStages = 2 * kDeqGroups;  // TMEM stages of dequantised weights, 32 columns (64 rows of W) each
+constexpr int kTmemCols = 512;            // 256 for the sums, 256 for the weights
+constexpr int kMaxStages = 8;       // x stages
+constexpr int kCodeDepth = 4;       // parts of codes in flight per warp
 constexpr int kMaxTileRows = 256;
 
 struct W4TileArgs {
@@ -48,17 +54,23 @@ struct W4TileArgs {
   int ck;          // CTAs of a cluster, along K
   int slice;       // k-blocks of a CTA
   int stages;
-  int tmem_cols;
   int* status;
   unsigned long long timeout_ns;
   int inject;
 };
 
-__device__ __forceinline__ void tile_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
+
+// scale words of a lane for a 64-row part of one column tile
+constexpr int part_words(int units, bool zp) { return (units == 4 ? 2 : 1) * (zp ? 2 : 1); }
+// a warp's slot: for its two column tiles, 16 bytes of codes and the scales of each lane
+constexpr int code_slot(int units, bool zp) { return 2 * 32 * (16 + 4 * part_words(units, zp)); }
 
 // 16 lanes x 32 columns: thread 4 g + t holds, per 8 columns, columns 2t and 2t + 1 of lane g, then of lane g + 8
 __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -68,6 +80,12 @@ __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
 
 // Codes of a lane as T: for the two columns r, the scale twice and the constant that takes the
@@ -135,24 +153,23 @@ struct TileDeq<__nv_bfloat16> {
 __device__ __forceinline__ int tile_column(int lane) { return (lane & ~15) + 2 * (lane & 7) + ((lane >> 3) & 1); }
 
 template <typename T, int UNITS, bool ZP>
-__global__ void __launch_bounds__(kTileThreads, 2)
+__global__ void __launch_bounds__(kTileThreads, 1)
     w4_tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ W4TileArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);
   constexpr int kScaleBytes = 32 * kWords;            // of a block of 16 columns
-  constexpr int kCodes = kTileTiles * kW4BlockBytes;  // of a stage
-  constexpr int kScales = kTileTiles * kScaleBytes;
+  constexpr int kPartWords = part_words(UNITS, ZP);
+  constexpr int kSlot = code_slot(UNITS, ZP);
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], a_full[kAStages], a_empty[kAStages], d_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
-  const int panel = a.rows * 128;                     // x rows of 64 columns, SWIZZLE_128B
-  const int stage_bytes = 2 * panel + kCodes + (kScales + 1023) / 1024 * 1024;
+  const int stage_bytes = a.rows * 128;               // x rows of 64 columns, SWIZZLE_128B
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = a.ck > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit = blockIdx.x / a.ck;
   const int tile0 = unit / a.row_tiles * kTileTiles;  // first 16-column tile
   const int64_t row0 = static_cast<int64_t>(unit % a.row_tiles) * a.rows;
-  const int b0 = rank * a.slice, nb = min(a.slice, a.l.blocks - b0);
+  const int b0 = rank * a.slice, parts = 2 * min(a.slice, a.l.blocks - b0);
   const int tiles = min(kTileTiles, a.l.n_tiles - tile0);
 
   if ((smem_u32(smem) & 1023u) != 0) {  // the same in every CTA of the grid
@@ -163,7 +180,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&empty[i]), 2 * 4 + 1);  // a block's two groups, and its products
+      mbar_init(smem_u32(&empty[i]), 1);
     }
     for (int i = 0; i < kAStages; ++i) {
       mbar_init(smem_u32(&a_full[i]), 4);
@@ -174,51 +191,41 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) prefetch_tmap(&tx);
+  // The first codes go into L2 while the previous kernel of the stream drains (a hint: nothing is
+  // read into the program before the wait).
+  if (warp >= 2 && warp < 2 + tiles && lane < min(parts, 16))
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                     static_cast<const uint8_t*>(a.packed) +
+                     (static_cast<int64_t>(tile0 + warp - 2) * a.l.blocks + b0) * kW4BlockBytes + lane * (kW4BlockBytes / 2)),
+                 "n"(kW4BlockBytes / 2));
   pdl_wait_prior();
   pdl_launch_dependents();
   if (warp == 1) {
-    tmem_alloc(smem_u32(&tmem_holder), a.tmem_cols);
+    tmem_alloc(smem_u32(&tmem_holder), kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (a.tmem_cols - kAStages * 32);
+  const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (kTmemCols - kAStages * 32);
   const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
   bool ok = true;  // of this role
 
   if (warp == 0) {
-    // lanes 0-7 the codes of a column tile each, lanes 8-15 its scales, lanes 16 and 17 the x panels:
-    // one thread issuing all eighteen copies of a stage took longer than the copies
-    if (a.inject == 0) {
+    if (lane == 0 && a.inject == 0) {
       const uint64_t keep = l2_policy_evict_last();  // x is read by every column tile
-      const int i = lane & 7;
-      const int64_t cell = static_cast<int64_t>(tile0 + i) * a.l.blocks + b0;
-      const uint8_t* src = static_cast<const uint8_t*>(a.packed) +
-                           (lane < 8 ? cell * kW4BlockBytes : a.l.scale_off + cell * kScaleBytes);
-      const uint32_t bytes = lane < 8 ? kW4BlockBytes : kScaleBytes;
-      const uint32_t to = 2 * panel + (lane < 8 ? i * kW4BlockBytes : kCodes + i * kScaleBytes);
       int s = 0, ph = 0;
-      for (int b = 0; b < nb; ++b) {
-        if (b >= a.stages) {
-          ok = mbar_wait(smem_u32(&empty[s]), ph ^ 1, wctx, kDevTimeoutProducer);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
+      for (int p = 0; p < parts; ++p) {
+        if (p >= a.stages && !mbar_wait(smem_u32(&empty[s]), ph ^ 1, wctx, kDevTimeoutProducer)) {
+          ok = false;
+          break;
         }
-        const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem) + s * stage_bytes;
-        if (lane == 0) mbar_arrive_expect_tx(bar, 2 * panel + tiles * (kW4BlockBytes + kScaleBytes));
-        __syncwarp();
-        if (lane < 16) {
-          if (i < tiles) tile_bulk_load(dst + to, src + b * static_cast<int64_t>(bytes), bytes, bar);
-        } else if (lane < 18) {
-          const int p = lane - 16;
-          tma_load_2d_hint(dst + p * panel, &tx, bar, (b0 + b) * kW4Block + p * 64, static_cast<int>(row0), keep);
-        }
+        mbar_arrive_expect_tx(smem_u32(&full[s]), stage_bytes);
+        tma_load_2d_hint(smem_u32(smem) + s * stage_bytes, &tx, smem_u32(&full[s]), b0 * kW4Block + p * 64,
+                         static_cast<int>(row0), keep);
         if (++s == a.stages) s = 0, ph ^= 1;
       }
-      if (!ok && lane == 0)  // copies under way end (waited for with a limit) before their memory is used again or goes away
+      if (!ok)  // copies under way end (waited for with a limit) before their memory is used again or goes away
         for (int j = 0; j < a.stages; ++j) {
           const uint64_t t0 = globaltimer_ns();
           while (!mbar_try_wait(smem_u32(&full[s]), ph ^ 1) && globaltimer_ns() - t0 < a.timeout_ns) {
@@ -231,22 +238,17 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     if (lane == 0) {
       const uint32_t idesc = make_idesc_f16(kTileN, a.rows, Elem<T>::kIsBf16, 0, 0);
       int s = 0, ph = 0, as = 0, aph = 0;
-      for (int b = 0; b < nb && ok; ++b) {
+      for (int p = 0; p < parts; ++p) {
         if (!mbar_wait(smem_u32(&full[s]), ph, wctx, kDevTimeoutMma)) break;
-        for (int p = 0; p < 2; ++p) {
-          if (!mbar_wait(smem_u32(&a_full[as]), aph, wctx, kDevTimeoutMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t bdesc = make_sdesc_sw128(smem_u32(smem) + s * stage_bytes + p * panel, 16, 1024);
+        if (!mbar_wait(smem_u32(&a_full[as]), aph, wctx, kDevTimeoutMma)) break;
+        tc_fence_after();
+        const uint64_t bdesc = make_sdesc_sw128(smem_u32(smem) + s * stage_bytes, 16, 1024);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ts(d_tmem, a_tmem + as * 32 + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, (b | p | k) != 0 ? 1u : 0u);
-          mma_commit(smem_u32(&a_empty[as]));
-          if (++as == kAStages) as = 0, aph ^= 1;
-        }
-        if (ok) mma_commit(smem_u32(&empty[s]));
+        for (int k = 0; k < 4; ++k)
+          mma_ts(d_tmem, a_tmem + as * 32 + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, (p | k) != 0 ? 1u : 0u);
+        mma_commit(smem_u32(&a_empty[as]));
+        mma_commit(smem_u32(&empty[s]));
+        if (++as == kAStages) as = 0, aph ^= 1;
         if (++s == a.stages) s = 0, ph ^= 1;
       }
       // every product issued has completed before TMEM is read or released
@@ -257,72 +259,85 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     }
   } else {
     const int q = warp & 3, group = (warp - 2) >> 2, g = lane >> 2;
-    int s = 0, ph = 0;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    // this group's parts are group, group + 4, ...: every other block, always the same TMEM stage
-    const int as = group;
-    auto next_stage = [&] {
-      if (++s == a.stages) s = 0, ph ^= 1;
+    const uint32_t ring = smem_u32(smem) + a.stages * stage_bytes + (warp - 2) * (kCodeDepth * kSlot);
+    // this warp's two column tiles of the tile's eight; an absent one stays zero
+    const bool have[2] = {2 * q < tiles, 2 * q + 1 < tiles};
+    const int64_t cell = static_cast<int64_t>(tile0 + 2 * q) * a.l.blocks + b0;
+    const uint8_t* codes = static_cast<const uint8_t*>(a.packed) + cell * kW4BlockBytes + lane * 16;
+    const uint8_t* scales = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + cell * kScaleBytes + g * (4 * kWords);
+    const int64_t next_codes = static_cast<int64_t>(a.l.blocks) * kW4BlockBytes;
+    const int64_t next_scales = static_cast<int64_t>(a.l.blocks) * kScaleBytes;
+    auto load = [&](int p, int slot) {
+      if (p < parts) {
+        const uint32_t d = ring + slot * kSlot;
+        // scales of the part in its block: the second half of the groups for an odd part, if it has its own
+        const uint8_t* sc = scales + (p >> 1) * kScaleBytes + (UNITS > 1 ? (p & 1) * (4 * kPartWords) : 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (have[i]) {
+            cp_async<16>(d + (i * 32 + lane) * 16, codes + p * (kW4BlockBytes / 2) + i * next_codes);
+            cp_async<4 * kPartWords>(d + 1024 + (i * 32 + lane) * (4 * kPartWords), sc + i * next_scales);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (group >= 2) next_stage();
-    for (int b = group >> 1, use = 0; b < nb; b += kDeqGroups / 2, ++use) {
-      ok = mbar_wait(smem_u32(&full[s]), ph, wctx, kDevTimeoutProducer) &&
-           (use == 0 || mbar_wait(smem_u32(&a_empty[as]), (use - 1) & 1, wctx, kDevTimeoutEpilogue));
+    // parts group, group + 4, ... in two TMEM stages in turn
+    if (a.inject == 0)
+      for (int i = 0; i < kCodeDepth - 1; ++i) load(group + i * kDeqGroups, i);
+    int slot = 0;
+    for (int p = group, use = 0; p < parts; p += kDeqGroups, ++use) {
+      load(p + (kCodeDepth - 1) * kDeqGroups, (slot + kCodeDepth - 1) % kCodeDepth);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kCodeDepth - 1) : "memory");
+      // codes to T in registers; the TMEM stage is only then waited for
+      const uint32_t d = ring + slot * kSlot;
+      slot = (slot + 1) % kCodeDepth;
+      uint32_t r[2][16];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t c[4] = {0, 0, 0, 0}, sw[kPartWords];
+#pragma unroll
+        for (int w = 0; w < kPartWords; ++w) sw[w] = 0;
+        if (have[i]) {
+          w4_lds<4>(d + (i * 32 + lane) * 16, c);
+          w4_lds<kPartWords>(d + 1024 + (i * 32 + lane) * (4 * kPartWords), sw);
+        }
+        TileDeq<T> dq;
+        dq.set(sw[0], sw[ZP ? 1 : 0], ZP);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (UNITS == 4 && h == 1) dq.set(sw[kPartWords / 2], sw[kPartWords - 1], ZP);
+          dq.word(c[2 * h], r[i] + 8 * h);
+          dq.word(c[2 * h + 1], r[i] + 8 * h + 4);
+        }
+      }
+      const int as = group + (use & 1) * kDeqGroups;
+      ok = use < 2 || mbar_wait(smem_u32(&a_empty[as]), ((use >> 1) - 1) & 1, wctx, kDevTimeoutEpilogue);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint8_t* st = smem + s * stage_bytes + 2 * panel;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int nt = 2 * q + i;  // column tile of this 16-lane half; absent ones hold old bytes: zeroed
-        uint4 c = make_uint4(0, 0, 0, 0);
-        uint32_t sw[kWords];
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) sw[w] = 0;
-        if (nt < tiles) {
-          c = *reinterpret_cast<const uint4*>(st + nt * kW4BlockBytes + (group & 1) * (kW4BlockBytes / 2) + lane * 16);
-#pragma unroll
-          for (int w = 0; w < kWords; ++w)
-            sw[w] = *reinterpret_cast<const uint32_t*>(st + kCodes + nt * kScaleBytes + (g * kWords + w) * 4);
-        }
-        uint32_t r[16];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int u = UNITS == 1 ? 0 : UNITS == 2 ? group & 1 : 2 * (group & 1) + h;
-          TileDeq<T> dq;
-          if constexpr (UNITS == 1) {
-            dq.set(sw[0], sw[ZP ? 1 : 0], ZP);
-          } else {  // constant indices: sw stays in registers
-            uint32_t s01 = 0, z01 = 0;
-#pragma unroll
-            for (int v = 0; v < UNITS; ++v)
-              if (v == u) s01 = sw[ZP ? 2 * v : v], z01 = ZP ? sw[2 * v + (ZP ? 1 : 0)] : 0u;
-            dq.set(s01, z01, ZP);
-          }
-          dq.word(h == 0 ? c.x : c.z, r + 8 * h);
-          dq.word(h == 0 ? c.y : c.w, r + 8 * h + 4);
-        }
-        tmem_st_16x256b_x4(a_tmem + as * 32 + lanes + (static_cast<uint32_t>(i * 16) << 16), r);
-      }
+      for (int i = 0; i < 2; ++i)
+        tmem_st_16x256b_x4(a_tmem + as * 32 + lanes + (static_cast<uint32_t>(i * 16) << 16), r[i]);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&a_full[as]));
-        mbar_arrive(smem_u32(&empty[s]));
-      }
-      for (int i = 0; i < kDeqGroups / 2; ++i) next_stage();
+      if (lane == 0) mbar_arrive(smem_u32(&a_full[as]));
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (ok) ok = mbar_wait(smem_u32(&d_full), 0, wctx, kDevTimeoutEpilogue);
     ok = __all_sync(0xffffffffu, ok) != 0;
     tc_fence_after();
   }
 
-  // ---- epilogue: each quarter's warps take every fourth 32 rows of x
+  // ---- epilogue: each quarter's warps take every fourth 8 rows of x (short loops: their code runs
+  // once per CTA, so its length is its cost)
   const int q = warp & 3, part = (warp - 2) >> 2, n = tile0 * 16 + q * 32 + tile_column(lane);
-  auto store = [&](int64_t row, float v, float bias) {
+  const bool has_n = warp >= 2 && n < a.l.n;
+  const float bias = has_n && a.bias != nullptr ? Elem<T>::to_f(static_cast<const T*>(a.bias)[n]) : 0.0f;
+  auto store = [&](int64_t row, float v) {
     v = w4_act(a.act, v + bias);
     if (a.out_f32) {
       static_cast<float*>(a.out)[row * a.l.n + n] = v;
@@ -330,67 +345,65 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       static_cast<uint16_t*>(a.out)[row * a.l.n + n] = static_cast<uint16_t>(Elem<T>::pack(v, 0.0f));
     }
   };
-  const bool has_n = warp >= 2 && n < a.l.n;
-  const float bias = has_n && a.bias != nullptr ? Elem<T>::to_f(static_cast<const T*>(a.bias)[n]) : 0.0f;
+  const uint32_t d_lanes = d_tmem + (static_cast<uint32_t>(q * 32) << 16);
   if (a.ck == 1) {
     if (warp >= 2 && ok)  // a wait that ran out leaves the rows unwritten
-      for (int c0 = part * 32; c0 < a.rows; c0 += 32 * kDeqGroups) {
-        if (row0 + c0 >= a.m) break;
-        uint32_t v[32];
-        tmem_ld32(d_tmem + (static_cast<uint32_t>(q * 32) << 16) + c0, v);
+#pragma unroll 1
+      for (int c0 = part * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * kDeqGroups) {
+        uint32_t v[8];
+        tmem_ld8(d_lanes + c0, v);
         tmem_wait_ld();
+        const int live = has_n ? static_cast<int>(min(static_cast<int64_t>(8), a.m - row0 - c0)) : 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (has_n && c0 + i < a.rows && row0 + c0 + i < a.m) store(row0 + c0 + i, __uint_as_float(v[i]), bias);
+        for (int i = 0; i < 8; ++i)
+          if (i < live) store(row0 + c0 + i, __uint_as_float(v[i]));
       }
   } else {
     // CTA r of the cluster finishes rows [r share, (r + 1) share) of the tile: sums [source][row][128]
-    // in its ring, which nothing uses after the first barrier
+    // in its shared memory, which nothing else uses after the first barrier
     const int share = a.rows / a.ck;
     __syncwarp();
     cluster_sync_all();
     if (warp >= 2)
-      for (int c0 = part * 32; c0 < a.rows; c0 += 32 * kDeqGroups) {
-        uint32_t v[32];
-        tmem_ld32(d_tmem + (static_cast<uint32_t>(q * 32) << 16) + c0, v);
+#pragma unroll 1
+      for (int c0 = part * 8; c0 < a.rows; c0 += 8 * kDeqGroups) {
+        uint32_t v[8];
+        tmem_ld8(d_lanes + c0, v);
         tmem_wait_ld();
+        int owner = c0 / share, r = c0 % share;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int c = c0 + i;
-          if (c >= a.rows) break;
-          const uint32_t at = smem_u32(smem) + ((rank * share + c % share) * kTileN + q * 32 + lane) * 4;
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(at, static_cast<uint32_t>(c / share))), "r"(v[i])
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t at = smem_u32(smem) + ((rank * share + r) * kTileN + q * 32 + lane) * 4;
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(at, static_cast<uint32_t>(owner))), "r"(v[i])
                        : "memory");
+          if (++r == share) r = 0, ++owner;
         }
       }
     __syncwarp();
     cluster_sync_all();
     if (warp >= 2 && ok)
+#pragma unroll 1
       for (int c = part; c < share; c += kDeqGroups) {
         const int64_t row = row0 + rank * share + c;
         float v = 0.0f;
         for (int i = 0; i < a.ck; ++i)
           v += reinterpret_cast<const float*>(smem)[(i * share + c) * kTileN + q * 32 + lane];
-        if (has_n && row < a.m) store(row, v, bias);
+        if (has_n && row < a.m) store(row, v);
       }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(d_tmem, a.tmem_cols);
+    tmem_dealloc(d_tmem, kTmemCols);
   }
-}
-
-int tile_stage_bytes(const W4Layout& l, int rows) {
-  return 2 * rows * 128 + kTileTiles * kW4BlockBytes + (kTileTiles * l.scale_bytes() + 1023) / 1024 * 1024;
 }
 
 template <typename T, int UNITS, bool ZP>
 int tile_launch(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int smem, cudaStream_t s, const PdlIo& io) {
   static unsigned long long done_mask = 0;
   auto kern = &w4_tile_kernel<T, UNITS, ZP>;
-  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kSmemLimit - 1024, &done_mask);
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kSmemLimit - 2048, &done_mask);
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
@@ -451,7 +464,6 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   const int64_t row_tiles = (in.m + kMaxTileRows - 1) / kMaxTileRows;
   a.rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
   a.row_tiles = static_cast<int>((in.m + a.rows - 1) / a.rows);
-  a.tmem_cols = a.rows + kAStages * 32 <= 256 ? 256 : 512;
   const int64_t units = static_cast<int64_t>((a.l.n_tiles + kTileTiles - 1) / kTileTiles) * a.row_tiles;
   // CTAs along K: the fewest rounds over the SMs, a round costing its blocks and about four more
   // (six more with the sums across a cluster)
@@ -466,12 +478,11 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
     a.slice = slice;
   }
   if (units * a.ck >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "w4 linear: m = %lld", (long long)in.m);
-  // two CTAs share an SM up to 64 rows
-  const int stage = tile_stage_bytes(a.l, a.rows);
-  const int budget = a.rows <= 64 ? kSmemLimit / 2 - 2048 : kSmemLimit - 1024;
-  a.stages = budget / stage;
+  const int stage = a.rows * 128;
+  const int rings = kDeqWarps * kCodeDepth * code_slot(a.l.units, a.l.zeros != 0);
+  a.stages = (kSmemLimit - 2048 - rings) / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  int smem = a.stages * stage;
+  int smem = a.stages * stage + rings;
   const int sums = a.ck > 1 ? a.rows * kTileN * 4 : 0;
   if (smem < sums) smem = sums;
   CUtensorMap tx;
