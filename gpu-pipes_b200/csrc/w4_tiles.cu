@@ -12,14 +12,15 @@
 // w4_dequantize gives it; the sums are fp32. Scaling the sums instead, group by group, as the row
 // kernel does, would read the accumulator once per group: more time than the tile's product.
 //
-//   loader (1 thread)   x panels of 64 columns by TMA into a ring of stages
-//   16 dequantising warps  four groups of four (one warp per TMEM lane quarter); a group takes every
-//                       fourth 64-row part. Each lane copies its own codes and scales with cp.async
-//                       into a private ring, four parts ahead, turns them into T in registers and
-//                       stores them to one of the group's two TMEM stages of 32 columns. (As bulk
-//                       copies, a part's codes are 16 pieces of 512 bytes and their scales: the copy
-//                       engine took about 1 us for a 128 x 128 block of them.)
-//   MMA issuer (1 thread) four K = 16 products per part; commits free the TMEM stage and the x stage
+// The unit is a k-block of 128 rows of W:
+//   loader (1 thread)   x panels (two of 64 columns) by TMA into a ring of stages
+//   16 dequantising warps  four groups of four (one warp per TMEM lane quarter); two groups make a
+//                       block, 64 rows each, the other two the next one. Each lane copies its own codes and scales with cp.async
+//                       into a private ring, four blocks ahead, turns them into T in registers and
+//                       stores them to one of four TMEM stages of 64 columns.
+//   MMA issuer (1 thread) eight K = 16 products per block; commits free the TMEM stage and the x stage.
+//                       Its waits and commits cost about 500 cycles a turn: with a turn per 64
+//                       rows they bounded the kernel (34 us at 64 x 4096 x 14336).
 //   epilogue            the dequantising warps: bias, activation, store
 // Where there are fewer tiles than SMs, a cluster of ck CTAs splits K and sums over distributed
 // shared memory in a fixed order.
@@ -35,7 +36,8 @@ constexpr int kDeqWarps = 4 * kDeqGroups;
 constexpr int kTileThreads = 32 * (2 + kDeqWarps);
 constexpr int kTileN = 128;        // columns of W per tile: the TMEM lanes
 constexpr int kTileTiles = kTileN / 16;
-constexpr int kAStages = 2 * kDeqGroups;  // TMEM stages of dequantised weights, 32 columns (64 rows of W) each
+constexpr int kAStages = 4;               // TMEM stages of dequantised weights, 64 columns (a block) each
+constexpr int kACols = 64;
 constexpr int kTmemCols = 512;            // 256 for the sums, 256 for the weights
 constexpr int kMaxStages = 8;       // x stages
 constexpr int kCodeDepth = 4;       // parts of codes in flight per warp
@@ -163,13 +165,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], a_full[kAStages], a_empty[kAStages], d_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
-  const int stage_bytes = a.rows * 128;               // x rows of 64 columns, SWIZZLE_128B
+  const int panel = a.rows * 128, stage_bytes = 2 * panel;  // x rows of 64 columns, SWIZZLE_128B
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = a.ck > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit = blockIdx.x / a.ck;
   const int tile0 = unit / a.row_tiles * kTileTiles;  // first 16-column tile
   const int64_t row0 = static_cast<int64_t>(unit % a.row_tiles) * a.rows;
-  const int b0 = rank * a.slice, parts = 2 * min(a.slice, a.l.blocks - b0);
+  const int b0 = rank * a.slice, nb = min(a.slice, a.l.blocks - b0);
   const int tiles = min(kTileTiles, a.l.n_tiles - tile0);
 
   if ((smem_u32(smem) & 1023u) != 0) {  // the same in every CTA of the grid
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(smem_u32(&empty[i]), 1);
     }
     for (int i = 0; i < kAStages; ++i) {
-      mbar_init(smem_u32(&a_full[i]), 4);
+      mbar_init(smem_u32(&a_full[i]), 8);
       mbar_init(smem_u32(&a_empty[i]), 1);
     }
     mbar_init(smem_u32(&d_full), 1);
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (warp == 0 && lane == 0) prefetch_tmap(&tx);
   // The first codes go into L2 while the previous kernel of the stream drains (a hint: nothing is
   // read into the program before the wait).
-  if (warp >= 2 && warp < 2 + tiles && lane < min(parts, 16))
+  if (warp >= 2 && warp < 2 + tiles && lane < min(2 * nb, 16))
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
                      static_cast<const uint8_t*>(a.packed) +
                      (static_cast<int64_t>(tile0 + warp - 2) * a.l.blocks + b0) * kW4BlockBytes + lane * (kW4BlockBytes / 2)),
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (kTmemCols - kAStages * 32);
+  const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (kTmemCols - kAStages * kACols);
   const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
   bool ok = true;  // of this role
 
@@ -215,14 +217,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (lane == 0 && a.inject == 0) {
       const uint64_t keep = l2_policy_evict_last();  // x is read by every column tile
       int s = 0, ph = 0;
-      for (int p = 0; p < parts; ++p) {
-        if (p >= a.stages && !mbar_wait(smem_u32(&empty[s]), ph ^ 1, wctx, kDevTimeoutProducer)) {
+      for (int b = 0; b < nb; ++b) {
+        if (b >= a.stages && !mbar_wait(smem_u32(&empty[s]), ph ^ 1, wctx, kDevTimeoutProducer)) {
           ok = false;
           break;
         }
         mbar_arrive_expect_tx(smem_u32(&full[s]), stage_bytes);
-        tma_load_2d_hint(smem_u32(smem) + s * stage_bytes, &tx, smem_u32(&full[s]), b0 * kW4Block + p * 64,
-                         static_cast<int>(row0), keep);
+        for (int p = 0; p < 2; ++p)
+          tma_load_2d_hint(smem_u32(smem) + s * stage_bytes + p * panel, &tx, smem_u32(&full[s]),
+                           (b0 + b) * kW4Block + p * 64, static_cast<int>(row0), keep);
         if (++s == a.stages) s = 0, ph ^= 1;
       }
       if (!ok)  // copies under way end (waited for with a limit) before their memory is used again or goes away
@@ -238,14 +241,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (lane == 0) {
       const uint32_t idesc = make_idesc_f16(kTileN, a.rows, Elem<T>::kIsBf16, 0, 0);
       int s = 0, ph = 0, as = 0, aph = 0;
-      for (int p = 0; p < parts; ++p) {
+      for (int b = 0; b < nb; ++b) {
         if (!mbar_wait(smem_u32(&full[s]), ph, wctx, kDevTimeoutMma)) break;
         if (!mbar_wait(smem_u32(&a_full[as]), aph, wctx, kDevTimeoutMma)) break;
         tc_fence_after();
         const uint64_t bdesc = make_sdesc_sw128(smem_u32(smem) + s * stage_bytes, 16, 1024);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_ts(d_tmem, a_tmem + as * 32 + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, (p | k) != 0 ? 1u : 0u);
+        for (int k = 0; k < 8; ++k)
+          mma_ts(d_tmem, a_tmem + as * kACols + k * 8, bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2),
+                 idesc, (b | k) != 0 ? 1u : 0u);
         mma_commit(smem_u32(&a_empty[as]));
         mma_commit(smem_u32(&empty[s]));
         if (++as == kAStages) as = 0, aph ^= 1;
@@ -268,26 +272,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint8_t* scales = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + cell * kScaleBytes + g * (4 * kWords);
     const int64_t next_codes = static_cast<int64_t>(a.l.blocks) * kW4BlockBytes;
     const int64_t next_scales = static_cast<int64_t>(a.l.blocks) * kScaleBytes;
-    auto load = [&](int p, int slot) {
-      if (p < parts) {
+    // this group's blocks: every other one; of a block its first or second 64 rows, with the second
+    // half's groups where it has its own
+    const int part = group & 1;
+    codes += part * (kW4BlockBytes / 2);
+    scales += UNITS > 1 ? part * (4 * kPartWords) : 0;
+    auto load = [&](int b, int slot) {
+      if (b < nb) {
         const uint32_t d = ring + slot * kSlot;
-        // scales of the part in its block: the second half of the groups for an odd part, if it has its own
-        const uint8_t* sc = scales + (p >> 1) * kScaleBytes + (UNITS > 1 ? (p & 1) * (4 * kPartWords) : 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (have[i]) {
-            cp_async<16>(d + (i * 32 + lane) * 16, codes + p * (kW4BlockBytes / 2) + i * next_codes);
-            cp_async<4 * kPartWords>(d + 1024 + (i * 32 + lane) * (4 * kPartWords), sc + i * next_scales);
+            cp_async<16>(d + (i * 32 + lane) * 16, codes + b * kW4BlockBytes + i * next_codes);
+            cp_async<4 * kPartWords>(d + 1024 + (i * 32 + lane) * (4 * kPartWords), scales + b * kScaleBytes + i * next_scales);
           }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // parts group, group + 4, ... in two TMEM stages in turn
-    if (a.inject == 0)
-      for (int i = 0; i < kCodeDepth - 1; ++i) load(group + i * kDeqGroups, i);
+    const int b_first = group >> 1;
+    for (int i = 0; i < kCodeDepth - 1; ++i) load(b_first + 2 * i, i);
     int slot = 0;
-    for (int p = group, use = 0; p < parts; p += kDeqGroups, ++use) {
-      load(p + (kCodeDepth - 1) * kDeqGroups, (slot + kCodeDepth - 1) % kCodeDepth);
+    for (int b = b_first; b < nb; b += 2) {
+      load(b + 2 * (kCodeDepth - 1), (slot + kCodeDepth - 1) % kCodeDepth);
       asm volatile("cp.async.wait_group %0;" ::"n"(kCodeDepth - 1) : "memory");
       // codes to T in registers; the TMEM stage is only then waited for
       const uint32_t d = ring + slot * kSlot;
@@ -311,8 +317,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           dq.word(c[2 * h + 1], r[i] + 8 * h + 4);
         }
       }
-      const int as = group + (use & 1) * kDeqGroups;
-      ok = use < 2 || mbar_wait(smem_u32(&a_empty[as]), ((use >> 1) - 1) & 1, wctx, kDevTimeoutEpilogue);
+      const int as = b % kAStages, use = b / kAStages;
+      ok = use == 0 || mbar_wait(smem_u32(&a_empty[as]), (use - 1) & 1, wctx, kDevTimeoutEpilogue);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
@@ -320,7 +326,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        tmem_st_16x256b_x4(a_tmem + as * 32 + lanes + (static_cast<uint32_t>(i * 16) << 16), r[i]);
+        tmem_st_16x256b_x4(a_tmem + as * kACols + part * 32 + lanes + (static_cast<uint32_t>(i * 16) << 16), r[i]);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   // ---- epilogue: each quarter's warps take every fourth 8 rows of x (short loops: their code runs
   // once per CTA, so its length is its cost)
-  const int q = warp & 3, part = (warp - 2) >> 2, n = tile0 * 16 + q * 32 + tile_column(lane);
+  const int q = warp & 3, quarter = (warp - 2) >> 2, n = tile0 * 16 + q * 32 + tile_column(lane);
   const bool has_n = warp >= 2 && n < a.l.n;
   const float bias = has_n && a.bias != nullptr ? Elem<T>::to_f(static_cast<const T*>(a.bias)[n]) : 0.0f;
   auto store = [&](int64_t row, float v) {
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (a.ck == 1) {
     if (warp >= 2 && ok)  // a wait that ran out leaves the rows unwritten
 #pragma unroll 1
-      for (int c0 = part * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * kDeqGroups) {
+      for (int c0 = quarter * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * kDeqGroups) {
         uint32_t v[8];
         tmem_ld8(d_lanes + c0, v);
         tmem_wait_ld();
@@ -366,7 +372,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     cluster_sync_all();
     if (warp >= 2)
 #pragma unroll 1
-      for (int c0 = part * 8; c0 < a.rows; c0 += 8 * kDeqGroups) {
+      for (int c0 = quarter * 8; c0 < a.rows; c0 += 8 * kDeqGroups) {
         uint32_t v[8];
         tmem_ld8(d_lanes + c0, v);
         tmem_wait_ld();
@@ -383,7 +389,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     cluster_sync_all();
     if (warp >= 2 && ok)
 #pragma unroll 1
-      for (int c = part; c < share; c += kDeqGroups) {
+      for (int c = quarter; c < share; c += kDeqGroups) {
         const int64_t row = row0 + rank * share + c;
         float v = 0.0f;
         for (int i = 0; i < a.ck; ++i)
@@ -478,7 +484,7 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
     a.slice = slice;
   }
   if (units * a.ck >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "w4 linear: m = %lld", (long long)in.m);
-  const int stage = a.rows * 128;
+  const int stage = 2 * a.rows * 128;
   const int rings = kDeqWarps * kCodeDepth * code_slot(a.l.units, a.l.zeros != 0);
   a.stages = (kSmemLimit - 2048 - rings) / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
