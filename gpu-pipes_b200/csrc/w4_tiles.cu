@@ -14,13 +14,14 @@
 //
 // The unit is a k-block of 128 rows of W:
 //   loader (1 thread)   x panels (two of 64 columns) by TMA into a ring of stages
-//   16 dequantising warps  four groups of four (one warp per TMEM lane quarter); two groups make a
-//                       block, 64 rows each, the other two the next one. Each lane copies its own codes and scales with cp.async
-//                       into a private ring, four blocks ahead, turns them into T in registers and
-//                       stores them to one of four TMEM stages of 64 columns.
+//   16 dequantising warps  four groups of four (one warp per TMEM lane quarter); a group makes every
+//                       fourth block. Each lane copies its own codes and scales with cp.async into a
+//                       private ring, one or two blocks ahead, turns them into T in registers and
+//                       stores them to the group's TMEM stage of 64 columns. A turn's waits and
+//                       fences take as long as the conversion of 64 rows does, hence whole blocks.
 //   MMA issuer (1 thread) eight K = 16 products per block; commits free the TMEM stage and the x stage.
-//                       Its waits and commits cost about 500 cycles a turn: with a turn per 64
-//                       rows they bounded the kernel (34 us at 64 x 4096 x 14336).
+//                       Up to 128 rows of x the products alternate between two accumulators: one
+//                       that waits for the sum of the last takes about 58 cycles at any such width.
 //   epilogue            the dequantising warps: bias, activation, store
 // Where there are fewer tiles than SMs, a cluster of ck CTAs splits K and sums over distributed
 // shared memory in a fixed order.
@@ -36,11 +37,10 @@ constexpr int kDeqWarps = 4 * kDeqGroups;
 constexpr int kTileThreads = 32 * (2 + kDeqWarps);
 constexpr int kTileN = 128;        // columns of W per tile: the TMEM lanes
 constexpr int kTileTiles = kTileN / 16;
-constexpr int kAStages = 4;               // TMEM stages of dequantised weights, 64 columns (a block) each
+constexpr int kAStages = kDeqGroups;      // TMEM stages of dequantised weights, 64 columns (a block) each
 constexpr int kACols = 64;
 constexpr int kTmemCols = 512;            // 256 for the sums, 256 for the weights
 constexpr int kMaxStages = 8;       // x stages
-constexpr int kCodeDepth = 4;       // parts of codes in flight per warp
 constexpr int kMaxTileRows = 256;
 
 struct W4TileArgs {
@@ -55,7 +55,8 @@ struct W4TileArgs {
   int row_tiles;
   int ck;          // CTAs of a cluster, along K
   int slice;       // k-blocks of a CTA
-  int stages;
+  int stages;      // x stages
+  int depth;       // slots of a warp's code ring (2 or 3)
   int* status;
   unsigned long long timeout_ns;
   int inject;
@@ -69,10 +70,8 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 
-// scale words of a lane for a 64-row part of one column tile
-constexpr int part_words(int units, bool zp) { return (units == 4 ? 2 : 1) * (zp ? 2 : 1); }
-// a warp's slot: for its two column tiles, 16 bytes of codes and the scales of each lane
-constexpr int code_slot(int units, bool zp) { return 2 * 32 * (16 + 4 * part_words(units, zp)); }
+// a warp's slot: for its two column tiles, 32 bytes of codes and the scales of each lane
+constexpr int code_slot(int units, bool zp) { return 2 * 32 * (32 + 4 * units * (zp ? 2 : 1)); }
 
 // 16 lanes x 32 columns: thread 4 g + t holds, per 8 columns, columns 2t and 2t + 1 of lane g, then of lane g + 8
 __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -159,7 +158,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     w4_tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ W4TileArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);
   constexpr int kScaleBytes = 32 * kWords;            // of a block of 16 columns
-  constexpr int kPartWords = part_words(UNITS, ZP);
   constexpr int kSlot = code_slot(UNITS, ZP);
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], a_full[kAStages], a_empty[kAStages], d_full;
@@ -185,7 +183,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(smem_u32(&empty[i]), 1);
     }
     for (int i = 0; i < kAStages; ++i) {
-      mbar_init(smem_u32(&a_full[i]), 8);
+      mbar_init(smem_u32(&a_full[i]), 4);
       mbar_init(smem_u32(&a_empty[i]), 1);
     }
     mbar_init(smem_u32(&d_full), 1);
@@ -210,6 +208,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (kTmemCols - kAStages * kACols);
+  const uint32_t second = a.rows <= 128 ? a.rows : 0;  // the second accumulator's first column, if there is one
   const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
   bool ok = true;  // of this role
 
@@ -248,8 +247,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint64_t bdesc = make_sdesc_sw128(smem_u32(smem) + s * stage_bytes, 16, 1024);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          mma_ts(d_tmem, a_tmem + as * kACols + k * 8, bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2),
-                 idesc, (b | k) != 0 ? 1u : 0u);
+          mma_ts(d_tmem + (k & 1) * second, a_tmem + as * kACols + k * 8,
+                 bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2), idesc,
+                 (b != 0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u);
         mma_commit(smem_u32(&a_empty[as]));
         mma_commit(smem_u32(&empty[s]));
         if (++as == kAStages) as = 0, aph ^= 1;
@@ -264,73 +264,89 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   } else {
     const int q = warp & 3, group = (warp - 2) >> 2, g = lane >> 2;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t ring = smem_u32(smem) + a.stages * stage_bytes + (warp - 2) * (kCodeDepth * kSlot);
+    const uint32_t ring = smem_u32(smem) + a.stages * stage_bytes + (warp - 2) * (a.depth * kSlot);
     // this warp's two column tiles of the tile's eight; an absent one stays zero
     const bool have[2] = {2 * q < tiles, 2 * q + 1 < tiles};
-    const int64_t cell = static_cast<int64_t>(tile0 + 2 * q) * a.l.blocks + b0;
-    const uint8_t* codes = static_cast<const uint8_t*>(a.packed) + cell * kW4BlockBytes + lane * 16;
-    const uint8_t* scales = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + cell * kScaleBytes + g * (4 * kWords);
-    const int64_t next_codes = static_cast<int64_t>(a.l.blocks) * kW4BlockBytes;
-    const int64_t next_scales = static_cast<int64_t>(a.l.blocks) * kScaleBytes;
-    // this group's blocks: every other one; of a block its first or second 64 rows, with the second
-    // half's groups where it has its own
-    const int part = group & 1;
-    codes += part * (kW4BlockBytes / 2);
-    scales += UNITS > 1 ? part * (4 * kPartWords) : 0;
-    auto load = [&](int b, int slot) {
-      if (b < nb) {
-        const uint32_t d = ring + slot * kSlot;
+    const uint8_t *codes[2], *scales[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+      const int64_t cell = static_cast<int64_t>(tile0 + 2 * q + i) * a.l.blocks + b0 + group;
+      codes[i] = static_cast<const uint8_t*>(a.packed) + cell * kW4BlockBytes + lane * 16;
+      scales[i] = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + cell * kScaleBytes + g * (4 * kWords);
+    }
+    const uint32_t my_codes = ring + lane * 16, my_scales = ring + 2048 + lane * (4 * kWords);
+    const uint32_t ring_end = a.depth * kSlot;
+    int ld_b = group;
+    uint32_t ld_at = 0;  // byte offset of the slot that is filled next
+    auto load = [&] {
+      if (ld_b < nb) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           if (have[i]) {
-            cp_async<16>(d + (i * 32 + lane) * 16, codes + b * kW4BlockBytes + i * next_codes);
-            cp_async<4 * kPartWords>(d + 1024 + (i * 32 + lane) * (4 * kPartWords), scales + b * kScaleBytes + i * next_scales);
+            cp_async<16>(my_codes + ld_at + i * 1024, codes[i]);
+            cp_async<16>(my_codes + ld_at + i * 1024 + 512, codes[i] + kW4BlockBytes / 2);
+            if constexpr (kWords == 8) {
+              cp_async<16>(my_scales + ld_at + i * (128 * kWords), scales[i]);
+              cp_async<16>(my_scales + ld_at + i * (128 * kWords) + 16, scales[i] + 16);
+            } else {
+              cp_async<4 * kWords>(my_scales + ld_at + i * (128 * kWords), scales[i]);
+            }
           }
+          codes[i] += kDeqGroups * kW4BlockBytes;
+          scales[i] += kDeqGroups * kScaleBytes;
+        }
       }
+      ld_b += kDeqGroups;
+      ld_at = ld_at + kSlot == ring_end ? 0 : ld_at + kSlot;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const int b_first = group >> 1;
-    for (int i = 0; i < kCodeDepth - 1; ++i) load(b_first + 2 * i, i);
-    int slot = 0;
-    for (int b = b_first; b < nb; b += 2) {
-      load(b + 2 * (kCodeDepth - 1), (slot + kCodeDepth - 1) % kCodeDepth);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kCodeDepth - 1) : "memory");
-      // codes to T in registers; the TMEM stage is only then waited for
-      const uint32_t d = ring + slot * kSlot;
-      slot = (slot + 1) % kCodeDepth;
-      uint32_t r[2][16];
+    for (int i = 1; i < a.depth; ++i) load();
+    uint32_t at = 0;
+    const uint32_t a_stage = a_tmem + group * kACols + lanes;
+    int parity = 1;  // of the stage's last use
+    for (int b = group; b < nb; b += kDeqGroups, parity ^= 1) {
+      load();
+      if (a.depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t c[4] = {0, 0, 0, 0}, sw[kPartWords];
+      for (int part = 0; part < 2; ++part) {
+        // 64 rows to T in registers; the TMEM stage is only then waited for
+        uint32_t r[2][16];
 #pragma unroll
-        for (int w = 0; w < kPartWords; ++w) sw[w] = 0;
-        if (have[i]) {
-          w4_lds<4>(d + (i * 32 + lane) * 16, c);
-          w4_lds<kPartWords>(d + 1024 + (i * 32 + lane) * (4 * kPartWords), sw);
+        for (int i = 0; i < 2; ++i) {
+          uint32_t c[4] = {0, 0, 0, 0}, sw[kWords];
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) sw[w] = 0;
+          if (have[i]) {
+            w4_lds<4>(my_codes + at + i * 1024 + part * 512, c);
+            w4_lds<kWords>(my_scales + at + i * (128 * kWords), sw);
+          }
+          TileDeq<T> dq;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            constexpr int kStep = ZP ? 2 : 1;
+            const int u = (UNITS == 1 ? 0 : UNITS == 2 ? part : 2 * part + h) * kStep;
+            if (UNITS == 4 || h == 0) dq.set(sw[u], sw[u + kStep - 1], ZP);
+            dq.word(c[2 * h], r[i] + 8 * h);
+            dq.word(c[2 * h + 1], r[i] + 8 * h + 4);
+          }
         }
-        TileDeq<T> dq;
-        dq.set(sw[0], sw[ZP ? 1 : 0], ZP);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (UNITS == 4 && h == 1) dq.set(sw[kPartWords / 2], sw[kPartWords - 1], ZP);
-          dq.word(c[2 * h], r[i] + 8 * h);
-          dq.word(c[2 * h + 1], r[i] + 8 * h + 4);
+        if (part == 0) {
+          ok = b == group || mbar_wait(smem_u32(&a_empty[group]), parity, wctx, kDevTimeoutEpilogue);
+          ok = __all_sync(0xffffffffu, ok) != 0;
+          if (!ok) break;
+          tc_fence_after();
         }
-      }
-      const int as = b % kAStages, use = b / kAStages;
-      ok = use == 0 || mbar_wait(smem_u32(&a_empty[as]), (use - 1) & 1, wctx, kDevTimeoutEpilogue);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        tmem_st_16x256b_x4(a_tmem + as * kACols + part * 32 + lanes + (static_cast<uint32_t>(i * 16) << 16), r[i]);
+        for (int i = 0; i < 2; ++i)
+          tmem_st_16x256b_x4(a_stage + part * 32 + (static_cast<uint32_t>(i * 16) << 16), r[i]);
+      }
+      if (!ok) break;
+      at = at + kSlot == ring_end ? 0 : at + kSlot;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&a_full[as]));
+      if (lane == 0) mbar_arrive(smem_u32(&a_full[group]));
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (ok) ok = mbar_wait(smem_u32(&d_full), 0, wctx, kDevTimeoutEpilogue);
@@ -352,17 +368,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   };
   const uint32_t d_lanes = d_tmem + (static_cast<uint32_t>(q * 32) << 16);
+  auto load_sums = [&](int c0, float (&v)[8]) {
+    uint32_t u[8], w[8];
+    tmem_ld8(d_lanes + c0, u);
+    if (second != 0) tmem_ld8(d_lanes + second + c0, w);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]) + (second != 0 ? __uint_as_float(w[i]) : 0.0f);
+  };
   if (a.ck == 1) {
     if (warp >= 2 && ok)  // a wait that ran out leaves the rows unwritten
 #pragma unroll 1
       for (int c0 = quarter * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * kDeqGroups) {
-        uint32_t v[8];
-        tmem_ld8(d_lanes + c0, v);
-        tmem_wait_ld();
+        float v[8];
+        load_sums(c0, v);
         const int live = has_n ? static_cast<int>(min(static_cast<int64_t>(8), a.m - row0 - c0)) : 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (i < live) store(row0 + c0 + i, __uint_as_float(v[i]));
+          if (i < live) store(row0 + c0 + i, v[i]);
       }
   } else {
     // CTA r of the cluster finishes rows [r share, (r + 1) share) of the tile: sums [source][row][128]
@@ -373,14 +396,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp >= 2)
 #pragma unroll 1
       for (int c0 = quarter * 8; c0 < a.rows; c0 += 8 * kDeqGroups) {
-        uint32_t v[8];
-        tmem_ld8(d_lanes + c0, v);
-        tmem_wait_ld();
+        float v[8];
+        load_sums(c0, v);
         int owner = c0 / share, r = c0 % share;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint32_t at = smem_u32(smem) + ((rank * share + r) * kTileN + q * 32 + lane) * 4;
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(at, static_cast<uint32_t>(owner))), "r"(v[i])
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(at, static_cast<uint32_t>(owner))), "f"(v[i])
                        : "memory");
           if (++r == share) r = 0, ++owner;
         }
@@ -467,7 +489,10 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   a.timeout_ns = current_timeout_ns();
   a.inject = current_fault_injection();
   // rows per tile: as even as multiples of 16 up to 256 allow
-  const int64_t row_tiles = (in.m + kMaxTileRows - 1) / kMaxTileRows;
+  // (128 where the scales and zero points of small groups take the shared memory)
+  const int slot = kDeqWarps * code_slot(a.l.units, a.l.zeros != 0);
+  const int max_rows = slot > 49152 ? kMaxTileRows / 2 : kMaxTileRows;
+  const int64_t row_tiles = (in.m + max_rows - 1) / max_rows;
   a.rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
   a.row_tiles = static_cast<int>((in.m + a.rows - 1) / a.rows);
   const int64_t units = static_cast<int64_t>((a.l.n_tiles + kTileTiles - 1) / kTileTiles) * a.row_tiles;
@@ -485,7 +510,8 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   }
   if (units * a.ck >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "w4 linear: m = %lld", (long long)in.m);
   const int stage = 2 * a.rows * 128;
-  const int rings = kDeqWarps * kCodeDepth * code_slot(a.l.units, a.l.zeros != 0);
+  a.depth = a.rows <= 128 && 3 * slot <= kSmemLimit / 2 ? 3 : 2;
+  const int rings = a.depth * slot;
   a.stages = (kSmemLimit - 2048 - rings) / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   int smem = a.stages * stage + rings;
