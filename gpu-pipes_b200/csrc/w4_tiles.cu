@@ -73,6 +73,13 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
 // a warp's slot: for its two column tiles, 32 bytes of codes and the scales of each lane
 constexpr int code_slot(int units, bool zp) { return 2 * 32 * (32 + 4 * units * (zp ? 2 : 1)); }
 
+// One lane of the (converged) warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+
 // 16 lanes x 32 columns: thread 4 g + t holds, per 8 columns, columns 2t and 2t + 1 of lane g, then of lane g + 8
 __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -237,30 +244,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = make_idesc_f16(kTileN, a.rows, Elem<T>::kIsBf16, 0, 0);
-      int s = 0, ph = 0, as = 0, aph = 0;
-      for (int b = 0; b < nb; ++b) {
-        if (!mbar_wait(smem_u32(&full[s]), ph, wctx, kDevTimeoutMma)) break;
-        if (!mbar_wait(smem_u32(&a_full[as]), aph, wctx, kDevTimeoutMma)) break;
-        tc_fence_after();
-        const uint64_t bdesc = make_sdesc_sw128(smem_u32(smem) + s * stage_bytes, 16, 1024);
+    // The whole warp runs the loop and one elected lane issues: the compiler then sees addresses and
+    // descriptors that are the same in all lanes and keeps them in uniform registers, where the
+    // product wants them (from a branch on lane 0, each product took 72 cycles to issue).
+    const uint32_t idesc = make_idesc_f16(kTileN, a.rows, Elem<T>::kIsBf16, 0, 0);
+    const uint32_t d = __shfl_sync(0xffffffffu, d_tmem, 0), at0 = __shfl_sync(0xffffffffu, a_tmem, 0);
+    const uint64_t desc0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
+    const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), a_full0 = smem_u32(a_full), a_empty0 = smem_u32(a_empty);
+    int s = 0, ph = 0, as = 0, aph = 0;
+    for (int b = 0; b < nb; ++b) {
+      ok = mbar_wait(full0 + s * 8, ph, wctx, kDevTimeoutMma) && mbar_wait(a_full0 + as * 8, aph, wctx, kDevTimeoutMma);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint64_t bdesc = desc0 + static_cast<uint64_t>(s * (stage_bytes >> 4));
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          mma_ts(d_tmem + (k & 1) * second, a_tmem + as * kACols + k * 8,
+          mma_ts(d + (k & 1) * second, at0 + as * kACols + k * 8,
                  bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2), idesc,
                  (b != 0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u);
-        mma_commit(smem_u32(&a_empty[as]));
-        mma_commit(smem_u32(&empty[s]));
-        if (++as == kAStages) as = 0, aph ^= 1;
-        if (++s == a.stages) s = 0, ph ^= 1;
+        mma_commit(a_empty0 + as * 8);
+        mma_commit(empty0 + s * 8);
       }
-      // every product issued has completed before TMEM is read or released
-      mma_commit(smem_u32(&d_full));
-      volatile int no_abort = 0;
-      const WaitCtx drain{a.status, &no_abort, a.timeout_ns};
-      mbar_wait(smem_u32(&d_full), 0, drain, kDevTimeoutMma);
+      __syncwarp();
+      if (++as == kAStages) as = 0, aph ^= 1;
+      if (++s == a.stages) s = 0, ph ^= 1;
     }
+    // every product issued has completed before TMEM is read or released
+    if (elect_one()) mma_commit(smem_u32(&d_full));
+    __syncwarp();
+    volatile int no_abort = 0;
+    const WaitCtx drain{a.status, &no_abort, a.timeout_ns};
+    mbar_wait(smem_u32(&d_full), 0, drain, kDevTimeoutMma);
+    __syncwarp();
   } else {
     const int q = warp & 3, group = (warp - 2) >> 2, g = lane >> 2;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
