@@ -106,6 +106,67 @@ __device__ __forceinline__ uint32_t w4_load_word(uint32_t v) {
   return __funnelshift_r(v, v, W4Deq<T>::kRotate);
 }
 
+// Codes of a lane as T, s (q - z) rounded once: for the two columns r, the scale twice and the constant that takes the
+// zero point and the code's offset away (both steps exact before the scale).
+//   half: 1024 + q minus 1024 + z; column 1 four bits higher: (1024 + 16 q) / 16 - (64 + z)
+//   bf16: 16 + q minus 16 + z
+template <typename T>
+struct W4Exact;
+
+template <>
+struct W4Exact<__half> {
+  __half2 s[2], c[2];
+  __device__ __forceinline__ void set(uint32_t s01, uint32_t z01, bool zp) {
+    const __half2 sv = *reinterpret_cast<const __half2*>(&s01);
+    s[0] = __low2half2(sv), s[1] = __high2half2(sv);
+    if (zp) {
+      const __half2 z = *reinterpret_cast<const __half2*>(&z01);
+      c[0] = __hneg2(__hadd2(__low2half2(z), __float2half2_rn(1024.0f)));
+      c[1] = __hneg2(__hadd2(__high2half2(z), __float2half2_rn(64.0f)));
+    } else {
+      c[0] = __float2half2_rn(-1032.0f), c[1] = __float2half2_rn(-72.0f);
+    }
+  }
+  // r[2 column + j]: rows (0, 1) (j = 0) and (2, 3) of the word, as tcgen05.st 16x256b takes them
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* r) const {
+    const __half2 sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t v = i == 0 ? w : w >> 8;
+      const uint32_t lo = (v & 0x000F000Fu) | 0x64006400u, hi = (v & 0x00F000F0u) | 0x64006400u;
+      const __half2 a = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&lo), c[0]), s[0]);
+      const __half2 b = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, c[1]), s[1]);
+      r[i] = *reinterpret_cast<const uint32_t*>(&a);
+      r[2 + i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+};
+
+template <>
+struct W4Exact<__nv_bfloat16> {
+  __nv_bfloat162 s[2], c[2];
+  __device__ __forceinline__ void set(uint32_t s01, uint32_t z01, bool zp) {
+    const __nv_bfloat162 sv = *reinterpret_cast<const __nv_bfloat162*>(&s01);
+    s[0] = __low2bfloat162(sv), s[1] = __high2bfloat162(sv);
+    if (zp) {
+      const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&z01), o = __float2bfloat162_rn(16.0f);
+      c[0] = __hneg2(__hadd2(__low2bfloat162(z), o));
+      c[1] = __hneg2(__hadd2(__high2bfloat162(z), o));
+    } else {
+      c[0] = c[1] = __float2bfloat162_rn(-24.0f);
+    }
+  }
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* r) const {
+    uint32_t p[4];
+    W4Deq<__nv_bfloat16>::pairs(w, p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // p[2 j + column], j: rows (0, 1) / (2, 3)
+      const __nv_bfloat162 a = __hmul2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&p[i]), c[i & 1]), s[i & 1]);
+      r[2 * (i & 1) + (i >> 1)] = *reinterpret_cast<const uint32_t*>(&a);
+    }
+  }
+};
+
 // W words from shared memory in one access (two for W = 8)
 template <int W>
 __device__ __forceinline__ void w4_lds(uint32_t p, uint32_t (&v)[W]) {

@@ -10,6 +10,8 @@
 #include "chain_registry.h"
 #include "w4.cuh"
 
+#include <type_traits>
+
 namespace gp {
 namespace {
 
@@ -82,63 +84,143 @@ __device__ __forceinline__ void put_half(uint4* block_pair, int h, F&& q) {
   }
 }
 
+// Range of packed pairs, column by column; a NaN stays.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using V = __half2;
+  __device__ __forceinline__ static V max(V a, V b) { return __hmax2_nan(a, b); }
+  __device__ __forceinline__ static V min(V a, V b) { return __hmin2_nan(a, b); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+  __device__ __forceinline__ static V max(V a, V b) { return __hmax2_nan(a, b); }
+  __device__ __forceinline__ static V min(V a, V b) { return __hmin2_nan(a, b); }
+};
+
+// rint(x / s) + z, without a division per weight, as the bits of the float 1.5 2^23 + rint(x / s) + z.
+// x and s are T: their quotient is either exactly half way between two integers or, for quotients
+// below 16, at least 2^-13 away from there (2 x - (2 k + 1) s is a multiple of half the last place of
+// s, and s has 11 bits). below and above are 1 / s less and more 2^-22 of it, so x below and x above lie
+// within 2^-17 of the quotient on both sides: they round to the same integer, or, at a tie, to its two
+// neighbours, of which the even one is wanted. The fused sum rounds the exact products to integers.
+constexpr float kMagic = 12582912.0f;  // 1.5 2^23: its last place is 1
+constexpr uint32_t kMagicBits = 0x4B400000u;
+
+__device__ __forceinline__ uint32_t w4_code_bits(float x, float below, float above, float magic_z, uint32_t z) {
+  const uint32_t a = __float_as_uint(fmaf(x, below, magic_z)), b = __float_as_uint(fmaf(x, above, magic_z));
+  return ((a ^ z) & 1u) ? b : a;
+}
+
 // Codes and scale of a group of G rows (largest magnitude to 7, or the range with zero to 15).
-// s is rounded to T first and the codes are taken against the rounded scale; quotients are IEEE
-// divisions, rounded half to even. A group whose scale rounds to zero has code = zero point. A
-// group with a NaN or an infinity has a scale that is not finite, and so has what it stands for.
+// s is rounded to T first and the codes are taken against the rounded scale. A group whose scale
+// rounds to zero has code = zero point; one with a NaN or an infinity has a scale that is not
+// finite, and so has what it stands for. A group of 128 is shared by two threads 16 lanes apart, 64
+// rows each: 128 values did not fit a thread's registers.
 template <typename T, int G, bool ZP, bool VEC>
 __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_constant__ W4Layout l,
                                                                    const T* __restrict__ w, void* packed) {
+  using P = Pair<T>;
+  using V = typename P::V;
+  constexpr int kPer = G > 64 ? 64 : G, kSplit = G / kPer;
   pdl_wait_prior();
   pdl_launch_dependents();
-  const Where at = where(l);
-  if (!at.in) return;
+  const int lane = threadIdx.x & 31;
+  const int part = kSplit == 2 ? lane >> 4 : 0;
+  const int pair = kSplit == 2 ? (blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5)) * 16 + (lane & 15)
+                               : static_cast<int>(blockIdx.x * kPackThreads + threadIdx.x);
+  const int tile = pair >> 3, g = pair & 7, c = 2 * pair;
+  const bool in = tile < l.n_tiles;
   for (int64_t grp = blockIdx.y; grp < l.blocks * l.units; grp += gridDim.y) {
-    const int k0 = static_cast<int>(grp) * G;
-    uint32_t v[G];
+    const int k0 = static_cast<int>(grp) * G + part * kPer;
+    uint32_t v[kPer];
 #pragma unroll
-    for (int i = 0; i < G; ++i) v[i] = (at.c < l.n && k0 + i < l.k) ? load_pair<VEC>(w, k0 + i, l.n, at.c) : 0u;
-    float hi[2] = {0.0f, 0.0f}, lo[2] = {0.0f, 0.0f}, bad[2] = {0.0f, 0.0f};
+    for (int i = 0; i < kPer; ++i) v[i] = (in && c < l.n && k0 + i < l.k) ? load_pair<VEC>(w, k0 + i, l.n, c) : 0u;
+    const uint32_t zero = 0;
+    V hi = *reinterpret_cast<const V*>(&zero), lo = hi;
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const float2 f = Elem<T>::unpack(v[i]);
-      hi[0] = fmaxf(hi[0], f.x), lo[0] = fminf(lo[0], f.x), bad[0] += f.x * 0.0f;
-      hi[1] = fmaxf(hi[1], f.y), lo[1] = fminf(lo[1], f.y), bad[1] += f.y * 0.0f;
+    for (int i = 0; i < kPer; ++i) {
+      const V x = *reinterpret_cast<const V*>(&v[i]);
+      hi = P::max(hi, ZP ? x : __habs2(x));
+      if (ZP) lo = P::min(lo, x);
     }
-    float s[2], z[2];
-    uint32_t s01 = 0, z01 = 0;
-    {
-      float raw[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r)  // max and min drop a NaN: bad (0, or NaN from a NaN or infinity) brings it back
-        raw[r] = (ZP ? __fdiv_rn(hi[r] - lo[r], 15.0f) : __fdiv_rn(fmaxf(hi[r], -lo[r]), 7.0f)) + bad[r];
-      s01 = Elem<T>::pack(raw[0], raw[1]);
-      const float2 f = Elem<T>::unpack(s01);
-      s[0] = f.x, s[1] = f.y;
+    uint32_t hb = *reinterpret_cast<const uint32_t*>(&hi), lb = *reinterpret_cast<const uint32_t*>(&lo);
+    if (kSplit == 2) {
+      const uint32_t ho = __shfl_xor_sync(0xffffffffu, hb, 16), lo_o = __shfl_xor_sync(0xffffffffu, lb, 16);
+      hi = P::max(hi, *reinterpret_cast<const V*>(&ho));
+      lo = P::min(lo, *reinterpret_cast<const V*>(&lo_o));
+      hb = *reinterpret_cast<const uint32_t*>(&hi), lb = *reinterpret_cast<const uint32_t*>(&lo);
     }
+    if (!in) continue;
+    const float2 h = Elem<T>::unpack(hb), b = Elem<T>::unpack(lb);
+    uint32_t s01 = ZP ? Elem<T>::pack(__fdiv_rn(h.x - b.x, 15.0f), __fdiv_rn(h.y - b.y, 15.0f))
+                      : Elem<T>::pack(__fdiv_rn(h.x, 7.0f), __fdiv_rn(h.y, 7.0f));
+    const float2 sv = Elem<T>::unpack(s01);
+    const float s[2] = {sv.x, sv.y}, low[2] = {b.x, b.y};
+    float below[2], above[2];
+    int z[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      z[r] = ZP ? (s[r] > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(-lo[r], s[r])), 0.0f), 15.0f) : 0.0f) : 8.0f;
+      const float inv = s[r] > 0.0f ? __fdiv_rn(1.0f, s[r]) : 0.0f;
+      below[r] = inv * (1.0f - 0x1p-22f);
+      above[r] = inv * (1.0f + 0x1p-22f);
+      z[r] = 8;
+      if (ZP) {
+        const uint32_t q = w4_code_bits(-low[r], below[r], above[r], kMagic, 0) - kMagicBits;
+        z[r] = s[r] > 0.0f ? static_cast<int>(q > 15u ? 15u : q) : 0;
+      }
     }
-    const bool real = at.c < l.n && k0 < l.k;
-    if (ZP) z01 = Elem<T>::pack(z[0], z[1]);
+    const bool real = c < l.n && static_cast<int>(grp) * G < l.k;
+    uint32_t z01 = ZP ? Elem<T>::pack(static_cast<float>(z[0]), static_cast<float>(z[1])) : 0u;
     if (!real) s01 = 0, z01 = 0;
-    if (at.c + 1 >= l.n) s01 &= 0xFFFFu, z01 &= 0xFFFFu;
-    uint32_t* sp = scale_ptr(l, packed, at.tile, static_cast<int>(grp), at.g);
-    if (ZP) *reinterpret_cast<uint2*>(sp) = make_uint2(s01, z01);
-    else *sp = s01;
-#pragma unroll
-    for (int hh = 0; hh < G / 32; ++hh) {
-      const int k = k0 + hh * 32;
-      put_half<T>(code_ptr(l, packed, at.tile, k / 64, at.g), (k / 32) & 1, [&](int r, int kk) {
-        const float2 f = Elem<T>::unpack(v[hh * 32 + kk]);
-        const float x = r == 0 ? f.x : f.y;
-        float q = z[r];
-        if (s[r] > 0.0f) q = fminf(fmaxf(rintf(__fdiv_rn(x, s[r])) + z[r], 0.0f), 15.0f);
-        const bool pad = k + kk >= l.k || at.c + r >= l.n;
-        return pad ? 0u : static_cast<uint32_t>(q);
-      });
+    if (c + 1 >= l.n) s01 &= 0xFFFFu, z01 &= 0xFFFFu;
+    if (part == 0) {
+      uint32_t* sp = scale_ptr(l, packed, tile, static_cast<int>(grp), g);
+      if (ZP) *reinterpret_cast<uint2*>(sp) = make_uint2(s01, z01);
+      else *sp = s01;
     }
+    const float mz[2] = {kMagic + static_cast<float>(z[0]), kMagic + static_cast<float>(z[1])};
+    // Lowest code: rint is odd, so rint(lo / s) + z is not below 0. Highest: s is within half a step of
+    // its unrounded value, so without zero points |x / s| stays below 7.5; with them two roundings can
+    // make 16. A subnormal s is rounded more coarsely, and the edge's columns and rows are zeros: those
+    // take every test.
+    auto put = [&](auto edge) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        uint32_t word[kPer / 16];  // (half, j)
+#pragma unroll
+        for (int hj = 0; hj < kPer / 16; ++hj) {
+          // the sum of the codes' bits 16^nibble apart; what 1.5 2^23 adds to it is constant
+          uint32_t acc = 0u - kMagicBits * 0x11111111u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int kk = 16 * hj + 4 * t + i;
+            const float2 f = Elem<T>::unpack(v[kk]);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              uint32_t q = w4_code_bits(r == 0 ? f.x : f.y, below[r], above[r], mz[r], static_cast<uint32_t>(z[r]));
+              if (edge) {
+                q = q < kMagicBits ? kMagicBits : q > kMagicBits + 15u ? kMagicBits + 15u : q;
+                if (k0 + kk >= l.k || c + r >= l.n) q = kMagicBits;
+              } else if (ZP) {
+                q = q > kMagicBits + 15u ? kMagicBits + 15u : q;
+              }
+              acc += q * (1u << (4 * w4_nibble(r, i)));
+            }
+          }
+          word[hj] = w4_store_word<T>(acc);
+        }
+        uint4* to = code_ptr(l, packed, tile, k0 / 64, g) + t;
+        if constexpr (kPer == 64) *to = make_uint4(word[0], word[1], word[2], word[3]);
+        else reinterpret_cast<uint2*>(to)[(k0 / 32) & 1] = make_uint2(word[0], word[1]);
+      }
+    };
+    constexpr float kNormal = Elem<T>::kIsBf16 ? 0x1p-126f : 0x1p-14f;
+    const bool plain = s[0] >= kNormal && s[1] >= kNormal && s[0] < 1e30f && s[1] < 1e30f;  // false for NaN
+    if (plain && c + 1 < l.n && k0 + kPer <= l.k) put(std::false_type{});
+    else put(std::true_type{});
   }
 }
 
@@ -216,7 +298,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_unpack_kernel(const __grid_co
   }
 }
 
-// s (q - z) in fp32 (exact: at most 11 + 5 bits), rounded once to T
+// s (q - z), rounded once to T, in packed arithmetic
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kPackThreads) w4_dequantize_kernel(const __grid_constant__ W4Layout l, void* packed,
                                                                      T* __restrict__ w) {
@@ -233,20 +315,20 @@ __global__ void __launch_bounds__(kPackThreads) w4_dequantize_kernel(const __gri
     for (int h = 0; h < 2; ++h) {
       const int k0 = static_cast<int>(b) * 64 + h * 32;
       const uint32_t* sp = scale_ptr(l, packed, at.tile, k0 / l.group, at.g);
-      const float2 s = Elem<T>::unpack(sp[0]);
-      float2 z = make_float2(8.0f, 8.0f);
-      if (l.zeros) z = Elem<T>::unpack(sp[1]);
+      W4Exact<T> dq;
+      dq.set(sp[0], l.zeros ? sp[1] : 0u, l.zeros != 0);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t wd[2] = {w4_load_word<T>(h == 0 ? u[t].x : u[t].z), w4_load_word<T>(h == 0 ? u[t].y : u[t].w)};
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = e >> 2, i = e & 3, k = k0 + 16 * j + 4 * t + i;
-          const float q0 = static_cast<float>((wd[j] >> (4 * w4_nibble(0, i))) & 15u);
-          const float q1 = static_cast<float>((wd[j] >> (4 * w4_nibble(1, i))) & 15u);
-          if (k < l.k) store_pair<VEC>(w, k, l.n, at.c, Elem<T>::pack(s.x * (q0 - z.x), s.y * (q1 - z.y)));
+        for (int j = 0; j < 2; ++j) {
+          uint32_t r[4];  // rows (0, 1) and (2, 3) of column 0, then of column 1
+          dq.word(h == 0 ? (j == 0 ? u[t].x : u[t].y) : (j == 0 ? u[t].z : u[t].w), r);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = k0 + 16 * j + 4 * t + i;
+            if (k < l.k) store_pair<VEC>(w, k, l.n, at.c, __byte_perm(r[i >> 1], r[2 + (i >> 1)], (i & 1) ? 0x7632 : 0x5410));
+          }
         }
-      }
     }
   }
 }
@@ -254,9 +336,10 @@ __global__ void __launch_bounds__(kPackThreads) w4_dequantize_kernel(const __gri
 // Launch over column pairs (x) and 64-row parts or groups (y, with a stride past the grid's limit).
 // `out` / `bytes`: what the launch writes.
 template <typename... KArgs, typename... Args>
-int launch_pack(void (*kern)(KArgs...), const W4Layout& l, int rows, cudaStream_t s, const PdlIo& io, Args... args) {
+int launch_pack(void (*kern)(KArgs...), const W4Layout& l, int rows, int threads_per_pair, cudaStream_t s,
+                const PdlIo& io, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  const int pairs = l.n_tiles * 8;
+  const int pairs = l.n_tiles * 8 * threads_per_pair;
   cfg.gridDim = dim3(static_cast<unsigned>((pairs + kPackThreads - 1) / kPackThreads),
                      static_cast<unsigned>(rows < 65535 ? rows : 65535), 1);
   cfg.blockDim = dim3(kPackThreads, 1, 1);
@@ -282,7 +365,7 @@ int quantize_g(const W4Layout& l, const T* w, void* packed, cudaStream_t s) {
   const bool vec = even_rows(l, w);
   auto kern = l.zeros ? (vec ? &w4_quantize_kernel<T, G, true, true> : &w4_quantize_kernel<T, G, true, false>)
                       : (vec ? &w4_quantize_kernel<T, G, false, true> : &w4_quantize_kernel<T, G, false, false>);
-  return launch_pack(kern, l, l.blocks * l.units, s, io, w, packed);
+  return launch_pack(kern, l, l.blocks * l.units, G > 64 ? 2 : 1, s, io, w, packed);
 }
 
 template <typename T>
@@ -299,7 +382,7 @@ int pack_t(const W4Layout& l, const uint8_t* codes, const void* scales, const ui
   PdlIo io;
   io.add(PdlIo::kWrite, packed, static_cast<uint64_t>(l.bytes));
   auto kern = even_rows(l, scales) ? &w4_pack_kernel<T, true> : &w4_pack_kernel<T, false>;
-  return launch_pack(kern, l, l.blocks * 2, s, io, codes, static_cast<const T*>(scales), zeros, packed);
+  return launch_pack(kern, l, l.blocks * 2, 1, s, io, codes, static_cast<const T*>(scales), zeros, packed);
 }
 
 template <typename T>
@@ -310,7 +393,7 @@ int unpack_t(const W4Layout& l, const void* packed, uint8_t* codes, void* scales
   io.add(PdlIo::kWrite, scales, ng * 2);
   io.add(PdlIo::kWrite, zeros, ng);
   auto kern = scales != nullptr && even_rows(l, scales) ? &w4_unpack_kernel<T, true> : &w4_unpack_kernel<T, false>;
-  return launch_pack(kern, l, l.blocks * 2, s, io, const_cast<void*>(packed), codes, static_cast<T*>(scales), zeros);
+  return launch_pack(kern, l, l.blocks * 2, 1, s, io, const_cast<void*>(packed), codes, static_cast<T*>(scales), zeros);
 }
 
 template <typename T>
@@ -318,7 +401,7 @@ int dequantize_t(const W4Layout& l, const void* packed, void* w, cudaStream_t s)
   PdlIo io;
   io.add(PdlIo::kWrite, w, static_cast<uint64_t>(l.k) * l.n * 2);
   auto kern = even_rows(l, w) ? &w4_dequantize_kernel<T, true> : &w4_dequantize_kernel<T, false>;
-  return launch_pack(kern, l, l.blocks * 2, s, io, const_cast<void*>(packed), static_cast<T*>(w));
+  return launch_pack(kern, l, l.blocks * 2, 1, s, io, const_cast<void*>(packed), static_cast<T*>(w));
 }
 
 }  // namespace
