@@ -100,11 +100,12 @@ def fused_mlp_out(x, weights, biases, out, *, acts, tail=L.TAIL_NONE, gamma=None
 
     weights may be W4Weight (all of them): the chain then runs on 4-bit weights (w4_mlp_out), which
     takes any widths and no skip layer."""
-    if any(isinstance(w, W4Weight) for w in weights):
-        if skip_layer:
-            raise RuntimeError("skip_layer is not available on 4-bit weights")
-        w4_mlp_out(x, weights, biases, out, acts=acts, tail=tail, gamma=gamma, beta=beta, ln_eps=ln_eps)
-        return
+    for w in weights:
+        if type(w) is W4Weight:
+            if skip_layer:
+                raise RuntimeError("skip_layer is not available on 4-bit weights")
+            w4_mlp_out(x, weights, biases, out, acts=acts, tail=tail, gamma=gamma, beta=beta, ln_eps=ln_eps)
+            return
     _check_input("x", x)
     dt = _DT.get(x.dtype)
     if dt is None:
@@ -550,10 +551,53 @@ def _dtype_code(name, dtype):
     return dt
 
 
-def _same_device(first, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"{name} is on {t.device}, expected {first.device}")
+# These calls take microseconds on the GPU for single tokens, so their host side is kept short: one
+# expression per tensor in the usual case (the messages are made in _refuse), raw addresses to ctypes.
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _refuse(name, t, dtype, shape, dev) -> None:
+    """Raise for a tensor that failed the short check (a None or a non-tensor included)."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    _check_input(name, t, dtype)
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.device != dev:
+        raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
+
+
+def _address(name, t, dtype, shape, dev):
+    """t's address if it is a contiguous tensor of that type and shape on dev; None for None."""
+    if t is None:
+        return None
+    try:
+        if t.dtype == dtype and t.shape == shape and t.device == dev and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(name, t, dtype, shape, dev)
+    return t.data_ptr()
+
+
+def _cuda_2d(name, t):
+    """t's device, of a 2-D CUDA tensor."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise RuntimeError(f"{name} must be a 2-D tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    return t.device
+
+
+def _launch(dev, fn, *args) -> None:
+    """fn(*args, stream) on dev's current stream, with dev as the current device."""
+    if _raw_stream is not None and _get_device() == dev.index:
+        rc = fn(*args, _raw_stream(dev.index))
+    else:
+        with _on_device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc != L.GP_OK:
+        L.check(rc)
 
 
 _NORM_SPECS: dict = {}
@@ -564,7 +608,7 @@ def _norm_spec(*key):
     if s is None:
         if len(_NORM_SPECS) >= 1024:  # gate_rows follows the row count: do not keep every one
             _NORM_SPECS.clear()
-        s = _NORM_SPECS[key] = L.GpBlockNormSpec(*key)
+        s = _NORM_SPECS[key] = ctypes.byref(L.GpBlockNormSpec(*key))
     return s
 
 
@@ -585,42 +629,36 @@ def block_norm_out(x, y, r, h, *, post=L.NORM_NONE, pre=L.NORM_NONE, gate=None, 
     first = x if x is not None else y
     if first is None or (r is None and h is None):
         raise RuntimeError("block_norm needs x or y, and r or h")
-    if not isinstance(first, torch.Tensor) or first.dim() != 2:
-        raise RuntimeError("x and y must be 2-D")
-    m, width = first.shape
-    params = (("gate", gate), ("post_gamma", post_gamma), ("post_beta", post_beta),
-              ("pre_gamma", pre_gamma), ("pre_beta", pre_beta))
-    dtype = h.dtype if h is not None else None
-    for t in [p[1] for p in params] + [y, x, r]:  # the 16-bit type of the call
-        if dtype is None and t is not None and t.dtype != torch.float32:
+    dev = _cuda_2d("x" if x is not None else "y", first)
+    shape = first.shape
+    m, width = shape
+    f32 = torch.float32
+    dtype = None  # the 16-bit type of the call
+    for t in (h, y, x, r, gate, post_gamma, post_beta, pre_gamma, pre_beta):
+        if t is not None and t.dtype != f32:
             dtype = t.dtype
-    if dtype is None:  # every tensor is fp32: the 16-bit type does not matter
-        dtype = torch.float16
-    dt = _dtype_code("h", dtype)
-    stream = torch.float32 if torch.float32 in [t.dtype for t in (x, r) if t is not None] else dtype
-    ydt = torch.float32 if y is not None and y.dtype == torch.float32 else dtype
-    for name, t, want in (("x", x, stream), ("r", r, stream), ("y", y, ydt), ("h", h, dtype)):
-        _check_input(name, t, want)
-        if t is not None and tuple(t.shape) != (m, width):
-            raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected ({m}, {width})")
-    gate_rows = 0
-    for name, t in params:
-        _check_input(name, t, dtype)
-        if t is None or tuple(t.shape) == (width,):
-            continue
-        if name != "gate" or t.dim() != 2 or t.shape[1] != width:
-            raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected ({width},)")
-        g = t.shape[0]
-        if m and (g == 0 or m % g):
-            raise RuntimeError(f"{m} rows are not a multiple of {g} gate rows")
-        gate_rows = m // g if m else 0
-    _same_device(first, y=y, r=r, h=h, **dict(params))
-    spec = _norm_spec(width, dt, int(stream == torch.float32), int(ydt == torch.float32), post, pre,
-                      post_eps, pre_eps, x_scale, y_scale, gate_rows)
-    with _on_device(first.device):
-        L.check(L.lib().gp_block_norm_out(ctypes.byref(spec), m, _ptr(x), _ptr(y), _ptr(gate),
-                                          _ptr(post_gamma), _ptr(post_beta), _ptr(pre_gamma),
-                                          _ptr(pre_beta), _ptr(r), _ptr(h), _stream(first)))
+            break
+    dt = _dtype_code("h", dtype if dtype is not None else torch.float16)  # all fp32: no matter
+    stream_t = x if x is not None else r
+    stream = f32 if stream_t is not None and stream_t.dtype == f32 else dtype
+    ydt = f32 if y is not None and y.dtype == f32 else dtype
+    gate_rows, gate_shape = 0, (width,)
+    if gate is not None and gate.dim() == 2:
+        groups = gate.shape[0]
+        if m and (groups == 0 or m % groups):
+            raise RuntimeError(f"{m} rows are not a multiple of {groups} gate rows")
+        gate_rows, gate_shape = m // groups if m else 0, (groups, width)
+    row = (width,)
+    _launch(dev, L.lib().gp_block_norm_out,
+            _norm_spec(width, dt, int(stream == f32), int(ydt == f32), post, pre, post_eps, pre_eps,
+                       x_scale, y_scale, gate_rows),
+            m, _address("x", x, stream, shape, dev), _address("y", y, ydt, shape, dev),
+            _address("gate", gate, dtype, gate_shape, dev),
+            _address("post_gamma", post_gamma, dtype, row, dev),
+            _address("post_beta", post_beta, dtype, row, dev),
+            _address("pre_gamma", pre_gamma, dtype, row, dev),
+            _address("pre_beta", pre_beta, dtype, row, dev),
+            _address("r", r, stream, shape, dev), _address("h", h, dtype, shape, dev))
 
 
 def block_norm(x, y=None, *, dtype=None, want_r=True, post=L.NORM_NONE, pre=L.NORM_NONE, **kw):
@@ -630,18 +668,18 @@ def block_norm(x, y=None, *, dtype=None, want_r=True, post=L.NORM_NONE, pre=L.NO
     first = x if x is not None else y
     if first is None:
         raise RuntimeError("block_norm needs x or y")
-    if dtype is None:
-        for t in (y, x, *kw.values()):
-            if isinstance(t, torch.Tensor) and t.dtype in _DT:
-                dtype = t.dtype
-                break
     r = h = None
     if want_r and y is not None:
-        r = torch.empty_like(first if x is not None else y)
+        r = torch.empty_like(first)
     if pre != L.NORM_NONE:
         if dtype is None:
-            raise RuntimeError("dtype must be given where every tensor is float32")
-        h = torch.empty(first.shape, dtype=dtype, device=first.device)
+            for t in (y, x, *kw.values()):
+                if isinstance(t, torch.Tensor) and t.dtype in _DT:
+                    dtype = t.dtype
+                    break
+            else:
+                raise RuntimeError("dtype must be given where every tensor is float32")
+        h = torch.empty_like(first, dtype=dtype)
     block_norm_out(x, y, r, h, post=post, pre=pre, **kw)
     return r, h
 
@@ -650,26 +688,27 @@ class W4Weight:
     """Weights [K, N] in 4 bits with group scales along K (gp_w4_spec): the packed buffer and what
     it holds. Made by w4_quantize or w4_pack."""
 
-    __slots__ = ("packed", "k", "n", "group", "dtype", "zero_points", "spec")
+    __slots__ = ("packed", "k", "n", "group", "dtype", "zero_points", "spec", "nbytes")
 
     def __init__(self, packed, k, n, group, dtype, zero_points):
-        self.packed, self.k, self.n, self.group = packed, int(k), int(n), int(group)
+        self.k, self.n, self.group = int(k), int(n), int(group)
         self.dtype, self.zero_points = dtype, bool(zero_points)
-        self.spec = L.GpW4Spec(self.k, self.n, self.group, _dtype_code("weights", dtype), int(self.zero_points))
-        nbytes = L.lib().gp_w4_packed_bytes(ctypes.byref(self.spec))
-        if nbytes < 0:
-            L.check(int(nbytes))
+        self.spec = ctypes.byref(L.GpW4Spec(self.k, self.n, self.group, _dtype_code("weights", dtype),
+                                            int(self.zero_points)))
+        self.nbytes = L.lib().gp_w4_packed_bytes(self.spec)
+        if self.nbytes < 0:
+            L.check(int(self.nbytes))
         if packed is not None:
             _check_input("packed", packed, torch.uint8)
-            if packed.numel() != nbytes:
-                raise RuntimeError(f"packed has {packed.numel()} bytes, expected {nbytes}")
+            if tuple(packed.shape) != (self.nbytes,):
+                raise RuntimeError(f"packed has shape {tuple(packed.shape)}, expected ({self.nbytes},)")
+        self.packed = packed
 
     @classmethod
     def empty(cls, k, n, group, dtype, zero_points, device):
         """An unfilled weight on `device`."""
         w = cls(None, k, n, group, dtype, zero_points)
-        nbytes = L.lib().gp_w4_packed_bytes(ctypes.byref(w.spec))
-        w.packed = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        w.packed = torch.empty(w.nbytes, dtype=torch.uint8, device=device)
         return w
 
     @property
@@ -680,50 +719,42 @@ class W4Weight:
     def device(self):
         return self.packed.device
 
-    def _unpack(self, codes=None, scales=None, zeros=None):
-        with _on_device(self.device):
-            L.check(L.lib().gp_w4_unpack_out(ctypes.byref(self.spec), _ptr(self.packed), _ptr(codes),
-                                             _ptr(scales), _ptr(zeros), _stream(self.packed)))
+    def _address(self, name, dev):
+        return _address(name, self.packed, torch.uint8, (self.nbytes,), dev)
+
+    def _unpack(self, rows, dtype, place):
+        t = torch.empty(rows, self.n, dtype=dtype, device=self.device)
+        outs = [None, None, None]
+        outs[place] = t.data_ptr()
+        _launch(self.device, L.lib().gp_w4_unpack_out, self.spec, self._address("packed", self.device), *outs)
+        return t
 
     def codes(self):
         """q [K, N], one code (0..15) per byte."""
-        t = torch.empty(self.k, self.n, dtype=torch.uint8, device=self.device)
-        self._unpack(codes=t)
-        return t
+        return self._unpack(self.k, torch.uint8, 0)
 
     def scales(self):
         """s [ceil(K / group), N]."""
-        t = torch.empty(-(-self.k // self.group), self.n, dtype=self.dtype, device=self.device)
-        self._unpack(scales=t)
-        return t
+        return self._unpack(-(-self.k // self.group), self.dtype, 1)
 
     def zeros(self):
         """z [ceil(K / group), N] (bytes 0..15), or None without zero points."""
-        if not self.zero_points:
-            return None
-        t = torch.empty(-(-self.k // self.group), self.n, dtype=torch.uint8, device=self.device)
-        self._unpack(zeros=t)
-        return t
+        return self._unpack(-(-self.k // self.group), torch.uint8, 2) if self.zero_points else None
 
 
 def w4_quantize_out(w, w4) -> None:
     """Quantise w [K, N] (float16 or bfloat16) into a W4Weight of the same shape and type."""
-    _check_input("w", w, w4.dtype)
-    if tuple(w.shape) != w4.shape:
-        raise RuntimeError(f"w has shape {tuple(w.shape)}, expected {w4.shape}")
-    _same_device(w, packed=w4.packed)
-    with _on_device(w.device):
-        L.check(L.lib().gp_w4_quantize_out(ctypes.byref(w4.spec), _ptr(w), _ptr(w4.packed), _stream(w)))
+    dev = _cuda_2d("w", w)
+    _launch(dev, L.lib().gp_w4_quantize_out, w4.spec, _address("w", w, w4.dtype, (w4.k, w4.n), dev),
+            w4._address("packed", dev))
 
 
 def w4_quantize(w, group=128, zero_points=False) -> W4Weight:
     """w [K, N] to 4 bits: per group of `group` rows and column, the largest magnitude becomes code
     distance 7 (or, with zero_points, the range with zero becomes 0..15); gp_w4_quantize_out has
     the rule."""
-    _check_input("w", w)
-    if w.dim() != 2:
-        raise RuntimeError("w must be [K, N]")
-    w4 = W4Weight.empty(w.shape[0], w.shape[1], group, w.dtype, zero_points, w.device)
+    dev = _cuda_2d("w", w)
+    w4 = W4Weight.empty(w.shape[0], w.shape[1], group, w.dtype, zero_points, dev)
     w4_quantize_out(w, w4)
     return w4
 
@@ -731,32 +762,22 @@ def w4_quantize(w, group=128, zero_points=False) -> W4Weight:
 def w4_pack(codes, scales, zeros=None, group=128) -> W4Weight:
     """Weights quantised elsewhere: codes uint8 [K, N] (0..15), scales [ceil(K / group), N] (float16
     or bfloat16, the type of the activations), zeros uint8 of the scales' shape or None (8)."""
-    _check_input("codes", codes, torch.uint8)
-    _check_input("scales", scales)
-    _check_input("zeros", zeros, torch.uint8)
-    if codes.dim() != 2:
-        raise RuntimeError("codes must be [K, N]")
+    dev = _cuda_2d("codes", codes)
+    _cuda_2d("scales", scales)
     k, n = codes.shape
-    w4 = W4Weight.empty(k, n, group, scales.dtype, zeros is not None, codes.device)
-    want = (-(-k // group), n)
-    for name, t in (("scales", scales), ("zeros", zeros)):
-        if t is not None and tuple(t.shape) != want:
-            raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {want}")
-    _same_device(codes, scales=scales, zeros=zeros)
-    with _on_device(codes.device):
-        L.check(L.lib().gp_w4_pack_out(ctypes.byref(w4.spec), _ptr(codes), _ptr(scales), _ptr(zeros),
-                                       _ptr(w4.packed), _stream(codes)))
+    w4 = W4Weight.empty(k, n, group, scales.dtype, zeros is not None, dev)
+    rows = (-(-k // group), n)
+    _launch(dev, L.lib().gp_w4_pack_out, w4.spec, _address("codes", codes, torch.uint8, (k, n), dev),
+            _address("scales", scales, scales.dtype, rows, dev),
+            _address("zeros", zeros, torch.uint8, rows, dev), w4.packed.data_ptr())
     return w4
 
 
 def w4_dequantize_out(w4, w) -> None:
     """w [K, N] = s (q - z), rounded once."""
-    _check_input("w", w, w4.dtype)
-    if tuple(w.shape) != w4.shape:
-        raise RuntimeError(f"w has shape {tuple(w.shape)}, expected {w4.shape}")
-    _same_device(w, packed=w4.packed)
-    with _on_device(w.device):
-        L.check(L.lib().gp_w4_dequantize_out(ctypes.byref(w4.spec), _ptr(w4.packed), _ptr(w), _stream(w)))
+    dev = _cuda_2d("w", w)
+    _launch(dev, L.lib().gp_w4_dequantize_out, w4.spec, w4._address("packed", dev),
+            _address("w", w, w4.dtype, (w4.k, w4.n), dev))
 
 
 def w4_dequantize(w4) -> torch.Tensor:
@@ -767,28 +788,42 @@ def w4_dequantize(w4) -> torch.Tensor:
 
 def w4_linear_out(x, w4, bias, out, act=L.ACT_NONE) -> None:
     """out [M, N] = act(x [M, K] W + bias) on 4-bit weights; x, bias (or None) and out have the
-    weights' type. Made for few rows (single tokens, decode batches); any M works."""
+    weights' type. Single tokens, decode batches, prompts."""
     if not isinstance(w4, W4Weight):
         raise RuntimeError("w4 must be a W4Weight")
-    _check_input("x", x, w4.dtype)
-    _check_input("bias", bias, w4.dtype)
-    _check_input("out", out, w4.dtype)
-    if x.dim() != 2 or x.shape[1] != w4.k:
-        raise RuntimeError(f"x has shape {tuple(x.shape)}, expected [M, {w4.k}]")
-    if tuple(out.shape) != (x.shape[0], w4.n):
-        raise RuntimeError(f"out has shape {tuple(out.shape)}, expected ({x.shape[0]}, {w4.n})")
-    if bias is not None and tuple(bias.shape) != (w4.n,):
-        raise RuntimeError(f"bias has shape {tuple(bias.shape)}, expected ({w4.n},)")
-    _same_device(x, packed=w4.packed, bias=bias, out=out)
-    with _on_device(x.device):
-        L.check(L.lib().gp_w4_linear_out(ctypes.byref(w4.spec), x.shape[0], act, _ptr(x), _ptr(w4.packed),
-                                         _ptr(bias), _ptr(out), _stream(x)))
+    dev = _cuda_2d("x", x)
+    m, dtype = x.shape[0], w4.dtype
+    if out is None:
+        raise RuntimeError("out must be a tensor")
+    _launch(dev, L.lib().gp_w4_linear_out, w4.spec, m, act, _address("x", x, dtype, (m, w4.k), dev),
+            w4._address("packed", dev), _address("bias", bias, dtype, (w4.n,), dev),
+            _address("out", out, dtype, (m, w4.n), dev))
 
 
 def w4_linear(x, w4, bias=None, act=L.ACT_NONE) -> torch.Tensor:
-    out = torch.empty(x.shape[0], w4.n, dtype=x.dtype, device=x.device)
+    if not isinstance(w4, W4Weight):
+        raise RuntimeError("w4 must be a W4Weight")
+    out = x.new_empty((x.shape[0], w4.n))
     w4_linear_out(x, w4, bias, out, act=act)
     return out
+
+
+_W4_CHAINS: dict = {}
+
+
+def _w4_chain(m, widths, acts, tail, dtype, ln_eps):
+    """The chain's description and the workspace bytes of m rows."""
+    key = (m, widths, acts, tail, dtype, ln_eps)
+    c = _W4_CHAINS.get(key)
+    if c is None:
+        spec = L.make_spec(widths, acts, tail, _DT[dtype], ln_eps, 0)
+        nbytes = L.lib().gp_w4_mlp_workspace_bytes(ctypes.byref(spec), m)
+        if nbytes < 0:
+            L.check(int(nbytes))
+        if len(_W4_CHAINS) >= 1024:
+            _W4_CHAINS.clear()
+        c = _W4_CHAINS[key] = (ctypes.byref(spec), int(nbytes))
+    return c
 
 
 def w4_mlp_out(x, weights, biases, out, *, acts, tail=L.TAIL_NONE, gamma=None, beta=None,
@@ -797,63 +832,48 @@ def w4_mlp_out(x, weights, biases, out, *, acts, tail=L.TAIL_NONE, gamma=None, b
     type and kind of zero points): any widths, every activation and tail. workspace: a uint8 CUDA
     tensor of at least w4_mlp_workspace_bytes; None takes one from torch's allocator. out may be x
     where the chain has a tail and ends in x's width."""
-    weights, biases = list(weights), list(biases)
     n = len(weights)
     if n == 0 or len(biases) != n or len(acts) != n:
         raise RuntimeError(f"{n} weights, {len(biases)} biases and {len(acts)} activations must match")
-    if not all(isinstance(w, W4Weight) for w in weights):
-        raise RuntimeError("either every weight of a chain is a W4Weight, or none")
+    for w in weights:
+        if not isinstance(w, W4Weight):
+            raise RuntimeError("either every weight of a chain is a W4Weight, or none")
+    dev = _cuda_2d("x", x)
     w0 = weights[0]
-    _check_input("x", x, w0.dtype)
-    if x.dim() != 2 or x.shape[1] != w0.k:
-        raise RuntimeError(f"x has shape {tuple(x.shape)}, expected [M, {w0.k}]")
-    m, width = x.shape
-    for i, (w, b) in enumerate(zip(weights, biases)):
-        if (w.group, w.dtype, w.zero_points) != (w0.group, w0.dtype, w0.zero_points):
+    dtype, m, width = w0.dtype, x.shape[0], w0.k
+    xp = _address("x", x, dtype, (m, width), dev)
+    wp, bp, widths = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), [width]
+    for i in range(n):
+        w = weights[i]
+        if w.group != w0.group or w.dtype != dtype or w.zero_points != w0.zero_points:
             raise RuntimeError(f"w{i + 1} differs from w1 in group size, type or zero points")
         if w.k != width:
             raise RuntimeError(f"w{i + 1} has shape {w.shape}, expected [{width}, N]")
         width = w.n
-        _check_input(f"b{i + 1}", b, w0.dtype)
-        if b is not None and tuple(b.shape) != (width,):
-            raise RuntimeError(f"b{i + 1} has shape {tuple(b.shape)}, expected ({width},)")
-        _same_device(x, **{f"w{i + 1}": w.packed, f"b{i + 1}": b})
-    for name, t in (("gamma", gamma), ("beta", beta)):
-        _check_input(name, t, w0.dtype)
-        if t is not None and tuple(t.shape) != (width,):
-            raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected ({width},)")
-    _check_input("out", out, w0.dtype)
-    if tuple(out.shape) != (m, width):
-        raise RuntimeError(f"out has shape {tuple(out.shape)}, expected ({m}, {width})")
-    _same_device(x, gamma=gamma, beta=beta, out=out)
-    spec = _spec([w0.k] + [w.n for w in weights], acts, tail, _DT[w0.dtype], ln_eps, 0)
-    nbytes = L.lib().gp_w4_mlp_workspace_bytes(ctypes.byref(spec), m)
-    if nbytes < 0:
-        L.check(int(nbytes))
+        widths.append(width)
+        wp[i] = w._address(f"w{i + 1}", dev)
+        bp[i] = _address(f"b{i + 1}", biases[i], dtype, (width,), dev)
+    gp, ep = _address("gamma", gamma, dtype, (width,), dev), _address("beta", beta, dtype, (width,), dev)
+    if out is None:
+        raise RuntimeError("out must be a tensor")
+    op = _address("out", out, dtype, (m, width), dev)
+    spec, nbytes = _w4_chain(m, tuple(widths), tuple(acts), tail, dtype, ln_eps)
     if workspace is None:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        workspace = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     else:
-        _check_input("workspace", workspace, torch.uint8)
-        _same_device(x, workspace=workspace)
-    wp = (ctypes.c_void_p * n)(*[w.packed.data_ptr() for w in weights])
-    bp = (ctypes.c_void_p * n)(*[(b.data_ptr() if b is not None else None) for b in biases])
-    with _on_device(x.device):
-        L.check(L.lib().gp_w4_mlp_out(ctypes.byref(spec), w0.group, int(w0.zero_points), m, _ptr(x), wp, bp,
-                                      _ptr(gamma), _ptr(beta), _ptr(out), _ptr(workspace),
-                                      workspace.numel(), _stream(x)))
+        _address("workspace", workspace, torch.uint8, (workspace.numel(),), dev)
+    _launch(dev, L.lib().gp_w4_mlp_out, spec, w0.group, int(w0.zero_points), m, xp, wp, bp, gp, ep, op,
+            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel())
 
 
 def w4_mlp_workspace_bytes(m, weights, *, acts, tail=L.TAIL_NONE) -> int:
     """Workspace of a w4_mlp_out call on m rows."""
-    spec = _spec([weights[0].k] + [w.n for w in weights], acts, tail, _DT[weights[0].dtype], 1e-5, 0)
-    nbytes = L.lib().gp_w4_mlp_workspace_bytes(ctypes.byref(spec), m)
-    if nbytes < 0:
-        L.check(int(nbytes))
-    return int(nbytes)
+    widths = (weights[0].k,) + tuple(w.n for w in weights)
+    return _w4_chain(m, widths, tuple(acts), tail, weights[0].dtype, 1e-5)[1]
 
 
 def w4_mlp(x, weights, biases, *, acts, tail=L.TAIL_NONE, gamma=None, beta=None, ln_eps=1e-5) -> torch.Tensor:
-    out = torch.empty(x.shape[0], weights[-1].n, dtype=x.dtype, device=x.device)
+    out = x.new_empty((x.shape[0], weights[-1].n))
     w4_mlp_out(x, weights, biases, out, acts=acts, tail=tail, gamma=gamma, beta=beta, ln_eps=ln_eps)
     return out
 
