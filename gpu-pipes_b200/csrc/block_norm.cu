@@ -17,18 +17,31 @@
 namespace gp {
 namespace {
 
-// 8 consecutive elements as fp32
+// 8 consecutive elements, as loaded and as fp32
+template <typename T>
+struct Vec8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const void* base, int64_t i) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(base) + i);
+    u[0] = p[0];
+    if constexpr (sizeof(T) == 4) u[1] = p[1];
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      v[0] = __uint_as_float(u[0].x), v[1] = __uint_as_float(u[0].y), v[2] = __uint_as_float(u[0].z), v[3] = __uint_as_float(u[0].w);
+      v[4] = __uint_as_float(u[1].x), v[5] = __uint_as_float(u[1].y), v[6] = __uint_as_float(u[1].z), v[7] = __uint_as_float(u[1].w);
+    } else {
+      const float2 a = Elem<T>::unpack(u[0].x), b = Elem<T>::unpack(u[0].y), c = Elem<T>::unpack(u[0].z), d = Elem<T>::unpack(u[0].w);
+      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+    }
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void load8(const void* base, int64_t i, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
-    const float4 a = p[0], b = p[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(base) + i);
-    const float2 a = Elem<T>::unpack(u.x), b = Elem<T>::unpack(u.y), c = Elem<T>::unpack(u.z), d = Elem<T>::unpack(u.w);
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
-  }
+  Vec8<T> r;
+  r.load(base, i);
+  r.get(v);
 }
 
 template <typename T>
@@ -66,10 +79,9 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 
 // TPR threads per row, NV vectors of 8 elements per thread; rows of one warp share a CTA of 256.
 template <typename T, typename X, typename Y, int TPR, int NV>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
   __shared__ float red[2][32];
-  constexpr int kRows = TPR < 256 ? 256 / TPR : 1;  // rows per CTA
-  static_assert(TPR == 32 || TPR >= 256, "a row is one warp or one CTA");
+  constexpr int kRows = TPR == 32 ? 8 : 1;  // rows per CTA: eight of a warp each, or one
   const int lane = threadIdx.x % TPR;
   const int width = a.width;
   pdl_wait_prior();
@@ -125,16 +137,27 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
     }
   };
 
+  // both operands are on their way before either is used
+  Vec8<X> xv[NV];
+  Vec8<Y> yv[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (lane + j * TPR) * 8;
+    if (c < width && a.y != nullptr) yv[j].load(a.y, base + c);
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (lane + j * TPR) * 8;
+    if (c < width && a.x != nullptr) xv[j].load(a.x, base + c);
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
   if (a.y != nullptr) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (lane + j * TPR) * 8;
-      if (c < width) load8<Y>(a.y, base + c, v[j]);
-    }
+    for (int j = 0; j < NV; ++j)
+      if ((lane + j * TPR) * 8 < width) yv[j].get(v[j]);
     if (a.post != GP_NORM_NONE) norm(a.post, a.post_eps, a.post_gamma, a.post_beta);
     const int64_t grow = a.gate_rows > 0 ? row / a.gate_rows : 0;
 #pragma unroll
@@ -154,10 +177,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
   if (a.x != nullptr) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (lane + j * TPR) * 8;
-      if (c >= width) continue;
+      if ((lane + j * TPR) * 8 >= width) continue;
       float p[8];
-      load8<X>(a.x, base + c, p);
+      xv[j].get(p);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[j][e] = fmaf(a.x_scale, p[e], v[j][e]);
     }
@@ -181,8 +203,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
 
 template <typename T, typename X, typename Y, int TPR, int NV>
 int launch_t(const BlockNormArgs& a, cudaStream_t stream) {
-  constexpr int kThreads = TPR < 256 ? 256 : TPR;
-  constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
+  constexpr int kThreads = TPR == 32 ? 256 : TPR;
+  constexpr int kRows = TPR == 32 ? 8 : 1;
   const int64_t grid = (a.m + kRows - 1) / kRows;
   const uint64_t h = static_cast<uint64_t>(a.width), rows = static_cast<uint64_t>(a.m) * h;
   PdlIo io;
@@ -195,15 +217,18 @@ int launch_t(const BlockNormArgs& a, cudaStream_t stream) {
   return e == cudaSuccess ? GP_OK : set_error(GP_ERR_CUDA, "block norm launch: %s", cudaGetErrorString(e));
 }
 
-// A row is one warp up to 1,024 columns (no barrier, eight rows in flight per CTA), one CTA above:
-// 256 threads of up to four vectors, then 512, then 1,024.
+// A row is one warp up to 1,024 columns (no barrier, eight rows in flight per CTA), one CTA above. The
+// CTA's size keeps two vectors per thread up to 4,096 columns, four above: a row's two reductions are
+// latency, which other CTAs on the SM cover, and more threads per row (512 x 2 instead of 256 x 4 at
+// 8,192 columns) leave fewer of them. Measured on 16-bit rows with a norm on both sides (TB/s of x, y, r, h):
+// 32,768 x 2,048 6.3 (256 x 1: 5.2), 16,384 x 4,096 6.8, 8,192 x 8,192 with gates 5.6 (512 x 2: 4.8).
 template <typename T, typename X, typename Y>
 int launch_w(const BlockNormArgs& a, cudaStream_t s) {
   const int h = a.width;
   if (h <= 256) return launch_t<T, X, Y, 32, 1>(a, s);
   if (h <= 512) return launch_t<T, X, Y, 32, 2>(a, s);
   if (h <= 1024) return launch_t<T, X, Y, 32, 4>(a, s);
-  if (h <= 2048) return launch_t<T, X, Y, 256, 1>(a, s);
+  if (h <= 2048) return launch_t<T, X, Y, 128, 2>(a, s);
   if (h <= 4096) return launch_t<T, X, Y, 256, 2>(a, s);
   if (h <= 8192) return launch_t<T, X, Y, 256, 4>(a, s);
   if (h <= 16384) return launch_t<T, X, Y, 512, 4>(a, s);

@@ -15,6 +15,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -219,6 +220,9 @@ struct W4LinearArgs {
   void* out;
   bool out_f32;
 };
+// How many clusters of ck CTAs (one CTA per SM) the device holds at a time: fewer than SMs / ck, as a
+// cluster stays within a GPC. `cache` is the caller's, one entry per device and log2(ck), zero at first.
+int w4_max_clusters(const void* kern, int threads, int smem, int ck, int sm_count, std::atomic<int> (*cache)[4]);
 int launch_w4_rows(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev);   // few rows (w4_linear.cu)
 int launch_w4_tiles(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev);  // more rows (w4_tiles.cu)
 int launch_w4_linear(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev);

@@ -512,10 +512,45 @@ int rows_tt(const W4RowsArgs& a, int tt, int run, int smem, int clusters, int64_
 
 }  // namespace
 
+int w4_max_clusters(const void* kern, int threads, int smem, int ck, int sm_count, std::atomic<int> (*cache)[4]) {
+  if (ck == 1) return sm_count;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>& slot = cache[dev & 63][ck == 2 ? 1 : ck == 4 ? 2 : 3];  // racing first calls store the same value
+  int n = slot.load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(sm_count / ck * ck), 1, 1);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(ck);
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = sm_count / ck;
+    }
+    slot.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev) {
   const W4Layout& l = in.l;
   const int64_t m = in.m;
-  const int sm_count = dev.sm_count;
+  // the number of CTAs that run at a time, from one instance at its full shared memory
+  static std::atomic<int> cluster_cache[64][4];
+  static unsigned long long probe_mask = 0;
+  auto probe = &w4_rows_kernel<__half, 1, 1, false, 2>;
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(probe), kRowsSmem, &probe_mask);
+  if (rc != GP_OK) return rc;
+  auto resident = [&](int ck) {
+    return w4_max_clusters(reinterpret_cast<const void*>(probe), kThreads, kRowsSmem, ck, dev.sm_count, cluster_cache);
+  };
   W4RowsArgs a;
   a.status = dev.status;
   a.timeout_ns = current_timeout_ns();
@@ -544,7 +579,7 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
         if (rows_smem(l, tt, ck, ws, slice, rows, 4 * 3) > kRowsSmem) r = 2;
         if (rows_smem(l, tt, ck, ws, slice, rows, r * kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
-        const int clusters = groups < sm_count / ck ? groups : sm_count / ck;
+        const int clusters = groups < resident(ck) ? groups : resident(ck);
         const int64_t iters = (groups + clusters - 1) / clusters;
         const int64_t cost = iters * (2 * per_warp + 3) + (ck > 1 ? 6 : 0);
         if (cost >= best) continue;
@@ -567,7 +602,7 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth) > kRowsSmem) --a.depth;
   const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth));
   const int groups = (l.n_tiles + kWarps / a.ws - 1) / (kWarps / a.ws);
-  const int clusters = groups < sm_count / a.ck ? groups : sm_count / a.ck;
+  const int clusters = groups < resident(a.ck) ? groups : resident(a.ck);
   PdlIo io;
   io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(m) * l.n * (in.out_f32 ? 4 : 2));
   // the grid's y dimension holds 65,535 row tiles; longer inputs go in several launches
@@ -578,7 +613,6 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
     c.x = static_cast<const char*>(in.x) + r0 * l.k * 2;
     c.out = static_cast<char*>(in.out) + r0 * l.n * (in.out_f32 ? 4 : 2);
     const int64_t rt = (c.m + per_pass - 1) / per_pass;
-    int rc;
     rc = in.dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(c, tt, run, smem, clusters, rt, s, io)
                           : rows_tt<__half>(c, tt, run, smem, clusters, rt, s, io);
     if (rc != GP_OK) return rc;

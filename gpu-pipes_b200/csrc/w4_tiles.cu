@@ -451,13 +451,20 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   a.rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
   a.row_tiles = static_cast<int>((in.m + a.rows - 1) / a.rows);
   const int64_t units = static_cast<int64_t>((a.l.n_tiles + kTileTiles - 1) / kTileTiles) * a.row_tiles;
-  // CTAs along K: the fewest rounds over the SMs, a round costing its blocks and about four more
-  // (six more with the sums across a cluster)
+  // CTAs along K, by time in tenths of a microsecond: a round of what runs at once costs 4 per block,
+  // 30 to start and end and 18 more with sums across a cluster (16 x 4,096 x 4,096: 16.1 us with one
+  // CTA along K, 11.2 with two, 8.4 with four)
+  static std::atomic<int> cluster_cache[64][4];
+  static unsigned long long probe_mask = 0;
+  const void* probe = reinterpret_cast<const void*>(&w4_tile_kernel<__half, 1, false>);
+  int rc = ensure_smem_attr(probe, kSmemLimit - 2048, &probe_mask);
+  if (rc != GP_OK) return rc;
   int64_t best = -1;
   for (int ck = 1; ck <= 8; ck *= 2) {
     const int slice = (a.l.blocks + ck - 1) / ck;
     if (ck > 1 && ((ck - 1) * slice >= a.l.blocks || a.rows % ck != 0)) break;
-    const int64_t cost = (units * ck + dev.sm_count - 1) / dev.sm_count * (slice + (ck > 1 ? 10 : 4));
+    const int at_once = w4_max_clusters(probe, kTileThreads, kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
+    const int64_t cost = (units + at_once - 1) / at_once * (4 * slice + (ck > 1 ? 48 : 30));
     if (best >= 0 && cost >= best) continue;
     best = cost;
     a.ck = ck;
@@ -473,7 +480,7 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   const int sums = a.ck > 1 ? a.rows * kTileN * 4 : 0;
   if (smem < sums) smem = sums;
   CUtensorMap tx;
-  int rc = make_tmap_2d(&tx, in.x, in.dtype, static_cast<uint64_t>(in.m), static_cast<uint64_t>(a.l.k), 64,
+  rc = make_tmap_2d(&tx, in.x, in.dtype, static_cast<uint64_t>(in.m), static_cast<uint64_t>(a.l.k), 64,
                         static_cast<uint32_t>(a.rows), 128);
   if (rc != GP_OK) return rc;
   PdlIo io;
