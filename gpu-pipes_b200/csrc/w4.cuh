@@ -185,19 +185,15 @@ __device__ __forceinline__ void w4_lds(uint32_t p, uint32_t (&v)[W]) {
   }
 }
 
-// Activations of the epilogues, in fp32 and not approximated: next to the weights they cost nothing.
-// The transcendental ones are a function call: they run once or twice per CTA, and copies of them in
-// an unrolled epilogue cost more in instruction fetches than the calls.
-static __device__ __noinline__ float w4_act_call(int act, float v) {
-  if (act == kActGeluTanh) return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * fmaf(0.044715f * v, v * v, v)));
-  const float e = 1.0f + expf(-v);
-  return act == kActSilu ? v / e : 1.0f / e;
-}
-
+// Activations of the epilogues in fp32: v sigmoid(u) with u = v (SiLU) or, for GELU's tanh form, twice
+// its argument (0.5 (1 + tanh(t)) = sigmoid(2 t)). The fast exponential and quotient are within a few
+// units of 2^-22 |u| of the exact ones, far below the 16-bit rounding that follows. Written without
+// calls: expf, tanhf and divisions in the epilogues took 36 of 98 us at 512 x 4,096 x 14,336.
 __device__ __forceinline__ float w4_act(int act, float v) {
   if (act == kActNone) return v;
   if (act == kActRelu) return v > 0.0f ? v : (v == v ? 0.0f : v);
-  return w4_act_call(act, v);
+  const float u = act == kActGeluTanh ? 1.5957691216057308f * fmaf(0.044715f * v, v * v, v) : v;
+  return __fdividef(act == kActSigmoid ? 1.0f : v, 1.0f + __expf(-u));
 }
 
 // ---- host interface (w4_pack.cu, w4_linear.cu); dtype is GP_F16 / GP_BF16

@@ -26,7 +26,6 @@
 //   - The warps' sums are joined in shared memory, the CTAs' through distributed shared memory,
 //     both in a fixed order: results do not depend on timing.
 #include <climits>
-#include <cstdlib>
 
 #include "../../include/gpipes.h"
 #include "chain_registry.h"
@@ -622,8 +621,6 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
 }
 
 int launch_w4_linear(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev) {
-  static const int force = [] { const char* e = std::getenv("GP_W4_PATH"); return e ? std::atoi(e) : 0; }();
-  if (force) return force == 1 ? launch_w4_rows(a, s, dev) : launch_w4_tiles(a, s, dev);
   return a.m <= 16 ? launch_w4_rows(a, s, dev) : launch_w4_tiles(a, s, dev);
 }
 

@@ -14,8 +14,8 @@
 //
 // The unit is a k-block of 128 rows of W:
 //   loader (1 thread)   x panels (two of 64 columns) by TMA into a ring of stages
-//   16 dequantising warps  four groups of four (one warp per TMEM lane quarter); a group makes every
-//                       fourth block. Each lane copies its own codes and scales with cp.async into a
+//   dequantising warps  four groups of four (one warp per TMEM lane quarter); the groups take the
+//                       blocks in turn. Each lane copies its own codes and scales with cp.async into a
 //                       private ring, one or two blocks ahead, turns them into T in registers and
 //                       stores them to the group's TMEM stage of 64 columns. A turn's waits and
 //                       fences take as long as the conversion of 64 rows does, hence whole blocks.
@@ -32,12 +32,14 @@
 namespace gp {
 namespace {
 
-constexpr int kDeqGroups = 4;      // of four warps, one per TMEM lane quarter
-constexpr int kDeqWarps = 4 * kDeqGroups;
-constexpr int kTileThreads = 32 * (2 + kDeqWarps);
+// Groups of four dequantising warps, one warp per TMEM lane quarter: four, but two above 128 rows of x with
+// zero points in groups of 32. There the code rings of four groups leave no room for two x stages of 256
+// rows (512 x 4,096 x 14,336: 97 us in tiles of 128 rows, 74 with two groups), and the products of a
+// block take longer than its conversion anyway. Elsewhere four are no slower (62 us; two: 65).
+constexpr int tile_threads(int groups) { return 32 * (2 + 4 * groups); }
 constexpr int kTileN = 128;        // columns of W per tile: the TMEM lanes
 constexpr int kTileTiles = kTileN / 16;
-constexpr int kAStages = kDeqGroups;      // TMEM stages of dequantised weights, 64 columns (a block) each
+// a TMEM stage of dequantised weights per group: 64 columns, a block
 constexpr int kACols = 64;
 constexpr int kTmemCols = 512;            // 256 for the sums, 256 for the weights
 constexpr int kMaxStages = 8;       // x stages
@@ -57,6 +59,7 @@ struct W4TileArgs {
   int slice;       // k-blocks of a CTA
   int stages;      // x stages
   int depth;       // slots of a warp's code ring (2 or 3)
+  int groups;
   int* status;
   unsigned long long timeout_ns;
   int inject;
@@ -99,14 +102,14 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
 // TMEM lane of a tile <-> column: lane 16 i + r holds column 16 i + 2 (r % 8) + r / 8
 __device__ __forceinline__ int tile_column(int lane) { return (lane & ~15) + 2 * (lane & 7) + ((lane >> 3) & 1); }
 
-template <typename T, int UNITS, bool ZP>
-__global__ void __launch_bounds__(kTileThreads, 1)
+template <typename T, int UNITS, bool ZP, int GROUPS>
+__global__ void __launch_bounds__(tile_threads(GROUPS), 1)
     w4_tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ W4TileArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);
   constexpr int kScaleBytes = 32 * kWords;            // of a block of 16 columns
   constexpr int kSlot = code_slot(UNITS, ZP);
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], a_full[kAStages], a_empty[kAStages], d_full;
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], a_full[GROUPS], a_empty[GROUPS], d_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
   const int panel = a.rows * 128, stage_bytes = 2 * panel;  // x rows of 64 columns, SWIZZLE_128B
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(smem_u32(&full[i]), 1);
       mbar_init(smem_u32(&empty[i]), 1);
     }
-    for (int i = 0; i < kAStages; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
       mbar_init(smem_u32(&a_full[i]), 4);
       mbar_init(smem_u32(&a_empty[i]), 1);
     }
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (kTmemCols - kAStages * kACols);
+  const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (kTmemCols - GROUPS * kACols);
   const uint32_t second = a.rows <= 128 ? a.rows : 0;  // the second accumulator's first column, if there is one
   const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
   bool ok = true;  // of this role
@@ -206,7 +209,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         mma_commit(empty0 + s * 8);
       }
       __syncwarp();
-      if (++as == kAStages) as = 0, aph ^= 1;
+      if (++as == GROUPS) as = 0, aph ^= 1;
       if (++s == a.stages) s = 0, ph ^= 1;
     }
     // every product issued has completed before TMEM is read or released
@@ -247,11 +250,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               cp_async<4 * kWords>(my_scales + ld_at + i * (128 * kWords), scales[i]);
             }
           }
-          codes[i] += kDeqGroups * kW4BlockBytes;
-          scales[i] += kDeqGroups * kScaleBytes;
+          codes[i] += GROUPS * kW4BlockBytes;
+          scales[i] += GROUPS * kScaleBytes;
         }
       }
-      ld_b += kDeqGroups;
+      ld_b += GROUPS;
       ld_at = ld_at + kSlot == ring_end ? 0 : ld_at + kSlot;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint32_t at = 0;
     const uint32_t a_stage = a_tmem + group * kACols + lanes;
     int parity = 1;  // of the stage's last use
-    for (int b = group; b < nb; b += kDeqGroups, parity ^= 1) {
+    for (int b = group; b < nb; b += GROUPS, parity ^= 1) {
       load();
       if (a.depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
       else asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (a.ck == 1) {
     if (warp >= 2 && ok)  // a wait that ran out leaves the rows unwritten
 #pragma unroll 1
-      for (int c0 = quarter * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * kDeqGroups) {
+      for (int c0 = quarter * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * GROUPS) {
         float v[8];
         load_sums(c0, v);
         const int live = has_n ? static_cast<int>(min(static_cast<int64_t>(8), a.m - row0 - c0)) : 0;
@@ -350,7 +353,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     cluster_sync_all();
     if (warp >= 2)
 #pragma unroll 1
-      for (int c0 = quarter * 8; c0 < a.rows; c0 += 8 * kDeqGroups) {
+      for (int c0 = quarter * 8; c0 < a.rows; c0 += 8 * GROUPS) {
         float v[8];
         load_sums(c0, v);
         int owner = c0 / share, r = c0 % share;
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     cluster_sync_all();
     if (warp >= 2 && ok)
 #pragma unroll 1
-      for (int c = quarter; c < share; c += kDeqGroups) {
+      for (int c = quarter; c < share; c += GROUPS) {
         const int64_t row = row0 + rank * share + c;
         float v = 0.0f;
         for (int i = 0; i < a.ck; ++i)
@@ -382,15 +385,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
-template <typename T, int UNITS, bool ZP>
+template <typename T, int UNITS, bool ZP, int GROUPS>
 int tile_launch(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int smem, cudaStream_t s, const PdlIo& io) {
   static unsigned long long done_mask = 0;
-  auto kern = &w4_tile_kernel<T, UNITS, ZP>;
+  auto kern = &w4_tile_kernel<T, UNITS, ZP, GROUPS>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kSmemLimit - 2048, &done_mask);
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-  cfg.blockDim = dim3(kTileThreads, 1, 1);
+  cfg.blockDim = dim3(tile_threads(GROUPS), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -416,10 +419,17 @@ int tile_launch(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int sm
   return e == cudaSuccess ? GP_OK : set_error(GP_ERR_CUDA, "w4 tile launch: %s", cudaGetErrorString(e));
 }
 
+template <typename T, int UNITS, bool ZP>
+int tile_groups(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int smem, cudaStream_t s, const PdlIo& io) {
+  if constexpr (UNITS == 4 && ZP)
+    if (a.groups == 2) return tile_launch<T, UNITS, ZP, 2>(a, tx, ctas, smem, s, io);
+  return tile_launch<T, UNITS, ZP, 4>(a, tx, ctas, smem, s, io);
+}
+
 template <typename T, int UNITS>
 int tile_zeros(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int smem, cudaStream_t s, const PdlIo& io) {
-  return a.l.zeros ? tile_launch<T, UNITS, true>(a, tx, ctas, smem, s, io)
-                   : tile_launch<T, UNITS, false>(a, tx, ctas, smem, s, io);
+  return a.l.zeros ? tile_groups<T, UNITS, true>(a, tx, ctas, smem, s, io)
+                   : tile_groups<T, UNITS, false>(a, tx, ctas, smem, s, io);
 }
 
 template <typename T>
@@ -444,10 +454,7 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   a.timeout_ns = current_timeout_ns();
   a.inject = current_fault_injection();
   // rows per tile: as even as multiples of 16 up to 256 allow
-  // (128 where the scales and zero points of small groups take the shared memory)
-  const int slot = kDeqWarps * code_slot(a.l.units, a.l.zeros != 0);
-  const int max_rows = slot > 49152 ? kMaxTileRows / 2 : kMaxTileRows;
-  const int64_t row_tiles = (in.m + max_rows - 1) / max_rows;
+  const int64_t row_tiles = (in.m + kMaxTileRows - 1) / kMaxTileRows;
   a.rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
   a.row_tiles = static_cast<int>((in.m + a.rows - 1) / a.rows);
   const int64_t units = static_cast<int64_t>((a.l.n_tiles + kTileTiles - 1) / kTileTiles) * a.row_tiles;
@@ -456,14 +463,14 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   // CTA along K, 11.2 with two, 8.4 with four)
   static std::atomic<int> cluster_cache[64][4];
   static unsigned long long probe_mask = 0;
-  const void* probe = reinterpret_cast<const void*>(&w4_tile_kernel<__half, 1, false>);
+  const void* probe = reinterpret_cast<const void*>(&w4_tile_kernel<__half, 1, false, 4>);
   int rc = ensure_smem_attr(probe, kSmemLimit - 2048, &probe_mask);
   if (rc != GP_OK) return rc;
   int64_t best = -1;
   for (int ck = 1; ck <= 8; ck *= 2) {
     const int slice = (a.l.blocks + ck - 1) / ck;
     if (ck > 1 && ((ck - 1) * slice >= a.l.blocks || a.rows % ck != 0)) break;
-    const int at_once = w4_max_clusters(probe, kTileThreads, kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
+    const int at_once = w4_max_clusters(probe, tile_threads(4), kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
     const int64_t cost = (units + at_once - 1) / at_once * (4 * slice + (ck > 1 ? 48 : 30));
     if (best >= 0 && cost >= best) continue;
     best = cost;
@@ -472,6 +479,8 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   }
   if (units * a.ck >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "w4 linear: m = %lld", (long long)in.m);
   const int stage = 2 * a.rows * 128;
+  a.groups = a.rows > 128 && a.l.units == 4 && a.l.zeros != 0 ? 2 : 4;
+  const int slot = 4 * a.groups * code_slot(a.l.units, a.l.zeros != 0);
   a.depth = a.rows <= 128 && 3 * slot <= kSmemLimit / 2 ? 3 : 2;
   const int rings = a.depth * slot;
   a.stages = (kSmemLimit - 2048 - rings) / stage;
