@@ -563,13 +563,14 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   // its warps' blocks plus a join (about one block's time within a CTA, about three more across a
   // cluster); the fewest rounds of that over the GPU's SMs win. A pass takes up to 16 rows, fewer
   // where they would not fit in shared memory even spread over eight CTAs.
-  int per_pass = m > 8 ? 16 : 8, run = 2;
+  int per_pass = m > 8 ? 16 : 8, run = 2, clusters_best = 1;
   for (;; per_pass /= 2) {
     const int rows = static_cast<int>(m < per_pass ? m : per_pass), tt = per_pass > 8 ? 2 : 1;
       int64_t best = LLONG_MAX;
     for (int ck = 1; ck <= kMaxCluster; ck *= 2) {
       const int slice = (l.blocks + ck - 1) / ck;
       if (ck > 1 && (ck - 1) * slice >= l.blocks) break;  // a CTA without work
+      const int at_once = resident(ck);
       for (int ws = kWarps; ws >= 1; ws /= 2) {
         if (ws > 1 && ws / 2 >= slice) continue;  // warps without a block
         if (slice > 4 * ws && ws < kWarps) break; // more than four blocks a warp: rather more warps per tile
@@ -578,7 +579,7 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
         if (rows_smem(l, tt, ck, ws, slice, rows, 4 * 3) > kRowsSmem) r = 2;
         if (rows_smem(l, tt, ck, ws, slice, rows, r * kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
-        const int clusters = groups < resident(ck) ? groups : resident(ck);
+        const int clusters = groups < at_once ? groups : at_once;
         const int64_t iters = (groups + clusters - 1) / clusters;
         const int64_t cost = iters * (2 * per_warp + 3) + (ck > 1 ? 6 : 0);
         if (cost >= best) continue;
@@ -588,6 +589,7 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
         run = r;
         a.ws = ws;
         a.iters = static_cast<int>(iters);
+        clusters_best = clusters;
       }
     }
     if (best != LLONG_MAX) break;
@@ -600,8 +602,7 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   a.depth = kMaxDepth;
   while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth) > kRowsSmem) --a.depth;
   const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth));
-  const int groups = (l.n_tiles + kWarps / a.ws - 1) / (kWarps / a.ws);
-  const int clusters = groups < resident(a.ck) ? groups : resident(a.ck);
+  const int clusters = clusters_best;
   PdlIo io;
   io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(m) * l.n * (in.out_f32 ? 4 : 2));
   // the grid's y dimension holds 65,535 row tiles; longer inputs go in several launches

@@ -16,6 +16,7 @@ Each call goes through the C ABI (libgpipes.so) with raw device pointers.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -557,22 +558,23 @@ _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _refuse(name, t, dtype, shape, dev) -> None:
-    """Raise for a tensor that failed the short check (a None or a non-tensor included)."""
+    """Raise for a tensor that failed the short check (a non-tensor included)."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor")
     _check_input(name, t, dtype)
     if tuple(t.shape) != tuple(shape):
         raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.device != dev:
-        raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
+    if t.get_device() != dev:
+        raise RuntimeError(f"{name} is on {t.device}, expected cuda:{dev}")
 
 
 def _address(name, t, dtype, shape, dev):
-    """t's address if it is a contiguous tensor of that type and shape on dev; None for None."""
+    """t's address if it is a contiguous tensor of that type and shape on CUDA device dev (an
+    index); None for None."""
     if t is None:
         return None
     try:
-        if t.dtype == dtype and t.shape == shape and t.device == dev and t.is_contiguous():
+        if t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.is_contiguous():
             return t.data_ptr()
     except AttributeError:
         pass
@@ -581,20 +583,20 @@ def _address(name, t, dtype, shape, dev):
 
 
 def _cuda_2d(name, t):
-    """t's device, of a 2-D CUDA tensor."""
+    """The CUDA device index of a 2-D tensor."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise RuntimeError(f"{name} must be a 2-D tensor")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
-    return t.device
+    return t.get_device()
 
 
 def _launch(dev, fn, *args) -> None:
-    """fn(*args, stream) on dev's current stream, with dev as the current device."""
-    if _raw_stream is not None and _get_device() == dev.index:
-        rc = fn(*args, _raw_stream(dev.index))
+    """fn(*args, stream) on device dev's current stream, with dev as the current device."""
+    if _raw_stream is not None and _get_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
     else:
-        with _on_device(dev):
+        with _on_device(torch.device("cuda", dev)):
             rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
     if rc != L.GP_OK:
         L.check(rc)
@@ -726,7 +728,8 @@ class W4Weight:
         t = torch.empty(rows, self.n, dtype=dtype, device=self.device)
         outs = [None, None, None]
         outs[place] = t.data_ptr()
-        _launch(self.device, L.lib().gp_w4_unpack_out, self.spec, self._address("packed", self.device), *outs)
+        dev = self.packed.get_device()
+        _launch(dev, L.lib().gp_w4_unpack_out, self.spec, self._address("packed", dev), *outs)
         return t
 
     def codes(self):
@@ -754,7 +757,7 @@ def w4_quantize(w, group=128, zero_points=False) -> W4Weight:
     distance 7 (or, with zero_points, the range with zero becomes 0..15); gp_w4_quantize_out has
     the rule."""
     dev = _cuda_2d("w", w)
-    w4 = W4Weight.empty(w.shape[0], w.shape[1], group, w.dtype, zero_points, dev)
+    w4 = W4Weight.empty(w.shape[0], w.shape[1], group, w.dtype, zero_points, w.device)
     w4_quantize_out(w, w4)
     return w4
 
@@ -765,7 +768,7 @@ def w4_pack(codes, scales, zeros=None, group=128) -> W4Weight:
     dev = _cuda_2d("codes", codes)
     _cuda_2d("scales", scales)
     k, n = codes.shape
-    w4 = W4Weight.empty(k, n, group, scales.dtype, zeros is not None, dev)
+    w4 = W4Weight.empty(k, n, group, scales.dtype, zeros is not None, codes.device)
     rows = (-(-k // group), n)
     _launch(dev, L.lib().gp_w4_pack_out, w4.spec, _address("codes", codes, torch.uint8, (k, n), dev),
             _address("scales", scales, scales.dtype, rows, dev),
@@ -803,9 +806,14 @@ def w4_linear_out(x, w4, bias, out, act=L.ACT_NONE) -> None:
 def w4_linear(x, w4, bias=None, act=L.ACT_NONE) -> torch.Tensor:
     if not isinstance(w4, W4Weight):
         raise RuntimeError("w4 must be a W4Weight")
-    out = x.new_empty((x.shape[0], w4.n))
+    out = torch.empty(x.shape[0], w4.n, dtype=x.dtype, device=x.device)
     w4_linear_out(x, w4, bias, out, act=act)
     return out
+
+
+@functools.lru_cache(maxsize=None)
+def _pointer_array(n):
+    return ctypes.c_void_p * n
 
 
 _W4_CHAINS: dict = {}
@@ -842,7 +850,7 @@ def w4_mlp_out(x, weights, biases, out, *, acts, tail=L.TAIL_NONE, gamma=None, b
     w0 = weights[0]
     dtype, m, width = w0.dtype, x.shape[0], w0.k
     xp = _address("x", x, dtype, (m, width), dev)
-    wp, bp, widths = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), [width]
+    wp, bp, widths = [], [], [width]
     for i in range(n):
         w = weights[i]
         if w.group != w0.group or w.dtype != dtype or w.zero_points != w0.zero_points:
@@ -851,19 +859,20 @@ def w4_mlp_out(x, weights, biases, out, *, acts, tail=L.TAIL_NONE, gamma=None, b
             raise RuntimeError(f"w{i + 1} has shape {w.shape}, expected [{width}, N]")
         width = w.n
         widths.append(width)
-        wp[i] = w._address(f"w{i + 1}", dev)
-        bp[i] = _address(f"b{i + 1}", biases[i], dtype, (width,), dev)
+        wp.append(w._address("w", dev))
+        bp.append(_address("bias", biases[i], dtype, (width,), dev))
     gp, ep = _address("gamma", gamma, dtype, (width,), dev), _address("beta", beta, dtype, (width,), dev)
     if out is None:
         raise RuntimeError("out must be a tensor")
     op = _address("out", out, dtype, (m, width), dev)
     spec, nbytes = _w4_chain(m, tuple(widths), tuple(acts), tail, dtype, ln_eps)
     if workspace is None:
-        workspace = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     else:
         _address("workspace", workspace, torch.uint8, (workspace.numel(),), dev)
-    _launch(dev, L.lib().gp_w4_mlp_out, spec, w0.group, int(w0.zero_points), m, xp, wp, bp, gp, ep, op,
-            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel())
+    ptrs = _pointer_array(n)
+    _launch(dev, L.lib().gp_w4_mlp_out, spec, w0.group, int(w0.zero_points), m, xp, ptrs(*wp), ptrs(*bp), gp, ep,
+            op, None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel())
 
 
 def w4_mlp_workspace_bytes(m, weights, *, acts, tail=L.TAIL_NONE) -> int:
@@ -873,7 +882,7 @@ def w4_mlp_workspace_bytes(m, weights, *, acts, tail=L.TAIL_NONE) -> int:
 
 
 def w4_mlp(x, weights, biases, *, acts, tail=L.TAIL_NONE, gamma=None, beta=None, ln_eps=1e-5) -> torch.Tensor:
-    out = x.new_empty((x.shape[0], weights[-1].n))
+    out = torch.empty(x.shape[0], weights[-1].n, dtype=x.dtype, device=x.device)
     w4_mlp_out(x, weights, biases, out, acts=acts, tail=tail, gamma=gamma, beta=beta, ln_eps=ln_eps)
     return out
 
