@@ -117,20 +117,20 @@ __device__ __forceinline__ uint32_t w4_code_bits(float x, float below, float abo
 // Codes and scale of a group of G rows (largest magnitude to 7, or the range with zero to 15).
 // s is rounded to T first and the codes are taken against the rounded scale. A group whose scale
 // rounds to zero has code = zero point; one with a NaN or an infinity has a scale that is not
-// finite, and so has what it stands for. A group of 128 is shared by two threads 16 lanes apart, 64
-// rows each: 128 values did not fit a thread's registers.
+// finite, and so has what it stands for. A thread takes 64 rows, so two threads of a warp share a
+// group of 128 (128 values did not fit a thread's registers); 32 rows where pairs are loaded as two
+// elements.
 template <typename T, int G, bool ZP, bool VEC>
 __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_constant__ W4Layout l,
                                                                    const T* __restrict__ w, void* packed) {
   using P = Pair<T>;
   using V = typename P::V;
-  constexpr int kPer = G > 64 ? 64 : G, kSplit = G / kPer;
+  constexpr int kPer = VEC && G >= 64 ? 64 : 32, kSplit = G / kPer, kSeg = 32 / kSplit;
   pdl_wait_prior();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int part = kSplit == 2 ? lane >> 4 : 0;
-  const int pair = kSplit == 2 ? (blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5)) * 16 + (lane & 15)
-                               : static_cast<int>(blockIdx.x * kPackThreads + threadIdx.x);
+  const int part = lane / kSeg;
+  const int pair = (blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5)) * kSeg + lane % kSeg;
   const int tile = pair >> 3, g = pair & 7, c = 2 * pair;
   const bool in = tile < l.n_tiles;
   for (int64_t grp = blockIdx.y; grp < l.blocks * l.units; grp += gridDim.y) {
@@ -147,8 +147,9 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_
       if (ZP) lo = P::min(lo, x);
     }
     uint32_t hb = *reinterpret_cast<const uint32_t*>(&hi), lb = *reinterpret_cast<const uint32_t*>(&lo);
-    if (kSplit == 2) {
-      const uint32_t ho = __shfl_xor_sync(0xffffffffu, hb, 16), lo_o = __shfl_xor_sync(0xffffffffu, lb, 16);
+#pragma unroll
+    for (int o = kSeg; o < 32; o *= 2) {
+      const uint32_t ho = __shfl_xor_sync(0xffffffffu, hb, o), lo_o = __shfl_xor_sync(0xffffffffu, lb, o);
       hi = P::max(hi, *reinterpret_cast<const V*>(&ho));
       lo = P::min(lo, *reinterpret_cast<const V*>(&lo_o));
       hb = *reinterpret_cast<const uint32_t*>(&hi), lb = *reinterpret_cast<const uint32_t*>(&lo);
@@ -365,7 +366,7 @@ int quantize_g(const W4Layout& l, const T* w, void* packed, cudaStream_t s) {
   const bool vec = even_rows(l, w);
   auto kern = l.zeros ? (vec ? &w4_quantize_kernel<T, G, true, true> : &w4_quantize_kernel<T, G, true, false>)
                       : (vec ? &w4_quantize_kernel<T, G, false, true> : &w4_quantize_kernel<T, G, false, false>);
-  return launch_pack(kern, l, l.blocks * l.units, G > 64 ? 2 : 1, s, io, w, packed);
+  return launch_pack(kern, l, l.blocks * l.units, vec ? (G > 64 ? 2 : 1) : G / 32, s, io, w, packed);
 }
 
 template <typename T>
