@@ -1,30 +1,34 @@
-// Products with 4-bit weights for few rows: out [m, N] = act(x [m, K] W + b), W = s (q - z) (w4.cuh).
+// Products with 4-bit weights for few rows (one token to 16): out [m, N] = act(x [m, K] W + b),
+// W = s (q - z) (w4.cuh).
 //
 // With few rows the time is the weights' bytes (half a byte each), and what stands between them and
 // the memory's rate is the number of instructions per weight. So:
 //   - The matrix instruction is mma.sync m16n8k16 with the WEIGHTS as its 16-row operand (16 columns
-//     of W) and up to 8 rows of x as its 8-column operand; one to eight rows cost the same and the
-//     sums are fp32. (tcgen05 takes 16-bit weights from shared memory, which for so few rows only
-//     adds a store and a load per weight.)
+//     of W) and 8 or 16 rows of x on the other side; one to eight rows cost the same and the sums are
+//     fp32. (tcgen05 wants 16-bit weights in TMEM or shared memory, a store and a read per weight
+//     more: that form is w4_tiles.cu, for more rows.)
 //   - A code becomes an operand with one mask (w4.cuh): the operand is q plus a constant, scaled by a
 //     power of two. sum_k x (q - z) = sum_k x (q + c) - (c + z) sum_k x, and the second term starts
 //     the accumulator; the sums of x over each group are taken once per CTA. The group's scale
 //     multiplies the fp32 sum, so no weight is rounded. A first form that subtracted z from each
-//     weight, took codes through a cp.async ring and divided to find the group ran 174 instructions
-//     per 1,024 weights and 57 us at 1 x 8192 x 28672.
+//     weight and divided to find the group ran 348 instructions per 2,048 weights and 57 us at
+//     1 x 8,192 x 28,672 (fp16, groups of 128), where the bytes take 18.5.
 //
-//   - A CTA of 16 warps owns a slice of K (one of `ck` CTAs of a cluster does; ck = 1: all of it),
-//     keeps its part of the x rows in shared memory and goes over column tiles of 16. `ws` warps
-//     share a tile, each taking every ws-th 128-row block, so together they read whole stretches.
-//   - A producing thread streams the codes and scales through a ring of stages in shared memory. A
-//     stage is what the 16 warps take next: for each tile one stretch of ws * RUN neighbouring
-//     blocks, one bulk copy each for codes and scales. Waiting and loading stay out of the
-//     computing warps, whose loop is bound by its integer instructions (148 per block of 2,048 weights
-//     with a ring per warp that the warp itself fed, 101 without).
+//   - A CTA of 16 computing warps owns a slice of K (one of `ck` CTAs of a cluster does; ck = 1: all of
+//     it), keeps its part of the x rows in shared memory and goes over column tiles of 16. `ws` warps
+//     share a tile; a warp takes RUN neighbouring 128-row blocks at a time.
+//   - One thread streams the codes and scales through a ring of stages in shared memory. A stage is
+//     what the 16 warps take next: for each tile one stretch of ws * RUN neighbouring blocks, one bulk
+//     copy each for codes and scales. (Copies of a block at a time, started by each warp for itself,
+//     were slower in two ways: the copy engine took about 35 ns a piece, and waiting and loading
+//     were 42 of the computing warps' 143 instructions per 2,048 weights. 31.5 us.)
 //   - The codes of the next tiles are in flight while the sums of this one are joined by warps of
-//     their own.
-//   - The warps' sums are joined in shared memory, the CTAs' through distributed shared memory,
-//     both in a fixed order: results do not depend on timing.
+//     their own, in shared memory and across a cluster through st.async, both in a fixed order:
+//     results do not depend on timing.
+// Measured (CUDA-graph replays over more weights than L2 holds): 1 x 8,192 x 28,672 fp16 26.7 us, 4.5
+// TB/s of 121 MB; 16 rows 48.7 us; 1 x 1,024 x 4,096 3.6 us. What is left at one row: about 3.5 us of
+// launch and first latency, 13 tiles on the busiest SM for 12.1 on average, and the integer pipe
+// (53 of its 88 cycles per block and SM).
 #include <climits>
 
 #include "../../include/gpipes.h"
@@ -42,6 +46,7 @@ constexpr int kJoiners = 32 * kJoinWarps;
 constexpr int kThreads = 32 * (kWarps + kJoinWarps + 1);
 constexpr int kPartStride = 20;     // floats per row of a warp's 16 x rows sums: conflict-free float2 stores
 constexpr int kMaxCluster = 8;
+constexpr int64_t kRowsMax = 16;    // rows that go to this kernel
 constexpr int kMaxDepth = 8;        // ring stages
 constexpr int kMinDepth = 2;
 constexpr int kRowsSmem = kSmemLimit - 3072;  // dynamic: the barriers are static
@@ -559,70 +564,67 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   a.bias = in.bias;
   a.out_f32 = in.out_f32;
   a.act = in.act;
-  // Split of the work: ck CTAs of a cluster along K, ws warps per column tile. A tile group costs
-  // its warps' blocks plus a join (about one block's time within a CTA, about three more across a
-  // cluster); the fewest rounds of that over the GPU's SMs win. A pass takes up to 16 rows, fewer
-  // where they would not fit in shared memory even spread over eight CTAs.
-  int per_pass = m > 8 ? 16 : 8, run = 2, clusters_best = 1;
+  // Split of the work. A pass takes up to 16 rows (8 and fewer for the kernel of one row tile), fewer
+  // where they would not fit in shared memory even spread over eight CTAs. Of the splits into ck CTAs
+  // along K and ws warps per tile, the one with the least time on the busiest SM: per tile group its
+  // warps' blocks and about one and a half blocks more, three more in all where a cluster joins. A warp has at
+  // most four blocks of a tile if there are warps for that: with more, few tiles are long under way
+  // (1 x 4,096 x 14,336: 9.3 us with ws = 8, 10.1 with 4, 10.8 with 2).
+  int per_pass = m > 8 ? 16 : 8, run = 2, clusters = 1;
   for (;; per_pass /= 2) {
     const int rows = static_cast<int>(m < per_pass ? m : per_pass), tt = per_pass > 8 ? 2 : 1;
-      int64_t best = LLONG_MAX;
+    int64_t best = LLONG_MAX;
     for (int ck = 1; ck <= kMaxCluster; ck *= 2) {
       const int slice = (l.blocks + ck - 1) / ck;
       if (ck > 1 && (ck - 1) * slice >= l.blocks) break;  // a CTA without work
       const int at_once = resident(ck);
       for (int ws = kWarps; ws >= 1; ws /= 2) {
         if (ws > 1 && ws / 2 >= slice) continue;  // warps without a block
-        if (slice > 4 * ws && ws < kWarps) break; // more than four blocks a warp: rather more warps per tile
+        if (slice > 4 * ws && ws < kWarps) break;
         const int per_warp = (slice + ws - 1) / ws;
         int r = per_warp > 2 ? 4 : 2;
         if (rows_smem(l, tt, ck, ws, slice, rows, 4 * 3) > kRowsSmem) r = 2;
         if (rows_smem(l, tt, ck, ws, slice, rows, r * kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
-        const int clusters = groups < at_once ? groups : at_once;
-        const int64_t iters = (groups + clusters - 1) / clusters;
+        const int n = groups < at_once ? groups : at_once;
+        const int64_t iters = (groups + n - 1) / n;
         const int64_t cost = iters * (2 * per_warp + 3) + (ck > 1 ? 6 : 0);
         if (cost >= best) continue;
         best = cost;
         a.ck = ck;
         a.slice = slice;
-        run = r;
         a.ws = ws;
         a.iters = static_cast<int>(iters);
-        clusters_best = clusters;
+        run = r;
+        clusters = n;
       }
     }
     if (best != LLONG_MAX) break;
     if (per_pass == 1) return set_error(GP_ERR_UNSUPPORTED, "w4 linear: K = %d", l.k);
   }
+  const int rows = static_cast<int>(m < per_pass ? m : per_pass), tt = per_pass > 8 ? 2 : 1;
+  a.m = m;
   a.rows = per_pass;
+  a.x = in.x;
+  a.out = in.out;
   a.x_stride = rows_x_stride(a.slice);
-  const int tt = per_pass > 8 ? 2 : 1;
-  const int rows = static_cast<int>(m < per_pass ? m : per_pass);
   a.depth = kMaxDepth;
   while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth) > kRowsSmem) --a.depth;
   const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth));
-  const int clusters = clusters_best;
   PdlIo io;
   io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(m) * l.n * (in.out_f32 ? 4 : 2));
-  // the grid's y dimension holds 65,535 row tiles; longer inputs go in several launches
-  const int64_t step = 65535ll * per_pass;
-  for (int64_t r0 = 0; r0 < m; r0 += step) {
-    W4RowsArgs c = a;
-    c.m = m - r0 < step ? m - r0 : step;
-    c.x = static_cast<const char*>(in.x) + r0 * l.k * 2;
-    c.out = static_cast<char*>(in.out) + r0 * l.n * (in.out_f32 ? 4 : 2);
-    const int64_t rt = (c.m + per_pass - 1) / per_pass;
-    rc = in.dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(c, tt, run, smem, clusters, rt, s, io)
-                          : rows_tt<__half>(c, tt, run, smem, clusters, rt, s, io);
-    if (rc != GP_OK) return rc;
-    count_launches(1);
-  }
-  return GP_OK;
+  const int64_t passes = (m + per_pass - 1) / per_pass;
+  rc = in.dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(a, tt, run, smem, clusters, passes, s, io)
+                           : rows_tt<__half>(a, tt, run, smem, clusters, passes, s, io);
+  if (rc == GP_OK) count_launches(1);
+  return rc;
 }
 
+// Up to 16 rows the row kernel, from 17 on the tile kernel. Measured on either side of the border
+// (us, row / tile kernel; 9, 16 and 64 rows): 4,096 x 14,336 15.3 / 16.3, 16.7 / 16.4, 66 / 19;
+// 8,192 x 28,672 42 / 58, 43 / 58, 199 / 66; 1,024 x 4,096 4.4 / 5.5, 5.3 / 5.5, 20 / 7.
 int launch_w4_linear(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev) {
-  return a.m <= 16 ? launch_w4_rows(a, s, dev) : launch_w4_tiles(a, s, dev);
+  return a.m <= kRowsMax ? launch_w4_rows(a, s, dev) : launch_w4_tiles(a, s, dev);
 }
 
 }  // namespace gp

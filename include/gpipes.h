@@ -324,8 +324,10 @@ GP_API int gp_w4_unpack_out(const gp_w4_spec* spec, const void* packed, uint8_t*
 /* w [K, N] (T) = s (q - z), rounded once. */
 GP_API int gp_w4_dequantize_out(const gp_w4_spec* spec, const void* packed, void* w, void* stream);
 
-/* out [m, N] = act(x [m, K] W + bias) on packed weights, T; bias [N] or NULL; act a gp_act. Made for
- * few rows, where the weights' bytes are the time; any m works. x 16-byte, out and bias 2-byte aligned. */
+/* out [m, N] = act(x [m, K] W + bias) on packed weights, T; bias [N] or NULL; act a gp_act. From single
+ * tokens to prompts: up to 16 rows the sums over each group are scaled in fp32 and no weight is rounded;
+ * from 17 rows on each weight s (q - z) is rounded to T first, as gp_w4_dequantize_out gives it. A row of x
+ * with an infinity may give NaN where the sum is infinite. x 16-byte, out and bias 2-byte aligned. */
 GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, const void* packed,
                             const void* bias, void* out, void* stream);
 

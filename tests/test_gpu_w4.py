@@ -211,6 +211,16 @@ def test_linear_shapes(cuda_dev, k, n, group):
         check_linear(m, k, n, dtype, group, zeros, L.ACT_NONE, False, cuda_dev)
 
 
+@pytest.mark.parametrize("m", [17, 128, 129, 257, 530])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_tiles(cuda_dev, m, group, zeros):
+    """Row tiles of every kind of the kernel for more rows: one and two accumulators, two and four
+    dequantising groups, several tiles, absent column tiles, K alone and split over a cluster."""
+    for k, n in ((328, 264), (2056, 136)):
+        check_linear(m, k, n, torch.float16 if zeros else torch.bfloat16, group, zeros, L.ACT_SILU, True, cuda_dev)
+
+
 @pytest.mark.parametrize("act", [L.ACT_NONE, L.ACT_RELU, L.ACT_GELU_TANH, L.ACT_SILU, L.ACT_SIGMOID])
 @pytest.mark.parametrize("m", [1, 20, 200])
 def test_linear_activations(cuda_dev, act, m):
@@ -485,6 +495,46 @@ def test_chain_kernels_next_to_them(cuda_dev):
     want = run(True)
     for _ in range(5):
         assert torch.equal(run(False), want)
+
+
+def test_host_threads(cuda_dev):
+    """Calls of several host threads at once, each on its own stream and buffers."""
+    import threading
+
+    dtype = torch.float16
+    w4 = cuda_ext.w4_pack(*make(1024, 520, dtype, 64, True), group=64)
+    xs = [rows(m, 1024, dtype, m) for m in (1, 5, 16, 40)]
+    wants = [cuda_ext.w4_linear(x, w4) for x in xs]
+    norms = [cuda_ext.block_norm(x, x, pre=L.NORM_RMS)[1] for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got, h = cuda_ext.w4_linear(xs[i], w4), cuda_ext.block_norm(xs[i], xs[i], pre=L.NORM_RMS)[1]
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(got, wants[i]) and torch.equal(h, norms[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one():
+    for m in (2, 40):
+        codes, scales, z = make(256, 96, torch.float16, 64, True, dev="cuda:1")
+        x = rows(m, 256, torch.float16, dev="cuda:1")
+        got = cuda_ext.w4_linear(x, cuda_ext.w4_pack(codes, scales, z, group=64))
+        _, h = cuda_ext.block_norm(x, pre=L.NORM_RMS)
+        assert got.device == h.device == x.device
+        w4 = cuda_ext.w4_pack(codes.to("cuda:0"), scales.to("cuda:0"), z.to("cuda:0"), group=64)
+        assert torch.equal(got.to("cuda:0"), cuda_ext.w4_linear(x.to("cuda:0"), w4))
 
 
 def test_device_refusals(cuda_dev):
