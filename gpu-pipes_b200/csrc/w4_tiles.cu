@@ -42,7 +42,7 @@ constexpr int kTileTiles = kTileN / 16;
 // a TMEM stage of dequantised weights per group: 64 columns, a block
 constexpr int kACols = 64;
 constexpr int kTmemCols = 512;            // 256 for the sums, 256 for the weights
-constexpr int kMaxStages = 8;       // x stages
+constexpr int kMaxStages = 4;       // x stages
 constexpr int kMaxTileRows = 256;
 
 struct W4TileArgs {
@@ -121,6 +121,12 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   const int b0 = rank * a.slice, nb = min(a.slice, a.l.blocks - b0);
   const int tiles = min(kTileTiles, a.l.n_tiles - tile0);
 
+  // With as many x stages as TMEM stages, a block's x panels and weights share one barrier for "full" and
+  // one for "free": one wait and one commit less per turn of the MMA issuer, whose turns bound the kernel
+  // at few rows.
+  const bool merged = a.stages == GROUPS;
+  const uint32_t full0 = smem_u32(merged ? a_full : full), empty0 = smem_u32(merged ? a_empty : empty);
+
   if ((smem_u32(smem) & 1023u) != 0) {  // the same in every CTA of the grid
     pdl_wait_prior();
     if (threadIdx.x == 0) atomicCAS(a.status, 0, kDevBadSmemAlign);
@@ -132,7 +138,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
       mbar_init(smem_u32(&empty[i]), 1);
     }
     for (int i = 0; i < GROUPS; ++i) {
-      mbar_init(smem_u32(&a_full[i]), 4);
+      mbar_init(smem_u32(&a_full[i]), merged ? 5 : 4);  // the group's warps (and the x panels)
       mbar_init(smem_u32(&a_empty[i]), 1);
     }
     mbar_init(smem_u32(&d_full), 1);
@@ -166,20 +172,20 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
       const uint64_t keep = l2_policy_evict_last();  // x is read by every column tile
       int s = 0, ph = 0;
       for (int b = 0; b < nb; ++b) {
-        if (b >= a.stages && !mbar_wait(smem_u32(&empty[s]), ph ^ 1, wctx, kDevTimeoutProducer)) {
+        if (b >= a.stages && !mbar_wait(empty0 + s * 8, ph ^ 1, wctx, kDevTimeoutProducer)) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(smem_u32(&full[s]), stage_bytes);
+        mbar_arrive_expect_tx(full0 + s * 8, stage_bytes);
         for (int p = 0; p < 2; ++p)
-          tma_load_2d_hint(smem_u32(smem) + s * stage_bytes + p * panel, &tx, smem_u32(&full[s]),
+          tma_load_2d_hint(smem_u32(smem) + s * stage_bytes + p * panel, &tx, full0 + s * 8,
                            (b0 + b) * kW4Block + p * 64, static_cast<int>(row0), keep);
         if (++s == a.stages) s = 0, ph ^= 1;
       }
       if (!ok)  // copies under way end (waited for with a limit) before their memory is used again or goes away
         for (int j = 0; j < a.stages; ++j) {
           const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(smem_u32(&full[s]), ph ^ 1) && globaltimer_ns() - t0 < a.timeout_ns) {
+          while (!mbar_try_wait(full0 + s * 8, ph ^ 1) && globaltimer_ns() - t0 < a.timeout_ns) {
           }
           if (++s == a.stages) s = 0, ph ^= 1;
         }
@@ -192,10 +198,11 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
     const uint32_t idesc = make_idesc_f16(kTileN, a.rows, Elem<T>::kIsBf16, 0, 0);
     const uint32_t d = __shfl_sync(0xffffffffu, d_tmem, 0), at0 = __shfl_sync(0xffffffffu, a_tmem, 0);
     const uint64_t desc0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
-    const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), a_full0 = smem_u32(a_full), a_empty0 = smem_u32(a_empty);
+    const uint32_t a_full0 = smem_u32(a_full), a_empty0 = smem_u32(a_empty);
     int s = 0, ph = 0, as = 0, aph = 0;
     for (int b = 0; b < nb; ++b) {
-      ok = mbar_wait(full0 + s * 8, ph, wctx, kDevTimeoutMma) && mbar_wait(a_full0 + as * 8, aph, wctx, kDevTimeoutMma);
+      ok = mbar_wait(a_full0 + as * 8, aph, wctx, kDevTimeoutMma) &&
+           (merged || mbar_wait(full0 + s * 8, ph, wctx, kDevTimeoutMma));
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint64_t bdesc = desc0 + static_cast<uint64_t>(s * (stage_bytes >> 4));
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
                  bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2), idesc,
                  (b != 0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u);
         mma_commit(a_empty0 + as * 8);
-        mma_commit(empty0 + s * 8);
+        if (!merged) mma_commit(empty0 + s * 8);
       }
       __syncwarp();
       if (++as == GROUPS) as = 0, aph ^= 1;
@@ -481,10 +488,12 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   const int stage = 2 * a.rows * 128;
   a.groups = a.rows > 128 && a.l.units == 4 && a.l.zeros != 0 ? 2 : 4;
   const int slot = 4 * a.groups * code_slot(a.l.units, a.l.zeros != 0);
-  a.depth = a.rows <= 128 && 3 * slot <= kSmemLimit / 2 ? 3 : 2;
+  // as many x stages as groups where that fits; then code slots, three if possible
+  const int budget = kSmemLimit - 2048;
+  a.depth = a.groups * stage + 3 * slot <= budget ? 3 : 2;
   const int rings = a.depth * slot;
-  a.stages = (kSmemLimit - 2048 - rings) / stage;
-  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  a.stages = (budget - rings) / stage;
+  if (a.stages > a.groups) a.stages = a.groups;
   int smem = a.stages * stage + rings;
   const int sums = a.ck > 1 ? a.rows * kTileN * 4 : 0;
   if (smem < sums) smem = sums;
