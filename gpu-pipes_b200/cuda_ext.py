@@ -591,13 +591,18 @@ def _cuda_2d(name, t):
     return t.get_device()
 
 
+def _elsewhere(dev, fn, *args) -> int:
+    """fn(*args, stream) with dev made the current device."""
+    with _on_device(torch.device("cuda", dev)):
+        return fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _launch(dev, fn, *args) -> None:
     """fn(*args, stream) on device dev's current stream, with dev as the current device."""
     if _raw_stream is not None and _get_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
-        with _on_device(torch.device("cuda", dev)):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = _elsewhere(dev, fn, *args)
     if rc != L.GP_OK:
         L.check(rc)
 
@@ -637,30 +642,33 @@ def block_norm_out(x, y, r, h, *, post=L.NORM_NONE, pre=L.NORM_NONE, gate=None, 
     f32 = torch.float32
     dtype = None  # the 16-bit type of the call
     for t in (h, y, x, r, gate, post_gamma, post_beta, pre_gamma, pre_beta):
-        if t is not None and t.dtype != f32:
+        if t is not None and t.dtype is not f32:
             dtype = t.dtype
             break
-    dt = _dtype_code("h", dtype if dtype is not None else torch.float16)  # all fp32: no matter
+    dt = _DT.get(dtype) if dtype is not None else L.GP_F16  # all fp32: no matter
+    if dt is None:
+        _dtype_code("h", dtype)
     stream_t = x if x is not None else r
-    stream = f32 if stream_t is not None and stream_t.dtype == f32 else dtype
-    ydt = f32 if y is not None and y.dtype == f32 else dtype
-    gate_rows, gate_shape = 0, (width,)
+    stream = f32 if stream_t is not None and stream_t.dtype is f32 else dtype
+    ydt = f32 if y is not None and y.dtype is f32 else dtype
+    row = (width,)
+    gate_rows, gate_shape = 0, row
     if gate is not None and gate.dim() == 2:
         groups = gate.shape[0]
         if m and (groups == 0 or m % groups):
             raise RuntimeError(f"{m} rows are not a multiple of {groups} gate rows")
         gate_rows, gate_shape = m // groups if m else 0, (groups, width)
-    row = (width,)
     _launch(dev, L.lib().gp_block_norm_out,
-            _norm_spec(width, dt, int(stream == f32), int(ydt == f32), post, pre, post_eps, pre_eps,
-                       x_scale, y_scale, gate_rows),
-            m, _address("x", x, stream, shape, dev), _address("y", y, ydt, shape, dev),
-            _address("gate", gate, dtype, gate_shape, dev),
-            _address("post_gamma", post_gamma, dtype, row, dev),
-            _address("post_beta", post_beta, dtype, row, dev),
-            _address("pre_gamma", pre_gamma, dtype, row, dev),
-            _address("pre_beta", pre_beta, dtype, row, dev),
-            _address("r", r, stream, shape, dev), _address("h", h, dtype, shape, dev))
+            _norm_spec(width, dt, stream is f32, ydt is f32, post, pre, post_eps, pre_eps, x_scale, y_scale, gate_rows),
+            m, None if x is None else _address("x", x, stream, shape, dev),
+            None if y is None else _address("y", y, ydt, shape, dev),
+            None if gate is None else _address("gate", gate, dtype, gate_shape, dev),
+            None if post_gamma is None else _address("post_gamma", post_gamma, dtype, row, dev),
+            None if post_beta is None else _address("post_beta", post_beta, dtype, row, dev),
+            None if pre_gamma is None else _address("pre_gamma", pre_gamma, dtype, row, dev),
+            None if pre_beta is None else _address("pre_beta", pre_beta, dtype, row, dev),
+            None if r is None else _address("r", r, stream, shape, dev),
+            None if h is None else _address("h", h, dtype, shape, dev))
 
 
 def block_norm(x, y=None, *, dtype=None, want_r=True, post=L.NORM_NONE, pre=L.NORM_NONE, **kw):
@@ -681,9 +689,19 @@ def block_norm(x, y=None, *, dtype=None, want_r=True, post=L.NORM_NONE, pre=L.NO
                     break
             else:
                 raise RuntimeError("dtype must be given where every tensor is float32")
-        h = torch.empty_like(first, dtype=dtype)
+        h = torch.empty_like(first) if first.dtype is dtype else torch.empty_like(first, dtype=dtype)
     block_norm_out(x, y, r, h, post=post, pre=pre, **kw)
     return r, h
+
+
+@functools.lru_cache(maxsize=1024)
+def _w4_spec(k, n, group, dtype, zero_points):
+    """(the C description, bytes of the packed form)"""
+    spec = ctypes.byref(L.GpW4Spec(k, n, group, _dtype_code("weights", dtype), int(zero_points)))
+    nbytes = L.lib().gp_w4_packed_bytes(spec)
+    if nbytes < 0:
+        L.check(int(nbytes))
+    return spec, nbytes
 
 
 class W4Weight:
@@ -695,11 +713,7 @@ class W4Weight:
     def __init__(self, packed, k, n, group, dtype, zero_points):
         self.k, self.n, self.group = int(k), int(n), int(group)
         self.dtype, self.zero_points = dtype, bool(zero_points)
-        self.spec = ctypes.byref(L.GpW4Spec(self.k, self.n, self.group, _dtype_code("weights", dtype),
-                                            int(self.zero_points)))
-        self.nbytes = L.lib().gp_w4_packed_bytes(self.spec)
-        if self.nbytes < 0:
-            L.check(int(self.nbytes))
+        self.spec, self.nbytes = _w4_spec(self.k, self.n, self.group, dtype, self.zero_points)
         if packed is not None:
             _check_input("packed", packed, torch.uint8)
             if tuple(packed.shape) != (self.nbytes,):
