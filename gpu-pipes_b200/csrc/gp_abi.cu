@@ -558,9 +558,6 @@ static int block_norm(const gp_block_norm_spec* s, int64_t m, const void* x, con
   for (int i = 2; i < 7; ++i)
     if (overlap(r, n * sb, ptrs[i], i == 2 ? gr * row : row) || overlap(h, n * 2, ptrs[i], i == 2 ? gr * row : row))
       return set_error(GP_ERR_ARG, "an output overlaps the gate or a norm's parameters");
-  DeviceInfo dev;
-  int rc = device_info(&dev);
-  if (rc != GP_OK) return rc;
   BlockNormArgs a;
   a.m = m;
   a.gate_rows = s->gate_rows;
@@ -580,7 +577,7 @@ static int block_norm(const gp_block_norm_spec* s, int64_t m, const void* x, con
   a.pre_beta = pre_beta;
   a.r = r;
   a.h = h;
-  rc = launch_block_norm(a, s->dtype, s->stream_f32 != 0, s->y_f32 != 0, stream);
+  const int rc = launch_block_norm(a, s->dtype, s->stream_f32 != 0, s->y_f32 != 0, stream);
   return rc == GP_OK ? finish_launch(stream, 1) : rc;
 }
 
@@ -622,20 +619,20 @@ static int w4_check(const W4Layout& l, const void* packed, const W4Buf* bufs, in
 }
 
 // One layer; the launcher counts its launches.
-static int w4_linear(const W4Layout& l, int dtype, int64_t m, int act, const void* x, const void* packed,
-                     const void* bias, void* out, bool out_f32, cudaStream_t stream) {
+static int w4_linear(const W4LinearArgs& a, cudaStream_t stream) {
   DeviceInfo dev;
   const int rc = device_info(&dev);
-  if (rc != GP_OK) return rc;
-  return launch_w4_linear({l, dtype, m, x, packed, bias, act, out, out_f32}, stream, dev);
+  return rc == GP_OK ? launch_w4_linear(a, stream, dev) : rc;
 }
 
 static uint64_t align256(uint64_t b) { return (b + 255) / 256 * 256; }
 
-// Two buffers of hidden activations (layers alternate), and the fp32 rows before a tail.
+// Two buffers of hidden activations (layers alternate), and the fp32 rows before a tail. Each rounding of
+// the activations between two layers adds about as much error as the one at the end. One such rounding is
+// accepted (two layers: sqrt(2) times the final rounding); in longer chains hidden activations are two T.
 struct W4MlpPlan {
   uint64_t hidden = 0, pre = 0, total = 0;
-  int buffers = 0;
+  int buffers = 0, planes = 1;
 };
 
 static int w4_mlp_plan(const gp_mlp_spec* s, int64_t m, W4MlpPlan* p) {
@@ -663,7 +660,10 @@ static int w4_mlp_plan(const gp_mlp_spec* s, int64_t m, W4MlpPlan* p) {
   int widest = 0;
   for (int i = 1; i < nl; ++i) widest = s->widths[i] > widest ? s->widths[i] : widest;
   p->buffers = nl > 2 ? 2 : nl - 1;
-  p->hidden = align256(static_cast<uint64_t>(m) * widest * 2);
+  p->planes = nl > 2 ? 2 : 1;
+  if (p->planes == 2 && m >= (int64_t(1) << 30))
+    return set_error(GP_ERR_SHAPE, "m = %lld exceeds 2^30-1 for %d layers", (long long)m, nl);
+  p->hidden = align256(static_cast<uint64_t>(m) * widest * 2 * p->planes);
   p->pre = s->tail != GP_TAIL_NONE ? align256(static_cast<uint64_t>(m) * last * 4) : 0;
   p->total = p->buffers * p->hidden + p->pre;
   return GP_OK;
@@ -717,8 +717,12 @@ static int w4_mlp(const gp_mlp_spec* s, int group, int zero_points, int64_t m, c
     const bool last = i + 1 == nl;
     void* to = last ? (normed ? static_cast<void*>(ws + plan.buffers * plan.hidden) : out)
                     : static_cast<void*>(ws + (plan.buffers == 2 ? (i & 1) : 0) * plan.hidden);
-    rc = w4_linear(l[i], s->dtype, m, last && normed ? GP_ACT_NONE : s->act[i], in, packed[i],
-                   b != nullptr ? b[i] : nullptr, to, last && normed, stream);
+    W4LinearArgs layer{l[i], s->dtype, m, in, packed[i], b != nullptr ? b[i] : nullptr,
+                       last && normed ? GP_ACT_NONE : s->act[i], to, last && normed};
+    layer.exact = nl > 1;  // the layers' errors add up
+    layer.x_planes = i > 0 ? plan.planes : 1;
+    layer.out_planes = last ? 1 : plan.planes;
+    rc = w4_linear(layer, stream);
     if (rc != GP_OK) return rc;
     in = to;
   }
@@ -1180,7 +1184,7 @@ int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, 
   rc = w4_check(l, packed, bufs, 3);
   if (rc != GP_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  rc = w4_linear(l, spec->dtype, m, act, x, packed, bias, out, false, s);
+  rc = w4_linear({l, spec->dtype, m, x, packed, bias, act, out, false}, s);
   return rc == GP_OK ? finish_launch(s, 1, 0) : rc;
 }
 

@@ -128,17 +128,25 @@ struct W4Exact<__half> {
       c[0] = __float2half2_rn(-1032.0f), c[1] = __float2half2_rn(-72.0f);
     }
   }
-  // r[2 column + j]: rows (0, 1) (j = 0) and (2, 3) of the word, as tcgen05.st 16x256b takes them
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* r) const {
+  // r[2 column + j]: rows (0, 1) (j = 0) and (2, 3) of the word, as tcgen05.st 16x256b takes them. rest: what
+  // each rounding took away, itself exact in T (s (q - z) has four bits more than T; only below T's
+  // smallest normal value is it rounded once more).
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* r, uint32_t* rest = nullptr) const {
     const __half2 sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t v = i == 0 ? w : w >> 8;
       const uint32_t lo = (v & 0x000F000Fu) | 0x64006400u, hi = (v & 0x00F000F0u) | 0x64006400u;
-      const __half2 a = __hmul2(__hadd2(*reinterpret_cast<const __half2*>(&lo), c[0]), s[0]);
-      const __half2 b = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, c[1]), s[1]);
+      const __half2 qa = __hadd2(*reinterpret_cast<const __half2*>(&lo), c[0]);
+      const __half2 qb = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, c[1]);
+      const __half2 a = __hmul2(qa, s[0]), b = __hmul2(qb, s[1]);
       r[i] = *reinterpret_cast<const uint32_t*>(&a);
       r[2 + i] = *reinterpret_cast<const uint32_t*>(&b);
+      if (rest != nullptr) {
+        const __half2 ea = __hfma2(qa, s[0], __hneg2(a)), eb = __hfma2(qb, s[1], __hneg2(b));
+        rest[i] = *reinterpret_cast<const uint32_t*>(&ea);
+        rest[2 + i] = *reinterpret_cast<const uint32_t*>(&eb);
+      }
     }
   }
 };
@@ -157,16 +165,29 @@ struct W4Exact<__nv_bfloat16> {
       c[0] = c[1] = __float2bfloat162_rn(-24.0f);
     }
   }
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* r) const {
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* r, uint32_t* rest = nullptr) const {
     uint32_t p[4];
     W4Deq<__nv_bfloat16>::pairs(w, p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // p[2 j + column], j: rows (0, 1) / (2, 3)
-      const __nv_bfloat162 a = __hmul2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&p[i]), c[i & 1]), s[i & 1]);
+      const __nv_bfloat162 q = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&p[i]), c[i & 1]);
+      const __nv_bfloat162 a = __hmul2(q, s[i & 1]);
       r[2 * (i & 1) + (i >> 1)] = *reinterpret_cast<const uint32_t*>(&a);
+      if (rest != nullptr) {
+        const __nv_bfloat162 e = __hfma2(q, s[i & 1], __hneg2(a));
+        rest[2 * (i & 1) + (i >> 1)] = *reinterpret_cast<const uint32_t*>(&e);
+      }
     }
   }
 };
+
+// v as two T, in the low halves; an infinity (a value past T's range) has no second part.
+template <typename T>
+__device__ __forceinline__ void w4_two(float v, uint16_t& hi, uint16_t& lo) {
+  hi = static_cast<uint16_t>(Elem<T>::pack(v, 0.0f));
+  const float f = Elem<T>::unpack(hi).x;
+  lo = static_cast<uint16_t>(fabsf(f) <= 3.4028235e38f ? Elem<T>::pack(v - f, 0.0f) : 0u);
+}
 
 // W words from shared memory in one access (two for W = 8)
 template <int W>
@@ -189,11 +210,23 @@ __device__ __forceinline__ void w4_lds(uint32_t p, uint32_t (&v)[W]) {
 // its argument (0.5 (1 + tanh(t)) = sigmoid(2 t)). The fast exponential and quotient are within a few
 // units of 2^-22 |u| of the exact ones, far below the 16-bit rounding that follows. Written without
 // calls: expf, tanhf and divisions in the epilogues took 36 of 98 us at 512 x 4,096 x 14,336.
-__device__ __forceinline__ float w4_act(int act, float v) {
-  if (act == kActNone) return v;
-  if (act == kActRelu) return v > 0.0f ? v : (v == v ? 0.0f : v);
-  const float u = act == kActGeluTanh ? 1.5957691216057308f * fmaf(0.044715f * v, v * v, v) : v;
-  return __fdividef(act == kActSigmoid ? 1.0f : v, 1.0f + __expf(-u));
+// The choice is made once for N values, whose arithmetic then overlaps.
+template <int N>
+__device__ __forceinline__ void w4_act(int act, float (&v)[N]) {
+  if (act == kActNone) return;
+  if (act == kActRelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] > 0.0f ? v[i] : (v[i] == v[i] ? 0.0f : v[i]);
+    return;
+  }
+  float e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = -v[i];
+  if (act == kActGeluTanh)
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = -1.5957691216057308f * fmaf(0.044715f * v[i], v[i] * v[i], v[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __fdividef(act == kActSigmoid ? 1.0f : v[i], 1.0f + __expf(e[i]));
 }
 
 // ---- host interface (w4_pack.cu, w4_linear.cu); dtype is GP_F16 / GP_BF16
@@ -204,7 +237,8 @@ int launch_w4_unpack(const W4Layout& l, int dtype, const void* packed, uint8_t* 
                      cudaStream_t s);
 int launch_w4_dequantize(const W4Layout& l, int dtype, const void* packed, void* w, cudaStream_t s);
 
-// out [m, n] = act(x [m, k] W + bias), out in T or fp32 (out_f32); x rows are read 16 bytes at a time
+// out [m, n] = act(x [m, k] W + bias), out in T or fp32 (out_f32); x rows are read 16 bytes at a time.
+// Two planes hold a value as two T, [2][m][width]: its rounding, and what that took away.
 struct W4LinearArgs {
   W4Layout l;
   int dtype;
@@ -215,6 +249,8 @@ struct W4LinearArgs {
   int act;
   void* out;
   bool out_f32;
+  int x_planes = 1, out_planes = 1;
+  bool exact = false;  // no weight is rounded, at any m
 };
 // How many clusters of ck CTAs (one CTA per SM) the device holds at a time: fewer than SMs / ck, as a
 // cluster stays within a GPC. `cache` is the caller's, one entry per device and log2(ck), zero at first.

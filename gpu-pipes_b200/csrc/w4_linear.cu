@@ -49,7 +49,7 @@ constexpr int kMaxCluster = 8;
 constexpr int64_t kRowsMax = 16;    // rows that go to this kernel
 constexpr int kMaxDepth = 8;        // ring stages
 constexpr int kMinDepth = 2;
-constexpr int kRowsSmem = kSmemLimit - 3072;  // dynamic: the barriers are static
+constexpr int kRowsSmem = kSmemLimit - 2048;  // dynamic: the barriers are static
 constexpr int kZeroBytes = 256;     // zeros in shared memory, read in place of absent x rows
 
 struct W4RowsArgs {
@@ -60,6 +60,7 @@ struct W4RowsArgs {
   void* out;
   int64_t m;
   int out_f32;
+  int out_planes;
   int act;
   int ck;            // CTAs of a cluster, along K
   int slice;         // k-blocks of a CTA
@@ -119,8 +120,8 @@ __device__ __forceinline__ void st_async_f32x4(uint32_t addr, uint32_t bar, floa
 }
 
 // TT: tiles of 8 x rows. UNITS: groups per k-block of 128. RUN: k-blocks of a ring slot, neighbours in the
-// packed codes.
-template <typename T, int TT, int UNITS, bool ZP, int RUN>
+// packed codes. PLANES: x rows as one T or as two (in a chain), with a product each on the same codes.
+template <typename T, int TT, int UNITS, bool ZP, int RUN, int PLANES>
 __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_constant__ W4RowsArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);                // scale words of a lane per block
   constexpr int kPart = TT * 8 * kPartStride;                 // floats of a warp's sums
@@ -229,14 +230,27 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       const int r = i / pieces, c = i % pieces;
       const int k = b0 * kW4Block + c * 8;
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows && k < a.l.k) v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (row0 + r) * a.l.k + k);
+      const T* from = static_cast<const T*>(a.x) + (row0 + r) * a.l.k + k;
+      if (r < rows && k < a.l.k) v = *reinterpret_cast<const uint4*>(from);
       if (r < rows) {  // rows 16 j + 4 t + i of a 32-row half where lane t reads them as 16 bytes, j by j
         uint8_t* to = xs + r * a.x_stride + (c >> 2) * 64 + (c & 1) * 32 + ((c >> 1) & 1) * 8;
         *reinterpret_cast<uint2*>(to) = make_uint2(v.x, v.y);
         *reinterpret_cast<uint2*>(to + 16) = make_uint2(v.z, v.w);
       }
+      float sum2 = 0.0f;
+      if constexpr (PLANES == 2) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < rows && k < a.l.k) u = *reinterpret_cast<const uint4*>(from + a.m * a.l.k);
+        if (r < rows) {
+          uint8_t* to = xs + (rows + r) * a.x_stride + (c >> 2) * 64 + (c & 1) * 32 + ((c >> 1) & 1) * 8;
+          *reinterpret_cast<uint2*>(to) = make_uint2(u.x, u.y);
+          *reinterpret_cast<uint2*>(to + 16) = make_uint2(u.z, u.w);
+        }
+        const float2 e0 = Elem<T>::unpack(u.x), e1 = Elem<T>::unpack(u.y), e2 = Elem<T>::unpack(u.z), e3 = Elem<T>::unpack(u.w);
+        sum2 = ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+      }
       const float2 f0 = Elem<T>::unpack(v.x), f1 = Elem<T>::unpack(v.y), f2 = Elem<T>::unpack(v.z), f3 = Elem<T>::unpack(v.w);
-      float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+      float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y)) + sum2;
 #pragma unroll
       for (int o = 1; o < 16 / UNITS; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (r < rows && c % (16 / UNITS) == 0) xsum[(c / (16 / UNITS)) * (8 * TT) + r] = sum;
@@ -274,10 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
         float v[4] = {u.x, u.y, u.z, u.w};
         const int live = a.l.n - n < 4 ? static_cast<int>(a.l.n - n) : 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i)
           if (a.bias != nullptr && i < live) v[i] += Elem<T>::to_f(static_cast<const T*>(a.bias)[n + i]);
-          v[i] = w4_act(a.act, v[i]);
-        }
+        w4_act(a.act, v);
         const int64_t at = (row0 + row_of(q)) * a.l.n + n;
         if (a.out_f32) {
           float* to = static_cast<float*>(a.out) + at;
@@ -290,13 +303,22 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
           }
         } else {
           uint16_t* to = static_cast<uint16_t*>(a.out) + at;
-          const uint32_t lo = Elem<T>::pack(v[0], v[1]), hi = Elem<T>::pack(v[2], v[3]);
-          if (vec) {
-            *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
-          } else {
+          auto put = [&](uint32_t lo, uint32_t hi) {
+            if (vec) {
+              *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (i < live) to[i] = static_cast<uint16_t>((i < 2 ? lo : hi) >> (16 * (i & 1)));
+              for (int i = 0; i < 4; ++i)
+                if (i < live) to[i] = static_cast<uint16_t>((i < 2 ? lo : hi) >> (16 * (i & 1)));
+            }
+          };
+          put(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]));
+          if (a.out_planes == 2) {
+            uint16_t first, rest[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w4_two<T>(v[i], first, rest[i]);
+            to += a.m * a.l.n;
+            put(rest[0] | static_cast<uint32_t>(rest[1]) << 16, rest[2] | static_cast<uint32_t>(rest[3]) << 16);
           }
         }
       };
@@ -329,12 +351,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
     }
   } else {
     // ---- codes to sums. Addresses run along: this loop is bound by its integer instructions.
-    uint32_t xa0[TT], xstep[TT];
+    uint32_t xa0[TT], xstep[TT], xsecond[TT];  // xsecond: bytes to the second plane
 #pragma unroll
     for (int i = 0; i < TT; ++i) {  // absent rows read the zeros again and again
       const bool live = i * 8 + g < rows;
       xa0[i] = smem_u32(live ? xs + (i * 8 + g) * a.x_stride + lead * (kW4Block * 2) : zeros) + t * 16;
       xstep[i] = live ? kW4Block * 2 : 0;
+      xsecond[i] = live ? rows * a.x_stride : 0;
     }
     const uint32_t xsum0 = smem_u32(xsum) + (lead * UNITS * 8 * TT + 2 * t) * 4;
     constexpr int kXsumBlock = UNITS * 8 * TT * 4;
@@ -376,6 +399,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
             const uint4 xv = lds128(xa[i] + h * 64);
             mma16816<T>(sum[i], p0, xv.x, xv.y);
             mma16816<T>(sum[i], p1, xv.z, xv.w);
+            if constexpr (PLANES == 2) {
+              const uint4 xl = lds128(xa[i] + xsecond[i] + h * 64);
+              mma16816<T>(sum[i], p0, xl.x, xl.y);
+              mma16816<T>(sum[i], p1, xl.z, xl.w);
+            }
           }
         }
         const float2 sc = Elem<T>::unpack(sbuf[ZP ? 2 * u : u]);
@@ -449,16 +477,17 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
 int rows_x_stride(int slice) { return slice * (kW4Block * 2) + 64; }  // conflict-free: 64 past a multiple of 128
 
 // Shared memory of a CTA: rings, warps' sums, clusters' sums, group sums of x, zeros, x rows
+// (`rows` times its planes)
 int64_t rows_smem(const W4Layout& l, int tt, int ck, int ws, int slice, int rows, int slots) {
   const int64_t outs = static_cast<int64_t>(kWarps / ws) * tt * 128;
   return static_cast<int64_t>(kWarps) * slots * (kW4BlockBytes + l.scale_bytes()) + 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) + 32ll * slice * l.units * tt +
          kZeroBytes + static_cast<int64_t>(rows) * rows_x_stride(slice);
 }
 
-template <typename T, int TT, int UNITS, bool ZP, int RUN>
+template <typename T, int TT, int UNITS, bool ZP, int RUN, int PLANES>
 int rows_launch(const W4RowsArgs& a, int smem, int clusters, int64_t row_tiles, cudaStream_t s, const PdlIo& io) {
   static unsigned long long done_mask = 0;
-  auto kern = &w4_rows_kernel<T, TT, UNITS, ZP, RUN>;
+  auto kern = &w4_rows_kernel<T, TT, UNITS, ZP, RUN, PLANES>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kRowsSmem, &done_mask);
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -490,28 +519,29 @@ int rows_launch(const W4RowsArgs& a, int smem, int clusters, int64_t row_tiles, 
 }
 
 template <typename T, int TT, int UNITS, bool ZP>
-int rows_run(const W4RowsArgs& a, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  return run == 4 ? rows_launch<T, TT, UNITS, ZP, 4>(a, smem, clusters, rt, s, io)
-                  : rows_launch<T, TT, UNITS, ZP, 2>(a, smem, clusters, rt, s, io);
+int rows_run(const W4RowsArgs& a, int run, int planes, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  if (planes == 2) return rows_launch<T, TT, UNITS, ZP, 2, 2>(a, smem, clusters, rt, s, io);
+  return run == 4 ? rows_launch<T, TT, UNITS, ZP, 4, 1>(a, smem, clusters, rt, s, io)
+                  : rows_launch<T, TT, UNITS, ZP, 2, 1>(a, smem, clusters, rt, s, io);
 }
 
 template <typename T, int TT, int UNITS>
-int rows_zeros(const W4RowsArgs& a, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  return a.l.zeros ? rows_run<T, TT, UNITS, true>(a, run, smem, clusters, rt, s, io)
-                   : rows_run<T, TT, UNITS, false>(a, run, smem, clusters, rt, s, io);
+int rows_zeros(const W4RowsArgs& a, int run, int planes, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return a.l.zeros ? rows_run<T, TT, UNITS, true>(a, run, planes, smem, clusters, rt, s, io)
+                   : rows_run<T, TT, UNITS, false>(a, run, planes, smem, clusters, rt, s, io);
 }
 
 template <typename T, int TT>
-int rows_units(const W4RowsArgs& a, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  return a.l.units == 1   ? rows_zeros<T, TT, 1>(a, run, smem, clusters, rt, s, io)
-         : a.l.units == 2 ? rows_zeros<T, TT, 2>(a, run, smem, clusters, rt, s, io)
-                          : rows_zeros<T, TT, 4>(a, run, smem, clusters, rt, s, io);
+int rows_units(const W4RowsArgs& a, int run, int planes, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return a.l.units == 1   ? rows_zeros<T, TT, 1>(a, run, planes, smem, clusters, rt, s, io)
+         : a.l.units == 2 ? rows_zeros<T, TT, 2>(a, run, planes, smem, clusters, rt, s, io)
+                          : rows_zeros<T, TT, 4>(a, run, planes, smem, clusters, rt, s, io);
 }
 
 template <typename T>
-int rows_tt(const W4RowsArgs& a, int tt, int run, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
-  return tt == 1 ? rows_units<T, 1>(a, run, smem, clusters, rt, s, io)
-                 : rows_units<T, 2>(a, run, smem, clusters, rt, s, io);
+int rows_tt(const W4RowsArgs& a, int tt, int run, int planes, int smem, int clusters, int64_t rt, cudaStream_t s, const PdlIo& io) {
+  return tt == 1 ? rows_units<T, 1>(a, run, planes, smem, clusters, rt, s, io)
+                 : rows_units<T, 2>(a, run, planes, smem, clusters, rt, s, io);
 }
 
 }  // namespace
@@ -549,7 +579,7 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   // the number of CTAs that run at a time, from one instance at its full shared memory
   static std::atomic<int> cluster_cache[64][4];
   static unsigned long long probe_mask = 0;
-  auto probe = &w4_rows_kernel<__half, 1, 1, false, 2>;
+  auto probe = &w4_rows_kernel<__half, 1, 1, false, 2, 1>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(probe), kRowsSmem, &probe_mask);
   if (rc != GP_OK) return rc;
   auto resident = [&](int ck) {
@@ -563,6 +593,8 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   a.packed = in.packed;
   a.bias = in.bias;
   a.out_f32 = in.out_f32;
+  a.out_planes = in.out_planes;
+  const int planes = in.x_planes;
   a.act = in.act;
   // Split of the work. A pass takes up to 16 rows (8 and fewer for the kernel of one row tile), fewer
   // where they would not fit in shared memory even spread over eight CTAs. Of the splits into ck CTAs
@@ -582,9 +614,9 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
         if (ws > 1 && ws / 2 >= slice) continue;  // warps without a block
         if (slice > 4 * ws && ws < kWarps) break;
         const int per_warp = (slice + ws - 1) / ws;
-        int r = per_warp > 2 ? 4 : 2;
-        if (rows_smem(l, tt, ck, ws, slice, rows, 4 * 3) > kRowsSmem) r = 2;
-        if (rows_smem(l, tt, ck, ws, slice, rows, r * kMinDepth) > kRowsSmem) continue;
+        int r = per_warp > 2 && planes == 1 ? 4 : 2;
+        if (rows_smem(l, tt, ck, ws, slice, rows * planes, 4 * 3) > kRowsSmem) r = 2;
+        if (rows_smem(l, tt, ck, ws, slice, rows * planes, r * kMinDepth) > kRowsSmem) continue;
         const int groups = (l.n_tiles + kWarps / ws - 1) / (kWarps / ws);
         const int n = groups < at_once ? groups : at_once;
         const int64_t iters = (groups + n - 1) / n;
@@ -609,13 +641,13 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   a.out = in.out;
   a.x_stride = rows_x_stride(a.slice);
   a.depth = kMaxDepth;
-  while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth) > kRowsSmem) --a.depth;
-  const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows, run * a.depth));
+  while (rows_smem(l, tt, a.ck, a.ws, a.slice, rows * planes, run * a.depth) > kRowsSmem) --a.depth;
+  const int smem = static_cast<int>(rows_smem(l, tt, a.ck, a.ws, a.slice, rows * planes, run * a.depth));
   PdlIo io;
-  io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(m) * l.n * (in.out_f32 ? 4 : 2));
+  io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(m) * l.n * (in.out_f32 ? 4 : 2 * in.out_planes));
   const int64_t passes = (m + per_pass - 1) / per_pass;
-  rc = in.dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(a, tt, run, smem, clusters, passes, s, io)
-                           : rows_tt<__half>(a, tt, run, smem, clusters, passes, s, io);
+  rc = in.dtype == GP_BF16 ? rows_tt<__nv_bfloat16>(a, tt, run, planes, smem, clusters, passes, s, io)
+                           : rows_tt<__half>(a, tt, run, planes, smem, clusters, passes, s, io);
   if (rc == GP_OK) count_launches(1);
   return rc;
 }

@@ -10,7 +10,11 @@
 //
 // Rounding: here a weight s (q - z) is rounded to T (q - z is exact, one multiplication), as
 // w4_dequantize gives it; the sums are fp32. Scaling the sums instead, group by group, as the row
-// kernel does, would read the accumulator once per group: more time than the tile's product.
+// kernel does, would read the accumulator once per group: more time than the tile's product. In a
+// chain (EXACT), whose layers' errors add up, the operand is two T per weight instead, the rounded one
+// and what rounding took away, with a product each: the weight is then exact. Likewise x may be two T
+// (planes): its second part meets the first part of the weights (second by second is at most 2^-16 of
+// a bf16 product, a 256th of what the output's rounding takes; 2^-22 for fp16).
 //
 // The unit is a k-block of 128 rows of W:
 //   loader (1 thread)   x panels (two of 64 columns) by TMA into a ring of stages
@@ -43,7 +47,7 @@ constexpr int kTileTiles = kTileN / 16;
 constexpr int kACols = 64;
 constexpr int kTmemCols = 512;            // 256 for the sums, 256 for the weights
 constexpr int kMaxStages = 4;       // x stages
-constexpr int kMaxTileRows = 256;
+constexpr int kMaxTileRows = 256;   // 128 where weights are two T: those take as much TMEM again
 
 struct W4TileArgs {
   W4Layout l;
@@ -57,9 +61,12 @@ struct W4TileArgs {
   int row_tiles;
   int ck;          // CTAs of a cluster, along K
   int slice;       // k-blocks of a CTA
+  int planes;      // of x
+  int out_planes;
   int stages;      // x stages
   int depth;       // slots of a warp's code ring (2 or 3)
   int groups;
+  int exact;
   int* status;
   unsigned long long timeout_ns;
   int inject;
@@ -73,8 +80,12 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 
-// a warp's slot: for its two column tiles, 32 bytes of codes and the scales of each lane
-constexpr int code_slot(int units, bool zp) { return 2 * 32 * (32 + 4 * units * (zp ? 2 : 1)); }
+// Words of scales that a lane needs per turn (a block, or with two T per weight a 64-row part of it), and a
+// warp's slot: for its two column tiles, a turn's codes and scales of each lane
+constexpr int turn_words(int units, bool zp, bool exact) { return (exact && units > 1 ? units / 2 : units) * (zp ? 2 : 1); }
+constexpr int code_slot(int units, bool zp, bool exact) {
+  return 2 * 32 * ((exact ? 16 : 32) + 4 * turn_words(units, zp, exact));
+}
 
 // One lane of the (converged) warp, always the same one.
 __device__ __forceinline__ bool elect_one() {
@@ -102,17 +113,20 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
 // TMEM lane of a tile <-> column: lane 16 i + r holds column 16 i + 2 (r % 8) + r / 8
 __device__ __forceinline__ int tile_column(int lane) { return (lane & ~15) + 2 * (lane & 7) + ((lane >> 3) & 1); }
 
-template <typename T, int UNITS, bool ZP, int GROUPS>
+template <typename T, int UNITS, bool ZP, int GROUPS, bool EXACT>
 __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
     w4_tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ W4TileArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);
   constexpr int kScaleBytes = 32 * kWords;            // of a block of 16 columns
-  constexpr int kSlot = code_slot(UNITS, ZP);
+  constexpr int kUse = turn_words(UNITS, ZP, EXACT);
+  constexpr int kSlot = code_slot(UNITS, ZP, EXACT);
+  constexpr int kTurns = EXACT ? 2 : 1;               // turns per block: the groups then take 64-row parts in turn
+  static_assert(!EXACT || GROUPS == 4, "a group keeps to one part of its blocks");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], a_full[GROUPS], a_empty[GROUPS], d_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
-  const int panel = a.rows * 128, stage_bytes = 2 * panel;  // x rows of 64 columns, SWIZZLE_128B
+  const int panel = a.rows * 128, stage_bytes = 2 * panel * a.planes;  // x rows of 64 columns, SWIZZLE_128B
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = a.ck > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit = blockIdx.x / a.ck;
@@ -124,7 +138,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   // With as many x stages as TMEM stages, a block's x panels and weights share one barrier for "full" and
   // one for "free": one wait and one commit less per turn of the MMA issuer, whose turns bound the kernel
   // at few rows.
-  const bool merged = a.stages == GROUPS;
+  const bool merged = !EXACT && a.stages == GROUPS;
   const uint32_t full0 = smem_u32(merged ? a_full : full), empty0 = smem_u32(merged ? a_empty : empty);
 
   if ((smem_u32(smem) & 1023u) != 0) {  // the same in every CTA of the grid
@@ -177,9 +191,9 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
           break;
         }
         mbar_arrive_expect_tx(full0 + s * 8, stage_bytes);
-        for (int p = 0; p < 2; ++p)
+        for (int p = 0; p < 2 * a.planes; ++p)  // rows past m of the first plane are not stored
           tma_load_2d_hint(smem_u32(smem) + s * stage_bytes + p * panel, &tx, full0 + s * 8,
-                           (b0 + b) * kW4Block + p * 64, static_cast<int>(row0), keep);
+                           (b0 + b) * kW4Block + (p & 1) * 64, static_cast<int>(row0 + (p >> 1) * a.m), keep);
         if (++s == a.stages) s = 0, ph ^= 1;
       }
       if (!ok)  // copies under way end (waited for with a limit) before their memory is used again or goes away
@@ -200,24 +214,39 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
     const uint64_t desc0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
     const uint32_t a_full0 = smem_u32(a_full), a_empty0 = smem_u32(a_empty);
     int s = 0, ph = 0, as = 0, aph = 0;
-    for (int b = 0; b < nb; ++b) {
+    for (int turn = 0; turn < kTurns * nb; ++turn) {
+      const int part = EXACT ? turn & 1 : 0;
       ok = mbar_wait(a_full0 + as * 8, aph, wctx, kDevTimeoutMma) &&
-           (merged || mbar_wait(full0 + s * 8, ph, wctx, kDevTimeoutMma));
+           (merged || part != 0 || mbar_wait(full0 + s * 8, ph, wctx, kDevTimeoutMma));
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint64_t bdesc = desc0 + static_cast<uint64_t>(s * (stage_bytes >> 4));
+      const uint64_t bdesc = desc0 + static_cast<uint64_t>((s * stage_bytes + part * panel) >> 4);
       if (elect_one()) {
+        const uint32_t stage = at0 + as * kACols;
+        auto more = [&](int k) { return (turn != 0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u; };
+        if constexpr (EXACT) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mma_ts(d + (k & 1) * second, at0 + as * kACols + k * 8,
-                 bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2), idesc,
-                 (b != 0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k)
+            mma_ts(d + (k & 1) * second, stage + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, more(k));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_ts(d + (k & 1) * second, stage + 32 + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, 1u);
+          if (a.planes == 2)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ts(d + (k & 1) * second, stage + k * 8, bdesc + static_cast<uint64_t>((panel >> 3) + k * 2), idesc, 1u);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_ts(d + (k & 1) * second, stage + k * 8,
+                   bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2), idesc, more(k));
+        }
         mma_commit(a_empty0 + as * 8);
-        if (!merged) mma_commit(empty0 + s * 8);
+        if (!merged && part == kTurns - 1) mma_commit(empty0 + s * 8);
       }
       __syncwarp();
       if (++as == GROUPS) as = 0, aph ^= 1;
-      if (++s == a.stages) s = 0, ph ^= 1;
+      if (part == kTurns - 1 && ++s == a.stages) s = 0, ph ^= 1;
     }
     // every product issued has completed before TMEM is read or released
     if (elect_one()) mma_commit(smem_u32(&d_full));
@@ -233,35 +262,39 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
     // this warp's two column tiles of the tile's eight; an absent one stays zero
     const bool have[2] = {2 * q < tiles, 2 * q + 1 < tiles};
     const uint8_t *codes[2], *scales[2];
+    const int my_part = EXACT ? group & 1 : 0, first = EXACT ? group >> 1 : group;
+    constexpr int kStep = GROUPS / kTurns;  // blocks from a turn of this group to its next
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t cell = static_cast<int64_t>(tile0 + 2 * q + i) * a.l.blocks + b0 + group;
-      codes[i] = static_cast<const uint8_t*>(a.packed) + cell * kW4BlockBytes + lane * 16;
-      scales[i] = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + cell * kScaleBytes + g * (4 * kWords);
+      const int64_t cell = static_cast<int64_t>(tile0 + 2 * q + i) * a.l.blocks + b0 + first;
+      codes[i] = static_cast<const uint8_t*>(a.packed) + cell * kW4BlockBytes + my_part * (kW4BlockBytes / 2) + lane * 16;
+      scales[i] = static_cast<const uint8_t*>(a.packed) + a.l.scale_off + cell * kScaleBytes + g * (4 * kWords) +
+                  (kUse < kWords ? my_part * (4 * kUse) : 0);
     }
-    const uint32_t my_codes = ring + lane * 16, my_scales = ring + 2048 + lane * (4 * kWords);
+    constexpr int kTurnCodes = kW4BlockBytes / kTurns;  // of a column tile
+    const uint32_t my_codes = ring + lane * 16, my_scales = ring + 2 * kTurnCodes + lane * (4 * kUse);
     const uint32_t ring_end = a.depth * kSlot;
-    int ld_b = group;
+    int ld_b = first;
     uint32_t ld_at = 0;  // byte offset of the slot that is filled next
     auto load = [&] {
       if (ld_b < nb) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (have[i]) {
-            cp_async<16>(my_codes + ld_at + i * 1024, codes[i]);
-            cp_async<16>(my_codes + ld_at + i * 1024 + 512, codes[i] + kW4BlockBytes / 2);
-            if constexpr (kWords == 8) {
-              cp_async<16>(my_scales + ld_at + i * (128 * kWords), scales[i]);
-              cp_async<16>(my_scales + ld_at + i * (128 * kWords) + 16, scales[i] + 16);
+            cp_async<16>(my_codes + ld_at + i * kTurnCodes, codes[i]);
+            if constexpr (!EXACT) cp_async<16>(my_codes + ld_at + i * kTurnCodes + 512, codes[i] + kW4BlockBytes / 2);
+            if constexpr (kUse == 8) {
+              cp_async<16>(my_scales + ld_at + i * (128 * kUse), scales[i]);
+              cp_async<16>(my_scales + ld_at + i * (128 * kUse) + 16, scales[i] + 16);
             } else {
-              cp_async<4 * kWords>(my_scales + ld_at + i * (128 * kWords), scales[i]);
+              cp_async<4 * kUse>(my_scales + ld_at + i * (128 * kUse), scales[i]);
             }
           }
-          codes[i] += GROUPS * kW4BlockBytes;
-          scales[i] += GROUPS * kScaleBytes;
+          codes[i] += kStep * kW4BlockBytes;
+          scales[i] += kStep * kScaleBytes;
         }
       }
-      ld_b += GROUPS;
+      ld_b += kStep;
       ld_at = ld_at + kSlot == ring_end ? 0 : ld_at + kSlot;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -269,42 +302,57 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
     uint32_t at = 0;
     const uint32_t a_stage = a_tmem + group * kACols + lanes;
     int parity = 1;  // of the stage's last use
-    for (int b = group; b < nb; b += GROUPS, parity ^= 1) {
+    // codes and scales of a column tile's 64 rows to T: r, and with two T per weight rest
+    auto convert = [&](int i, int part, uint32_t* r, uint32_t* rest) {
+      uint32_t c[4] = {0, 0, 0, 0}, sw[kUse];
+#pragma unroll
+      for (int w = 0; w < kUse; ++w) sw[w] = 0;
+      if (have[i]) {
+        w4_lds<4>(my_codes + at + i * kTurnCodes + part * 512, c);
+        w4_lds<kUse>(my_scales + at + i * (128 * kUse), sw);
+      }
+      W4Exact<T> dq;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        constexpr int kPer = ZP ? 2 : 1;
+        const int u = (UNITS == 1 ? 0 : UNITS == 2 ? part : 2 * part + h) * kPer;
+        if (UNITS == 4 || h == 0) dq.set(sw[u], sw[u + kPer - 1], ZP);
+        dq.word(c[2 * h], r + 8 * h, rest == nullptr ? nullptr : rest + 8 * h);
+        dq.word(c[2 * h + 1], r + 8 * h + 4, rest == nullptr ? nullptr : rest + 8 * h + 4);
+      }
+    };
+    // the TMEM stage is free: its last products have completed
+    auto stage_free = [&](bool never_used) {
+      ok = never_used || mbar_wait(smem_u32(&a_empty[group]), parity, wctx, kDevTimeoutEpilogue);
+      ok = __all_sync(0xffffffffu, ok) != 0;
+      if (ok) tc_fence_after();
+      return ok;
+    };
+    for (int b = first; b < nb; b += kStep, parity ^= 1) {
       load();
       if (a.depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
       else asm volatile("cp.async.wait_group 1;" ::: "memory");
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        // 64 rows to T in registers; the TMEM stage is only then waited for
-        uint32_t r[2][16];
+      // in registers first; the stage is only then waited for
+      if constexpr (EXACT) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t c[4] = {0, 0, 0, 0}, sw[kWords];
-#pragma unroll
-          for (int w = 0; w < kWords; ++w) sw[w] = 0;
-          if (have[i]) {
-            w4_lds<4>(my_codes + at + i * 1024 + part * 512, c);
-            w4_lds<kWords>(my_scales + at + i * (128 * kWords), sw);
-          }
-          W4Exact<T> dq;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            constexpr int kStep = ZP ? 2 : 1;
-            const int u = (UNITS == 1 ? 0 : UNITS == 2 ? part : 2 * part + h) * kStep;
-            if (UNITS == 4 || h == 0) dq.set(sw[u], sw[u + kStep - 1], ZP);
-            dq.word(c[2 * h], r[i] + 8 * h);
-            dq.word(c[2 * h + 1], r[i] + 8 * h + 4);
-          }
+          uint32_t r[16], rest[16];
+          convert(i, 0, r, rest);
+          if (i == 0 && !stage_free(b == first)) break;
+          tmem_st_16x256b_x4(a_stage + (static_cast<uint32_t>(i * 16) << 16), r);
+          tmem_st_16x256b_x4(a_stage + 32 + (static_cast<uint32_t>(i * 16) << 16), rest);
         }
-        if (part == 0) {
-          ok = b == group || mbar_wait(smem_u32(&a_empty[group]), parity, wctx, kDevTimeoutEpilogue);
-          ok = __all_sync(0xffffffffu, ok) != 0;
-          if (!ok) break;
-          tc_fence_after();
-        }
+      } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          tmem_st_16x256b_x4(a_stage + part * 32 + (static_cast<uint32_t>(i * 16) << 16), r[i]);
+        for (int part = 0; part < 2; ++part) {
+          uint32_t r[2][16];
+          convert(0, part, r[0], nullptr);
+          convert(1, part, r[1], nullptr);
+          if (part == 0 && !stage_free(b == first)) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            tmem_st_16x256b_x4(a_stage + part * 32 + (static_cast<uint32_t>(i * 16) << 16), r[i]);
+        }
       }
       if (!ok) break;
       at = at + kSlot == ring_end ? 0 : at + kSlot;
@@ -324,12 +372,28 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   const int q = warp & 3, quarter = (warp - 2) >> 2, n = tile0 * 16 + q * 32 + tile_column(lane);
   const bool has_n = warp >= 2 && n < a.l.n;
   const float bias = has_n && a.bias != nullptr ? Elem<T>::to_f(static_cast<const T*>(a.bias)[n]) : 0.0f;
-  auto store = [&](int64_t row, float v) {
-    v = w4_act(a.act, v + bias);
+  // rows row, row + 1, ... of column n: the first `live` of v
+  auto store = [&](int64_t row, auto& v, int live) {
+    constexpr int kN = sizeof(v) / sizeof(float);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] += bias;
+    w4_act(a.act, v);
+    const int64_t at = row * a.l.n + n;
     if (a.out_f32) {
-      static_cast<float*>(a.out)[row * a.l.n + n] = v;
+      float* to = static_cast<float*>(a.out) + at;
+#pragma unroll
+      for (int i = 0; i < kN; ++i, to += a.l.n)
+        if (i < live) *to = v[i];
     } else {
-      static_cast<uint16_t*>(a.out)[row * a.l.n + n] = static_cast<uint16_t>(Elem<T>::pack(v, 0.0f));
+      uint16_t* to = static_cast<uint16_t*>(a.out) + at;
+      const int64_t plane = a.m * a.l.n;
+#pragma unroll
+      for (int i = 0; i < kN; ++i, to += a.l.n) {
+        uint16_t hi, lo;
+        w4_two<T>(v[i], hi, lo);
+        if (i < live) *to = hi;
+        if (EXACT && i < live && a.out_planes == 2) to[plane] = lo;
+      }
     }
   };
   const uint32_t d_lanes = d_tmem + (static_cast<uint32_t>(q * 32) << 16);
@@ -347,10 +411,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
       for (int c0 = quarter * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * GROUPS) {
         float v[8];
         load_sums(c0, v);
-        const int live = has_n ? static_cast<int>(min(static_cast<int64_t>(8), a.m - row0 - c0)) : 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < live) store(row0 + c0 + i, v[i]);
+        store(row0 + c0, v, has_n ? static_cast<int>(min(static_cast<int64_t>(8), a.m - row0 - c0)) : 0);
       }
   } else {
     // CTA r of the cluster finishes rows [r share, (r + 1) share) of the tile: sums [source][row][128]
@@ -378,10 +439,10 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
 #pragma unroll 1
       for (int c = quarter; c < share; c += GROUPS) {
         const int64_t row = row0 + rank * share + c;
-        float v = 0.0f;
+        float v[1] = {0.0f};
         for (int i = 0; i < a.ck; ++i)
-          v += reinterpret_cast<const float*>(smem)[(i * share + c) * kTileN + q * 32 + lane];
-        if (has_n && row < a.m) store(row, v);
+          v[0] += reinterpret_cast<const float*>(smem)[(i * share + c) * kTileN + q * 32 + lane];
+        store(row, v, has_n && row < a.m ? 1 : 0);
       }
   }
   tc_fence_before();
@@ -392,10 +453,10 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   }
 }
 
-template <typename T, int UNITS, bool ZP, int GROUPS>
+template <typename T, int UNITS, bool ZP, int GROUPS, bool EXACT>
 int tile_launch(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int smem, cudaStream_t s, const PdlIo& io) {
   static unsigned long long done_mask = 0;
-  auto kern = &w4_tile_kernel<T, UNITS, ZP, GROUPS>;
+  auto kern = &w4_tile_kernel<T, UNITS, ZP, GROUPS, EXACT>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kSmemLimit - 2048, &done_mask);
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -428,9 +489,10 @@ int tile_launch(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int sm
 
 template <typename T, int UNITS, bool ZP>
 int tile_groups(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int smem, cudaStream_t s, const PdlIo& io) {
+  if (a.exact) return tile_launch<T, UNITS, ZP, 4, true>(a, tx, ctas, smem, s, io);
   if constexpr (UNITS == 4 && ZP)
-    if (a.groups == 2) return tile_launch<T, UNITS, ZP, 2>(a, tx, ctas, smem, s, io);
-  return tile_launch<T, UNITS, ZP, 4>(a, tx, ctas, smem, s, io);
+    if (a.groups == 2) return tile_launch<T, UNITS, ZP, 2, false>(a, tx, ctas, smem, s, io);
+  return tile_launch<T, UNITS, ZP, 4, false>(a, tx, ctas, smem, s, io);
 }
 
 template <typename T, int UNITS>
@@ -457,11 +519,15 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   a.m = in.m;
   a.out_f32 = in.out_f32;
   a.act = in.act;
+  a.planes = in.x_planes;
+  a.out_planes = in.out_planes;
+  a.exact = in.exact || in.x_planes == 2 || in.out_planes == 2;
   a.status = dev.status;
   a.timeout_ns = current_timeout_ns();
   a.inject = current_fault_injection();
-  // rows per tile: as even as multiples of 16 up to 256 allow
-  const int64_t row_tiles = (in.m + kMaxTileRows - 1) / kMaxTileRows;
+  // rows per tile: as even as multiples of 16 up to 256 (128) allow
+  const int64_t most = a.exact ? kMaxTileRows / 2 : kMaxTileRows;
+  const int64_t row_tiles = (in.m + most - 1) / most;
   a.rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
   a.row_tiles = static_cast<int>((in.m + a.rows - 1) / a.rows);
   const int64_t units = static_cast<int64_t>((a.l.n_tiles + kTileTiles - 1) / kTileTiles) * a.row_tiles;
@@ -470,7 +536,7 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   // CTA along K, 11.2 with two, 8.4 with four)
   static std::atomic<int> cluster_cache[64][4];
   static unsigned long long probe_mask = 0;
-  const void* probe = reinterpret_cast<const void*>(&w4_tile_kernel<__half, 1, false, 4>);
+  const void* probe = reinterpret_cast<const void*>(&w4_tile_kernel<__half, 1, false, 4, false>);
   int rc = ensure_smem_attr(probe, kSmemLimit - 2048, &probe_mask);
   if (rc != GP_OK) return rc;
   int64_t best = -1;
@@ -478,16 +544,16 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
     const int slice = (a.l.blocks + ck - 1) / ck;
     if (ck > 1 && ((ck - 1) * slice >= a.l.blocks || a.rows % ck != 0)) break;
     const int at_once = w4_max_clusters(probe, tile_threads(4), kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
-    const int64_t cost = (units + at_once - 1) / at_once * (4 * slice + (ck > 1 ? 48 : 30));
+    const int64_t cost = (units + at_once - 1) / at_once * ((a.exact ? 6 : 4) * slice + (ck > 1 ? 48 : 30));
     if (best >= 0 && cost >= best) continue;
     best = cost;
     a.ck = ck;
     a.slice = slice;
   }
   if (units * a.ck >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "w4 linear: m = %lld", (long long)in.m);
-  const int stage = 2 * a.rows * 128;
+  const int stage = 2 * a.rows * 128 * a.planes;
   a.groups = a.rows > 128 && a.l.units == 4 && a.l.zeros != 0 ? 2 : 4;
-  const int slot = 4 * a.groups * code_slot(a.l.units, a.l.zeros != 0);
+  const int slot = 4 * a.groups * code_slot(a.l.units, a.l.zeros != 0, a.exact != 0);
   // as many x stages as groups where that fits; then code slots, three if possible
   const int budget = kSmemLimit - 2048;
   a.depth = a.groups * stage + 3 * slot <= budget ? 3 : 2;
@@ -498,11 +564,11 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   const int sums = a.ck > 1 ? a.rows * kTileN * 4 : 0;
   if (smem < sums) smem = sums;
   CUtensorMap tx;
-  rc = make_tmap_2d(&tx, in.x, in.dtype, static_cast<uint64_t>(in.m), static_cast<uint64_t>(a.l.k), 64,
+  rc = make_tmap_2d(&tx, in.x, in.dtype, static_cast<uint64_t>(in.m) * a.planes, static_cast<uint64_t>(a.l.k), 64,
                         static_cast<uint32_t>(a.rows), 128);
   if (rc != GP_OK) return rc;
   PdlIo io;
-  io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(in.m) * a.l.n * (in.out_f32 ? 4 : 2));
+  io.add(PdlIo::kWrite, in.out, static_cast<uint64_t>(in.m) * a.l.n * (in.out_f32 ? 4 : 2 * a.out_planes));
   rc = in.dtype == GP_BF16 ? tile_units<__nv_bfloat16>(a, tx, units * a.ck, smem, s, io)
                            : tile_units<__half>(a, tx, units * a.ck, smem, s, io);
   if (rc == GP_OK) count_launches(1);

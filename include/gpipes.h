@@ -257,10 +257,11 @@ GP_API int gp_fused_mlp_host(const gp_mlp_spec* spec, int64_t m, const void* x_h
  * Norms around a block, and layers with 4-bit weights, for serving transformer blocks next to the
  * chains above. No reference counterpart.
  *   Shared rules: every buffer is contiguous; sums, statistics and activations are fp32 and each
- *   output is rounded once; nothing is allocated and no library workspace is used, so a call may be
- *   captured into a CUDA graph without an eager call before it, and calls on different streams or
- *   replays of different graphs may overlap as long as their own buffers do not. Inputs and outputs
- *   that overlap without being named as allowed return GP_ERR_ARG.
+ *   output is rounded once; no library workspace is used, so calls on different streams or replays of
+ *   different graphs may overlap as long as their own buffers do not. Every call may be captured into a
+ *   CUDA graph. The norms and the calls that quantise, pack and read back allocate nothing; the first
+ *   product on a device allocates the status word if no chain has, so make one before a capture.
+ *   Inputs and outputs that overlap without being named as allowed return GP_ERR_ARG.
  * ------------------------------------------------------------------------------------------- */
 typedef enum gp_norm {
   GP_NORM_NONE = 0,
@@ -327,14 +328,16 @@ GP_API int gp_w4_dequantize_out(const gp_w4_spec* spec, const void* packed, void
 /* out [m, N] = act(x [m, K] W + bias) on packed weights, T; bias [N] or NULL; act a gp_act. From single
  * tokens to prompts: up to 16 rows the sums over each group are scaled in fp32 and no weight is rounded;
  * from 17 rows on each weight s (q - z) is rounded to T first, as gp_w4_dequantize_out gives it. A row of x
- * with an infinity may give NaN where the sum is infinite. x 16-byte, out and bias 2-byte aligned. */
+ * with an infinity (or, in bf16, with values whose sum over a group is one in fp32) may give NaN where the
+ * sum is infinite (or very large). x 16-byte, out and bias 2-byte aligned. */
 GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, const void* packed,
                             const void* bias, void* out, void* stream);
 
 /* A chain of layers (gp_mlp_spec) on packed weights: widths of any multiple of 8 (the last one any
  * N without a tail), every activation and tail, no skip layer. Layer l is packed[l], a gp_w4_spec of
- * widths[l] x widths[l + 1], the group and zero_points given here and the spec's dtype. Hidden
- * activations are rounded to T; the last layer goes into a LayerNorm tail in fp32. workspace: caller's,
+ * widths[l] x widths[l + 1], the group and zero_points given here and the spec's dtype. In a chain no weight
+ * is rounded, at any m. The hidden activations of two layers are rounded to T; in longer chains they are
+ * kept as two T (m below 2^30). The last layer goes into a LayerNorm tail in fp32. workspace: caller's,
  * 16-byte aligned, at least gp_w4_mlp_workspace_bytes(spec, m) long (0 bytes: NULL is fine), free for
  * other use once the call's work has run. gamma and beta 16-byte aligned. */
 GP_API int gp_w4_mlp_out(const gp_mlp_spec* spec, int group, int zero_points, int64_t m, const void* x,

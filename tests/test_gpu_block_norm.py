@@ -4,6 +4,10 @@ Bounds: all arithmetic is fp32 on a row of H values. A sum of H values taken as 
 thread, then 5 + 32 partial sums, is off by at most about 80 half steps of the sum of magnitudes; with
 the few operations per element after it, C = 128 half steps bound each statistic and each element's
 arithmetic, relative to the magnitudes that go into it. Stored values add one rounding."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -196,3 +200,28 @@ def test_binding_refusals_on_device(cuda_dev):
         cuda_ext.block_norm(flat[4:].view(6, 64), pre=RMS)
     with pytest.raises(L.GpError, match="multiple of 8"):
         cuda_ext.block_norm(torch.zeros(6, 60, dtype=torch.float16, device=cuda_dev), pre=RMS)
+
+
+def test_first_call_of_a_process_may_be_captured(cuda_dev):
+    # the norms and the conversions of weights allocate nothing, not even on their first call
+    code = """if True:
+        import torch
+        import __graft_entry__ as e
+        e.load_package()
+        from gpu_pipes_b200 import _lib as L, cuda_ext
+        x = torch.randn(5, 256, device="cuda").half()
+        w = torch.randn(256, 64, device="cuda").half()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            _, h = cuda_ext.block_norm(x, pre=L.NORM_RMS)
+            d = cuda_ext.w4_dequantize(cuda_ext.w4_quantize(w))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(h, cuda_ext.block_norm(x, pre=L.NORM_RMS)[1])
+        assert torch.equal(d, cuda_ext.w4_dequantize(cuda_ext.w4_quantize(w)))
+        print("captured")
+    """
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]

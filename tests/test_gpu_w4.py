@@ -351,6 +351,34 @@ def test_mlp(cuda_dev, widths, acts, tail, m):
             assert torch.equal(y, got)
 
 
+@pytest.mark.parametrize("widths", [(128, 512, 128), (256, 136, 72, 264), (72, 80, 88, 96, 40)])
+@pytest.mark.parametrize("m", [9, 37, 130])
+def test_roundings_of_a_chain(cuda_dev, widths, m):
+    """What a chain's result is off by, as a root mean square, against the rounding of the exact result.
+    No weight is rounded and longer chains keep their hidden activations as two T: what is left is the
+    final rounding. Two layers round the hidden activations once: independent relative errors of the
+    terms of a sum are at most as much of the sum, so sqrt(2) of the final rounding in all. Both with a
+    tenth for the sample (360 values or more: the root mean square of as many roundings varies by 2.4%),
+    and fp32's sums and the products of second parts on top, within their bounds."""
+    for dtype, group, zeros in ((torch.bfloat16, 128, False), (torch.float16, 32, True)):
+        layers = [make(k, n, dtype, group, zeros, i) for i, (k, n) in enumerate(zip(widths[:-1], widths[1:]))]
+        ws = [cuda_ext.w4_pack(*layer, group=group) for layer in layers]
+        x = rows(m, widths[0], dtype)
+        got = cuda_ext.w4_mlp(x, ws, [None] * len(ws), acts=[L.ACT_RELU] * (len(ws) - 1) + [L.ACT_NONE]).double()
+        v, err = x.double(), torch.zeros_like(x, dtype=torch.float64)
+        for i, (codes, scales, z) in enumerate(layers):
+            w = weights64(codes, scales, z, group)
+            mag = v.abs() @ w.abs()
+            # up to three products per term, and the parts left out
+            err = err @ w.abs() + (2 * U32 * (3 * w.shape[0] / 16 + 96) + 2 * half_step(dtype) ** 2) * mag
+            v = v @ w
+            if i + 1 < len(layers):
+                v = v.clamp(min=0)
+        rms = lambda t: t.square().mean().sqrt().item()  # noqa: E731
+        final = rms(v.to(dtype).double() - v)
+        assert rms(got - v) <= 1.1 * final * (2 ** 0.5 if len(layers) == 2 else 1.0) + rms(err), (widths, m, dtype)
+
+
 def test_bert_ffn_takes_packed_weights(cuda_dev):
     """The BERT-large block's entry point with 4-bit weights, against the same block on the 16-bit
     values that they stand for: the fused 16-bit chain has its own roundings (fp16 hidden

@@ -111,7 +111,7 @@ def test_mlp_workspace_bytes():
     assert _ws([64, 32], L.TAIL_NONE, 5) == 0
     assert _ws([64, 40], L.TAIL_LAYERNORM, 5) == 1024  # 5 x 40 fp32 = 800, in 256-byte pieces
     assert _ws([64, 200, 64], L.TAIL_NONE, 5) == 2048  # one hidden buffer: 2,000
-    assert _ws([64, 200, 80, 40, 64], L.TAIL_NONE, 5) == 2 * 2048  # two that alternate
+    assert _ws([64, 200, 80, 40, 64], L.TAIL_NONE, 5) == 2 * 4096  # two that alternate, of two T per value
     assert _ws([1024, 4096, 1024], L.TAIL_RESIDUAL_LN, 2**20) == 2**20 * (4096 * 2 + 1024 * 4)
     assert _ws([64, 200, 64], L.TAIL_NONE, -1) == L.GP_ERR_ARG
     assert _ws([64, 201, 64], L.TAIL_NONE, 1) == L.GP_ERR_SHAPE
