@@ -24,8 +24,11 @@
 //                       stores them to the group's TMEM stage of 64 columns. A turn's waits and
 //                       fences take as long as the conversion of 64 rows does, hence whole blocks.
 //   MMA issuer (1 thread) eight K = 16 products per block; commits free the TMEM stage and the x stage.
-//                       Up to 128 rows of x the products alternate between two accumulators: one
-//                       that waits for the sum of the last takes about 58 cycles at any such width.
+//                       Up to 128 rows of x the products alternate between two accumulators. With two T
+//                       per weight there are two issuers, as a turn then is half a block and an issuer's
+//                       wait is answered behind its own products (4,096 -> 14,336 -> 4,096 at 32 rows: 53 us
+//                       with one, 41 with two; single layers gain nothing): up to 128 rows they take the
+//                       turns alternately, each with an accumulator; above, each has half of the rows.
 //   epilogue            the dequantising warps: bias, activation, store
 // Where there are fewer tiles than SMs, a cluster of ck CTAs splits K and sums over distributed
 // shared memory in a fixed order.
@@ -38,16 +41,16 @@ namespace {
 
 // Groups of four dequantising warps, one warp per TMEM lane quarter: four, but two above 128 rows of x with
 // zero points in groups of 32. There the code rings of four groups leave no room for two x stages of 256
-// rows (512 x 4,096 x 14,336: 97 us in tiles of 128 rows, 74 with two groups), and the products of a
+// rows (512 x 4,096 x 14,336: 97 us in tiles of 128 rows, 76 with two groups), and the products of a
 // block take longer than its conversion anyway. Elsewhere four are no slower (62 us; two: 65).
-constexpr int tile_threads(int groups) { return 32 * (2 + 4 * groups); }
+constexpr int tile_threads(int groups, bool exact) { return 32 * ((exact ? 3 : 2) + 4 * groups); }
 constexpr int kTileN = 128;        // columns of W per tile: the TMEM lanes
 constexpr int kTileTiles = kTileN / 16;
 // a TMEM stage of dequantised weights per group: 64 columns, a block
 constexpr int kACols = 64;
 constexpr int kTmemCols = 512;            // 256 for the sums, 256 for the weights
 constexpr int kMaxStages = 4;       // x stages
-constexpr int kMaxTileRows = 256;   // 128 where weights are two T: those take as much TMEM again
+constexpr int kMaxTileRows = 256;
 
 struct W4TileArgs {
   W4Layout l;
@@ -114,7 +117,7 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
 __device__ __forceinline__ int tile_column(int lane) { return (lane & ~15) + 2 * (lane & 7) + ((lane >> 3) & 1); }
 
 template <typename T, int UNITS, bool ZP, int GROUPS, bool EXACT>
-__global__ void __launch_bounds__(tile_threads(GROUPS), 1)
+__global__ void __launch_bounds__(tile_threads(GROUPS, EXACT), 1)
     w4_tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ W4TileArgs a) {
   constexpr int kWords = UNITS * (ZP ? 2 : 1);
   constexpr int kScaleBytes = 32 * kWords;            // of a block of 16 columns
@@ -139,6 +142,8 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   // one for "free": one wait and one commit less per turn of the MMA issuer, whose turns bound the kernel
   // at few rows.
   const bool merged = !EXACT && a.stages == GROUPS;
+  const bool split = EXACT && a.rows > 128;  // the two issuers take half of the rows each; else every other turn
+  const uint32_t second = !EXACT && a.rows <= 128 ? a.rows : 0;  // one issuer: its second accumulator, if there is one
   const uint32_t full0 = smem_u32(merged ? a_full : full), empty0 = smem_u32(merged ? a_empty : empty);
 
   if ((smem_u32(smem) & 1023u) != 0) {  // the same in every CTA of the grid
@@ -149,13 +154,13 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&empty[i]), 1);
+      mbar_init(smem_u32(&empty[i]), EXACT ? 2 : 1);
     }
     for (int i = 0; i < GROUPS; ++i) {
       mbar_init(smem_u32(&a_full[i]), merged ? 5 : 4);  // the group's warps (and the x panels)
-      mbar_init(smem_u32(&a_empty[i]), 1);
+      mbar_init(smem_u32(&a_empty[i]), split ? 2 : 1);
     }
-    mbar_init(smem_u32(&d_full), 1);
+    mbar_init(smem_u32(&d_full), EXACT ? 2 : 1);
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -177,8 +182,8 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t d_tmem = tmem_holder, a_tmem = d_tmem + (kTmemCols - GROUPS * kACols);
-  const uint32_t second = a.rows <= 128 ? a.rows : 0;  // the second accumulator's first column, if there is one
   const WaitCtx wctx{a.status, &abort_flag, a.timeout_ns};
+  const bool worker = warp >= 2 && warp < 2 + 4 * GROUPS;  // dequantises, then stores
   bool ok = true;  // of this role
 
   if (warp == 0) {
@@ -205,36 +210,39 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
         }
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (!worker) {
     // The whole warp runs the loop and one elected lane issues: the compiler then sees addresses and
     // descriptors that are the same in all lanes and keeps them in uniform registers, where the
     // product wants them (from a branch on lane 0, each product took 72 cycles to issue).
-    const uint32_t idesc = make_idesc_f16(kTileN, a.rows, Elem<T>::kIsBf16, 0, 0);
-    const uint32_t d = __shfl_sync(0xffffffffu, d_tmem, 0), at0 = __shfl_sync(0xffffffffu, a_tmem, 0);
-    const uint64_t desc0 = make_sdesc_sw128(smem_u32(smem), 16, 1024);
+    const int me = warp == 1 ? 0 : 1, mine = split ? a.rows / 2 : a.rows;  // rows of this issuer's products
+    const uint32_t idesc = make_idesc_f16(kTileN, mine, Elem<T>::kIsBf16, 0, 0);
+    const uint32_t d = __shfl_sync(0xffffffffu, d_tmem + me * mine, 0), at0 = __shfl_sync(0xffffffffu, a_tmem, 0);
+    const uint64_t desc0 = make_sdesc_sw128(smem_u32(smem) + (split ? me * mine * 128 : 0), 16, 1024);
+    const int turn0 = split ? 0 : me, step = EXACT && !split ? 2 : 1;
     const uint32_t a_full0 = smem_u32(a_full), a_empty0 = smem_u32(a_empty);
-    int s = 0, ph = 0, as = 0, aph = 0;
-    for (int turn = 0; turn < kTurns * nb; ++turn) {
+    int s = 0, ph = 0, as = turn0, aph = 0;
+    for (int turn = turn0; turn < kTurns * nb; turn += step) {
       const int part = EXACT ? turn & 1 : 0;
+      const bool both = EXACT && split;  // the turns of a block's two parts are this issuer's
       ok = mbar_wait(a_full0 + as * 8, aph, wctx, kDevTimeoutMma) &&
-           (merged || part != 0 || mbar_wait(full0 + s * 8, ph, wctx, kDevTimeoutMma));
+           (merged || (both && part != 0) || mbar_wait(full0 + s * 8, ph, wctx, kDevTimeoutMma));
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint64_t bdesc = desc0 + static_cast<uint64_t>((s * stage_bytes + part * panel) >> 4);
       if (elect_one()) {
         const uint32_t stage = at0 + as * kACols;
-        auto more = [&](int k) { return (turn != 0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u; };
+        auto more = [&](int k) { return (turn != turn0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u; };
         if constexpr (EXACT) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_ts(d + (k & 1) * second, stage + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, more(k));
+            mma_ts(d, stage + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, more(k));
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_ts(d + (k & 1) * second, stage + 32 + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, 1u);
+            mma_ts(d, stage + 32 + k * 8, bdesc + static_cast<uint64_t>(k * 2), idesc, 1u);
           if (a.planes == 2)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_ts(d + (k & 1) * second, stage + k * 8, bdesc + static_cast<uint64_t>((panel >> 3) + k * 2), idesc, 1u);
+              mma_ts(d, stage + k * 8, bdesc + static_cast<uint64_t>((panel >> 3) + k * 2), idesc, 1u);
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -242,11 +250,13 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
                    bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2), idesc, more(k));
         }
         mma_commit(a_empty0 + as * 8);
-        if (!merged && part == kTurns - 1) mma_commit(empty0 + s * 8);
+        if (!merged && (!both || part == 1)) mma_commit(empty0 + s * 8);
       }
       __syncwarp();
-      if (++as == GROUPS) as = 0, aph ^= 1;
-      if (part == kTurns - 1 && ++s == a.stages) s = 0, ph ^= 1;
+      as += step;
+      if (as >= GROUPS) as -= GROUPS, aph ^= 1;
+      if (!both || part == 1)
+        if (++s == a.stages) s = 0, ph ^= 1;
     }
     // every product issued has completed before TMEM is read or released
     if (elect_one()) mma_commit(smem_u32(&d_full));
@@ -370,7 +380,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   // ---- epilogue: each quarter's warps take every fourth 8 rows of x (short loops: their code runs
   // once per CTA, so its length is its cost)
   const int q = warp & 3, quarter = (warp - 2) >> 2, n = tile0 * 16 + q * 32 + tile_column(lane);
-  const bool has_n = warp >= 2 && n < a.l.n;
+  const bool has_n = worker && n < a.l.n;
   const float bias = has_n && a.bias != nullptr ? Elem<T>::to_f(static_cast<const T*>(a.bias)[n]) : 0.0f;
   // rows row, row + 1, ... of column n: the first `live` of v
   auto store = [&](int64_t row, auto& v, int live) {
@@ -399,14 +409,15 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
   const uint32_t d_lanes = d_tmem + (static_cast<uint32_t>(q * 32) << 16);
   auto load_sums = [&](int c0, float (&v)[8]) {
     uint32_t u[8], w[8];
+    const bool two = EXACT ? !split : second != 0;  // (a block has a turn for each issuer)
     tmem_ld8(d_lanes + c0, u);
-    if (second != 0) tmem_ld8(d_lanes + second + c0, w);
+    if (two) tmem_ld8(d_lanes + a.rows + c0, w);
     tmem_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]) + (second != 0 ? __uint_as_float(w[i]) : 0.0f);
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]) + (two ? __uint_as_float(w[i]) : 0.0f);
   };
   if (a.ck == 1) {
-    if (warp >= 2 && ok)  // a wait that ran out leaves the rows unwritten
+    if (worker && ok)  // a wait that ran out leaves the rows unwritten
 #pragma unroll 1
       for (int c0 = quarter * 8; c0 < a.rows && row0 + c0 < a.m; c0 += 8 * GROUPS) {
         float v[8];
@@ -419,7 +430,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
     const int share = a.rows / a.ck;
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 2)
+    if (worker)
 #pragma unroll 1
       for (int c0 = quarter * 8; c0 < a.rows; c0 += 8 * GROUPS) {
         float v[8];
@@ -435,7 +446,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS), 1)
       }
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 2 && ok)
+    if (worker && ok)
 #pragma unroll 1
       for (int c = quarter; c < share; c += GROUPS) {
         const int64_t row = row0 + rank * share + c;
@@ -461,7 +472,7 @@ int tile_launch(const W4TileArgs& a, const CUtensorMap& tx, int64_t ctas, int sm
   if (rc != GP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-  cfg.blockDim = dim3(tile_threads(GROUPS), 1, 1);
+  cfg.blockDim = dim3(tile_threads(GROUPS, EXACT), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -525,15 +536,17 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   a.status = dev.status;
   a.timeout_ns = current_timeout_ns();
   a.inject = current_fault_injection();
-  // rows per tile: as even as multiples of 16 up to 256 (128) allow
-  const int64_t most = a.exact ? kMaxTileRows / 2 : kMaxTileRows;
+  // rows per tile: as even as multiples of 16 (32 where two issuers halve them) allow, up to 256, or 128
+  // where x is two T (a stage of 256 such rows takes 128 KB)
+  const int64_t most = a.planes == 2 ? kMaxTileRows / 2 : kMaxTileRows;
   const int64_t row_tiles = (in.m + most - 1) / most;
   a.rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
+  if (a.exact && a.rows > 128) a.rows = (a.rows + 31) / 32 * 32;
   a.row_tiles = static_cast<int>((in.m + a.rows - 1) / a.rows);
   const int64_t units = static_cast<int64_t>((a.l.n_tiles + kTileTiles - 1) / kTileTiles) * a.row_tiles;
   // CTAs along K, by time in tenths of a microsecond: a round of what runs at once costs 4 per block,
-  // 30 to start and end and 18 more with sums across a cluster (16 x 4,096 x 4,096: 16.1 us with one
-  // CTA along K, 11.2 with two, 8.4 with four)
+  // 30 to start and end and 18 more with sums across a cluster; 6 per block with two T per weight
+  // (16 x 4,096 x 4,096: 16.1 us with one CTA along K, 11.2 with two, 8.4 with four)
   static std::atomic<int> cluster_cache[64][4];
   static unsigned long long probe_mask = 0;
   const void* probe = reinterpret_cast<const void*>(&w4_tile_kernel<__half, 1, false, 4, false>);
@@ -543,7 +556,7 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   for (int ck = 1; ck <= 8; ck *= 2) {
     const int slice = (a.l.blocks + ck - 1) / ck;
     if (ck > 1 && ((ck - 1) * slice >= a.l.blocks || a.rows % ck != 0)) break;
-    const int at_once = w4_max_clusters(probe, tile_threads(4), kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
+    const int at_once = w4_max_clusters(probe, tile_threads(4, false), kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
     const int64_t cost = (units + at_once - 1) / at_once * ((a.exact ? 6 : 4) * slice + (ck > 1 ? 48 : 30));
     if (best >= 0 && cost >= best) continue;
     best = cost;
@@ -552,7 +565,7 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   }
   if (units * a.ck >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "w4 linear: m = %lld", (long long)in.m);
   const int stage = 2 * a.rows * 128 * a.planes;
-  a.groups = a.rows > 128 && a.l.units == 4 && a.l.zeros != 0 ? 2 : 4;
+  a.groups = !a.exact && a.rows > 128 && a.l.units == 4 && a.l.zeros != 0 ? 2 : 4;
   const int slot = 4 * a.groups * code_slot(a.l.units, a.l.zeros != 0, a.exact != 0);
   // as many x stages as groups where that fits; then code slots, three if possible
   const int budget = kSmemLimit - 2048;
