@@ -24,8 +24,7 @@
 //                       stores them to the group's TMEM stage of 64 columns. A turn's waits and
 //                       fences take as long as the conversion of 64 rows does, hence whole blocks.
 //   MMA issuer (1 thread) eight K = 16 products per block; commits free the TMEM stage and the x stage.
-//                       Up to 128 rows of x the products alternate between two accumulators. With two T
-//                       per weight there are two issuers, as a turn then is half a block and an issuer's
+//                       With two T per weight there are two issuers, as a turn then is half a block and an issuer's
 //                       wait is answered behind its own products (4,096 -> 14,336 -> 4,096 at 32 rows: 53 us
 //                       with one, 41 with two; single layers gain nothing): up to 128 rows they take the
 //                       turns alternately, each with an accumulator; above, each has half of the rows.
@@ -143,7 +142,6 @@ __global__ void __launch_bounds__(tile_threads(GROUPS, EXACT), 1)
   // at few rows.
   const bool merged = !EXACT && a.stages == GROUPS;
   const bool split = EXACT && a.rows > 128;  // the two issuers take half of the rows each; else every other turn
-  const uint32_t second = !EXACT && a.rows <= 128 ? a.rows : 0;  // one issuer: its second accumulator, if there is one
   const uint32_t full0 = smem_u32(merged ? a_full : full), empty0 = smem_u32(merged ? a_empty : empty);
 
   if ((smem_u32(smem) & 1023u) != 0) {  // the same in every CTA of the grid
@@ -231,7 +229,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS, EXACT), 1)
       const uint64_t bdesc = desc0 + static_cast<uint64_t>((s * stage_bytes + part * panel) >> 4);
       if (elect_one()) {
         const uint32_t stage = at0 + as * kACols;
-        auto more = [&](int k) { return (turn != turn0 || k > (second != 0 ? 1 : 0)) ? 1u : 0u; };
+        auto more = [&](int k) { return (turn != turn0 || k > 0) ? 1u : 0u; };
         if constexpr (EXACT) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -246,7 +244,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS, EXACT), 1)
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            mma_ts(d + (k & 1) * second, stage + k * 8,
+            mma_ts(d, stage + k * 8,
                    bdesc + static_cast<uint64_t>((k >> 2) * (panel >> 4) + (k & 3) * 2), idesc, more(k));
         }
         mma_commit(a_empty0 + as * 8);
@@ -409,7 +407,7 @@ __global__ void __launch_bounds__(tile_threads(GROUPS, EXACT), 1)
   const uint32_t d_lanes = d_tmem + (static_cast<uint32_t>(q * 32) << 16);
   auto load_sums = [&](int c0, float (&v)[8]) {
     uint32_t u[8], w[8];
-    const bool two = EXACT ? !split : second != 0;  // (a block has a turn for each issuer)
+    const bool two = EXACT && !split;  // an accumulator of each issuer (a block has a turn for both)
     tmem_ld8(d_lanes + c0, u);
     if (two) tmem_ld8(d_lanes + a.rows + c0, w);
     tmem_wait_ld();
@@ -536,33 +534,38 @@ int launch_w4_tiles(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& de
   a.status = dev.status;
   a.timeout_ns = current_timeout_ns();
   a.inject = current_fault_injection();
-  // rows per tile: as even as multiples of 16 (32 where two issuers halve them) allow, up to 256, or 128
-  // where x is two T (a stage of 256 such rows takes 128 KB)
-  const int64_t most = a.planes == 2 ? kMaxTileRows / 2 : kMaxTileRows;
-  const int64_t row_tiles = (in.m + most - 1) / most;
-  a.rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
-  if (a.exact && a.rows > 128) a.rows = (a.rows + 31) / 32 * 32;
-  a.row_tiles = static_cast<int>((in.m + a.rows - 1) / a.rows);
-  const int64_t units = static_cast<int64_t>((a.l.n_tiles + kTileTiles - 1) / kTileTiles) * a.row_tiles;
-  // CTAs along K, by time in tenths of a microsecond: a round of what runs at once costs 4 per block,
-  // 30 to start and end and 18 more with sums across a cluster; 6 per block with two T per weight
-  // (16 x 4,096 x 4,096: 16.1 us with one CTA along K, 11.2 with two, 8.4 with four)
   static std::atomic<int> cluster_cache[64][4];
   static unsigned long long probe_mask = 0;
   const void* probe = reinterpret_cast<const void*>(&w4_tile_kernel<__half, 1, false, 4, false>);
   int rc = ensure_smem_attr(probe, kSmemLimit - 2048, &probe_mask);
   if (rc != GP_OK) return rc;
-  int64_t best = -1;
-  for (int ck = 1; ck <= 8; ck *= 2) {
-    const int slice = (a.l.blocks + ck - 1) / ck;
-    if (ck > 1 && ((ck - 1) * slice >= a.l.blocks || a.rows % ck != 0)) break;
-    const int at_once = w4_max_clusters(probe, tile_threads(4, false), kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
-    const int64_t cost = (units + at_once - 1) / at_once * ((a.exact ? 6 : 4) * slice + (ck > 1 ? 48 : 30));
-    if (best >= 0 && cost >= best) continue;
-    best = cost;
-    a.ck = ck;
-    a.slice = slice;
+  // Rows per tile and CTAs along K, by time in hundredths of a microsecond. A round of what runs at once
+  // costs 280 and a row's share to start and end, 180 more with sums across a cluster, and per block 34 (two T per
+  // weight: 42) and what its rows add, as measured at 32 to 256 rows. Rows: as even as multiples of 16
+  // (32 where two issuers halve them) allow, up to 256, or 128 where x is two T (a stage of 256 such rows
+  // takes 128 KB); fewer, down to 64, where that puts more SMs to work.
+  const int64_t most = a.planes == 2 ? kMaxTileRows / 2 : kMaxTileRows, columns = (a.l.n_tiles + kTileTiles - 1) / kTileTiles;
+  int64_t best = -1, units = 0;
+  for (int64_t row_tiles = (in.m + most - 1) / most;; row_tiles *= 2) {
+    int rows = static_cast<int>(((in.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
+    if (a.exact && rows > 128) rows = (rows + 31) / 32 * 32;
+    const int64_t n = columns * ((in.m + rows - 1) / rows);
+    for (int ck = 1; ck <= 8; ck *= 2) {
+      const int slice = (a.l.blocks + ck - 1) / ck;
+      if (ck > 1 && ((ck - 1) * slice >= a.l.blocks || rows % ck != 0)) break;
+      const int at_once = w4_max_clusters(probe, tile_threads(4, false), kSmemLimit - 2048, ck, dev.sm_count, cluster_cache);
+      const int64_t block = a.exact ? 42 + rows / 3 : 34 + rows / 6;
+      const int64_t cost = (n + at_once - 1) / at_once * (block * slice + rows / 2 + (ck > 1 ? 460 : 280));
+      if (best >= 0 && cost >= best) continue;
+      best = cost;
+      units = n;
+      a.rows = rows;
+      a.ck = ck;
+      a.slice = slice;
+    }
+    if (rows <= 64) break;
   }
+  a.row_tiles = static_cast<int>(units / columns);
   if (units * a.ck >= (int64_t(1) << 31)) return set_error(GP_ERR_SHAPE, "w4 linear: m = %lld", (long long)in.m);
   const int stage = 2 * a.rows * 128 * a.planes;
   a.groups = !a.exact && a.rows > 128 && a.l.units == 4 && a.l.zeros != 0 ? 2 : 4;
