@@ -22,12 +22,14 @@
 //                       blocks in turn. Each lane copies its own codes and scales with cp.async into a
 //                       private ring, one or two blocks ahead, turns them into T in registers and
 //                       stores them to the group's TMEM stage of 64 columns. A turn's waits and
-//                       fences take as long as the conversion of 64 rows does, hence whole blocks.
+//                       fences take as long as the conversion of 64 rows does, hence whole blocks
+//                       (half of one where a weight is two T: as many columns).
 //   MMA issuer (1 thread) eight K = 16 products per block; commits free the TMEM stage and the x stage.
-//                       With two T per weight there are two issuers, as a turn then is half a block and an issuer's
-//                       wait is answered behind its own products (4,096 -> 14,336 -> 4,096 at 32 rows: 53 us
-//                       with one, 41 with two; single layers gain nothing): up to 128 rows they take the
-//                       turns alternately, each with an accumulator; above, each has half of the rows.
+//                       With two T per weight there are two issuers, as a turn then is half a block
+//                       and an issuer's wait is answered behind its own products (4,096 -> 14,336 ->
+//                       4,096 at 32 rows: 53 us with one, 41 with two; single layers gain nothing): up to
+//                       128 rows they take the turns alternately, each with an accumulator; above,
+//                       each has half of the rows.
 //   epilogue            the dequantising warps: bias, activation, store
 // Where there are fewer tiles than SMs, a cluster of ck CTAs splits K and sums over distributed
 // shared memory in a fixed order.

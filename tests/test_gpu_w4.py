@@ -351,6 +351,18 @@ def test_mlp(cuda_dev, widths, acts, tail, m):
             assert torch.equal(y, got)
 
 
+@pytest.mark.parametrize("m", [7, 16, 33])
+def test_mlp_wide_hidden_layer(cuda_dev, m):
+    """A hidden layer so wide that the rows of the next product, two T per value, take more than one pass."""
+    widths, dtype, group = (64, 40008, 24, 8), torch.float16, 128
+    layers = [make(k, n, dtype, group, True, i) for i, (k, n) in enumerate(zip(widths[:-1], widths[1:]))]
+    ws = [cuda_ext.w4_pack(*layer, group=group) for layer in layers]
+    x, acts = rows(m, widths[0], dtype), [L.ACT_SILU, L.ACT_GELU_TANH, L.ACT_NONE]
+    got = cuda_ext.w4_mlp(x, ws, [None] * 3, acts=acts)
+    ref, bound = mlp_ref(x, layers, [None] * 3, acts, 0, None, None, 1e-5, group, dtype)
+    check(got, ref, bound, f"m={m}")
+
+
 @pytest.mark.parametrize("widths", [(128, 512, 128), (256, 136, 72, 264), (72, 80, 88, 96, 40)])
 @pytest.mark.parametrize("m", [9, 37, 130])
 def test_roundings_of_a_chain(cuda_dev, widths, m):
@@ -610,3 +622,23 @@ def test_missing_codes_time_out_and_the_next_call_is_right(cuda_dev):
         assert L.device_status(0, clear=True) in (0x100, 0x200, 0x300)  # whichever role gave up first
         assert torch.equal(cuda_ext.w4_linear(x, w4), want)
         assert L.device_status(0) == 0
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_chain_with_missing_codes_times_out(cuda_dev, m):
+    layers = [make(k, n, torch.bfloat16, 128, False) for k, n in ((256, 512), (512, 136), (136, 64))]
+    ws = [cuda_ext.w4_pack(*layer, group=128) for layer in layers]
+    x, kw = rows(m, 256, torch.bfloat16), dict(acts=[L.ACT_RELU, L.ACT_RELU, L.ACT_NONE])
+    want = cuda_ext.w4_mlp(x, ws, [None] * 3, **kw)
+    assert L.device_status(0, clear=True) == 0
+    try:
+        L.set_timeout_ns(5_000_000)
+        L.set_fault_injection(1)
+        cuda_ext.w4_mlp(x, ws, [None] * 3, **kw)
+        torch.cuda.synchronize()
+    finally:
+        L.set_fault_injection(0)
+        L.set_timeout_ns(0)
+    assert L.device_status(0, clear=True) in (0x100, 0x200, 0x300)
+    assert torch.equal(cuda_ext.w4_mlp(x, ws, [None] * 3, **kw), want)
+    assert L.device_status(0) == 0

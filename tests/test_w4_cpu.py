@@ -113,6 +113,8 @@ def test_mlp_workspace_bytes():
     assert _ws([64, 200, 64], L.TAIL_NONE, 5) == 2048  # one hidden buffer: 2,000
     assert _ws([64, 200, 80, 40, 64], L.TAIL_NONE, 5) == 2 * 4096  # two that alternate, of two T per value
     assert _ws([1024, 4096, 1024], L.TAIL_RESIDUAL_LN, 2**20) == 2**20 * (4096 * 2 + 1024 * 4)
+    assert _ws([8, 8, 8], L.TAIL_NONE, 2**30) == 2**30 * 16
+    assert _ws([8, 8, 8, 8], L.TAIL_NONE, 2**30) == L.GP_ERR_SHAPE  # rows of two T are counted in 31 bits
     assert _ws([64, 200, 64], L.TAIL_NONE, -1) == L.GP_ERR_ARG
     assert _ws([64, 201, 64], L.TAIL_NONE, 1) == L.GP_ERR_SHAPE
     assert _ws([64, 200, 7], L.TAIL_NONE, 1) == 512  # the last width is free without a tail
