@@ -26,7 +26,7 @@
 //     their own, in shared memory and across a cluster through st.async, both in a fixed order:
 //     results do not depend on timing.
 // Measured (CUDA-graph replays over more weights than L2 holds): 1 x 8,192 x 28,672 fp16 26.7 us, 4.5
-// TB/s of 121 MB; 16 rows 48.7 us; 1 x 1,024 x 4,096 3.6 us. What is left at one row: about 3.5 us of
+// TB/s of 121 MB; 16 rows 46.9 us; 1 x 1,024 x 4,096 3.6 us. What is left at one row: about 3.5 us of
 // launch and first latency, 13 tiles on the busiest SM for 12.1 on average, and the integer pipe
 // (53 of its 88 cycles per block and SM).
 #include <climits>
