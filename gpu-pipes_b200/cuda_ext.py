@@ -566,6 +566,7 @@ def _refuse(name, t, dtype, shape, dev) -> None:
         raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.get_device() != dev:
         raise RuntimeError(f"{name} is on {t.device}, expected cuda:{dev}")
+    raise RuntimeError(f"{name} cannot be used as {dtype} {tuple(shape)}")  # every refusal raises
 
 
 def _address(name, t, dtype, shape, dev):
@@ -631,21 +632,28 @@ def block_norm_out(x, y, r, h, *, post=L.NORM_NONE, pre=L.NORM_NONE, gate=None, 
     the first block; without x: no residual). gate: [H] for all rows, or [G, H] with M a multiple
     of G: one row for each M / G consecutive rows. r is the new stream, h the next block's input;
     either may be None. x and r have one type (16-bit, or float32 for a stream kept in 32 bits), y
-    may be 16-bit or float32, h, gate, gammas and betas are float16 or bfloat16, all the same. r
-    may be x or y and h may be x or y (in place) where the types match."""
+    may be 16-bit or float32, h, gate, gammas and betas are float16 or bfloat16, all the same (float32
+    ones are refused). r may be x or y and h may be x or y (in place) where the types match."""
     first = x if x is not None else y
     if first is None or (r is None and h is None):
         raise RuntimeError("block_norm needs x or y, and r or h")
-    dev = _cuda_2d("x" if x is not None else "y", first)
-    shape = first.shape
-    m, width = shape
     f32 = torch.float32
     dtype = None  # the 16-bit type of the call
     for t in (h, y, x, r, gate, post_gamma, post_beta, pre_gamma, pre_beta):
-        if t is not None and t.dtype is not f32:
+        if t is not None and getattr(t, "dtype", f32) is not f32:
             dtype = t.dtype
             break
-    dt = _DT.get(dtype) if dtype is not None else L.GP_F16  # all fp32: no matter
+    else:  # all fp32: only x, y and r may be
+        for name, t in (("h", h), ("gate", gate), ("post_gamma", post_gamma), ("post_beta", post_beta),
+                        ("pre_gamma", pre_gamma), ("pre_beta", pre_beta)):
+            if t is not None:
+                if not isinstance(t, torch.Tensor):
+                    raise RuntimeError(f"{name} must be a tensor")
+                raise RuntimeError(f"{name} must be float16 or bfloat16, got {t.dtype}")
+    dev = _cuda_2d("x" if x is not None else "y", first)
+    shape = first.shape
+    m, width = shape
+    dt = _DT.get(dtype) if dtype is not None else L.GP_F16  # all fp32: nothing is of that type
     if dt is None:
         _dtype_code("h", dtype)
     stream_t = x if x is not None else r
@@ -653,7 +661,7 @@ def block_norm_out(x, y, r, h, *, post=L.NORM_NONE, pre=L.NORM_NONE, gate=None, 
     ydt = f32 if y is not None and y.dtype is f32 else dtype
     row = (width,)
     gate_rows, gate_shape = 0, row
-    if gate is not None and gate.dim() == 2:
+    if gate is not None and getattr(gate, "ndim", 1) == 2:
         groups = gate.shape[0]
         if m and (groups == 0 or m % groups):
             raise RuntimeError(f"{m} rows are not a multiple of {groups} gate rows")

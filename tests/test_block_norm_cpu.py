@@ -62,3 +62,21 @@ def test_binding_refusals():
         cuda_ext.block_norm(x.float(), x.float(), pre=L.NORM_RMS)
     with pytest.raises(RuntimeError, match="2-D"):
         cuda_ext.block_norm(x[0], pre=L.NORM_RMS)
+
+
+def test_binding_refuses_32_bit_parameters_and_outputs():
+    """With x and y in fp32 nothing else names the 16-bit type: a gate, a norm's parameters or an h in
+    fp32 are refused by name, not read or written as 16-bit values."""
+    x = torch.zeros(4, 64)
+    row = torch.zeros(64)
+    for name in ("gate", "post_gamma", "post_beta", "pre_gamma", "pre_beta"):
+        with pytest.raises(RuntimeError, match=f"{name} must be float16 or bfloat16"):
+            cuda_ext.block_norm(x, x, post=L.NORM_RMS, **{name: row})
+    with pytest.raises(RuntimeError, match="h must be float16 or bfloat16"):
+        cuda_ext.block_norm_out(x, x, None, torch.zeros(4, 64), pre=L.NORM_RMS)
+    with pytest.raises(RuntimeError, match="h must be float16 or bfloat16"):
+        cuda_ext.block_norm(x, x, pre=L.NORM_RMS, dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="gate must be a tensor"):
+        cuda_ext.block_norm(x, x, gate=[1.0] * 64)
+    with pytest.raises(RuntimeError, match="CUDA"):  # nothing else amiss
+        cuda_ext.block_norm(x, x)

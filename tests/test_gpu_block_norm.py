@@ -225,3 +225,16 @@ def test_first_call_of_a_process_may_be_captured(cuda_dev):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
+def test_all_in_32_bits(cuda_dev):
+    """x, y and r in fp32 and nothing in 16 bits: the sums and norms that need no parameters run; fp32
+    parameters, gates and normed rows are refused."""
+    x, y, gate, pg, pb, ng, nb = _make(cuda_dev, 6, 264, torch.float16, torch.float32, torch.float32, 1)
+    _run_and_check(x, y, LAYER, NONE, None, None, None, None, None, torch.float16, xs=0.5, ys=2.0)
+    with pytest.raises(RuntimeError, match="gate must be float16 or bfloat16"):
+        cuda_ext.block_norm(x, y, gate=gate.float())
+    with pytest.raises(RuntimeError, match="post_gamma must be float16 or bfloat16"):
+        cuda_ext.block_norm(x, y, post=RMS, post_gamma=pg.float())
+    with pytest.raises(RuntimeError, match="h must be float16 or bfloat16"):
+        cuda_ext.block_norm_out(x, y, torch.empty_like(x), torch.empty_like(x), pre=RMS)
