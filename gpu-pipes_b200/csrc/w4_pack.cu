@@ -106,6 +106,8 @@ struct Pair<__nv_bfloat16> {
 // s, and s has 11 bits). below and above are 1 / s less and more 2^-22 of it, so x below and x above lie
 // within 2^-17 of the quotient on both sides: they round to the same integer, or, at a tie, to its two
 // neighbours, of which the even one is wanted. The fused sum rounds the exact products to integers.
+// Below fp32's normal range (bf16 only) 1 / s may be past its largest number: there x and s are both
+// taken 2^24 times, which is exact.
 constexpr float kMagic = 12582912.0f;  // 1.5 2^23: its last place is 1
 constexpr uint32_t kMagicBits = 0x4B400000u;
 
@@ -160,16 +162,17 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_
                       : Elem<T>::pack(__fdiv_rn(h.x, 7.0f), __fdiv_rn(h.y, 7.0f));
     const float2 sv = Elem<T>::unpack(s01);
     const float s[2] = {sv.x, sv.y}, low[2] = {b.x, b.y};
-    float below[2], above[2];
+    float below[2], above[2], up[2];
     int z[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float inv = s[r] > 0.0f ? __fdiv_rn(1.0f, s[r]) : 0.0f;
+      up[r] = Elem<T>::kIsBf16 && s[r] < 0x1p-126f ? 0x1p24f : 1.0f;
+      const float inv = s[r] > 0.0f ? __fdiv_rn(1.0f, s[r] * up[r]) : 0.0f;
       below[r] = inv * (1.0f - 0x1p-22f);
       above[r] = inv * (1.0f + 0x1p-22f);
       z[r] = 8;
       if (ZP) {
-        const uint32_t q = w4_code_bits(-low[r], below[r], above[r], kMagic, 0) - kMagicBits;
+        const uint32_t q = w4_code_bits(-low[r] * up[r], below[r], above[r], kMagic, 0) - kMagicBits;
         z[r] = s[r] > 0.0f ? static_cast<int>(q > 15u ? 15u : q) : 0;
       }
     }
@@ -201,7 +204,9 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_
             const float2 f = Elem<T>::unpack(v[kk]);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              uint32_t q = w4_code_bits(r == 0 ? f.x : f.y, below[r], above[r], mz[r], static_cast<uint32_t>(z[r]));
+              float x = r == 0 ? f.x : f.y;
+              if (edge) x *= up[r];
+              uint32_t q = w4_code_bits(x, below[r], above[r], mz[r], static_cast<uint32_t>(z[r]));
               if (edge) {
                 q = q < kMagicBits ? kMagicBits : q > kMagicBits + 15u ? kMagicBits + 15u : q;
                 if (k0 + kk >= l.k || c + r >= l.n) q = kMagicBits;

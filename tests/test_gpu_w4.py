@@ -151,6 +151,27 @@ def test_quantize_ties_and_extremes(cuda_dev, dtype):
         assert not cuda_ext.w4_dequantize(b4).cpu()[:, 9:12].isfinite().any()
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n", [24, 23])
+def test_quantize_smallest_bf16_groups(cuda_dev, n, zeros):
+    """Groups down to bf16's smallest numbers: 1 / s is past fp32's range for s of 2^-128 and less. Each
+    column is whole numbers (zeros and both signs among them) times 2^(c - 133)."""
+    g = torch.Generator().manual_seed(n)
+    ints = torch.randint(-120, 121, (160, n), generator=g).double()
+    ints[3], ints[7] = 0, 120
+    ints[64:128, 1] = torch.arange(64).double() % 4 - 2  # a scale that rounds to zero or to the smallest number
+    ints[64:128, 2] = torch.arange(64).double() % 12 - 1
+    w = (ints * torch.pow(2.0, torch.arange(n).double() - 133)).to(torch.bfloat16)
+    assert torch.equal(w.double(), ints * torch.pow(2.0, torch.arange(n).double() - 133))
+    for group in (32, 64, 128):
+        w4 = cuda_ext.w4_quantize(w.to(cuda_dev), group=group, zero_points=zeros)
+        codes, scales, z = quantize_ref(w, group, zeros)
+        assert torch.equal(w4.scales().cpu(), scales)
+        assert torch.equal(w4.codes().cpu(), codes)
+        if zeros:
+            assert torch.equal(w4.zeros().cpu(), z)
+
+
 @pytest.mark.parametrize("k,n", SHAPES)
 @pytest.mark.parametrize("zeros", [False, True])
 def test_pack_round_trip(cuda_dev, k, n, zeros):
