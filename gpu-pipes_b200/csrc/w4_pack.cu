@@ -116,6 +116,15 @@ __device__ __forceinline__ uint32_t w4_code_bits(float x, float below, float abo
   return ((a ^ z) & 1u) ? b : a;
 }
 
+// (hi - lo) / 15 in fp32. bf16's hi - lo may be past fp32's largest number, where the halves' difference is not:
+// then it is taken from those (halving and doubling are exact there). Infinities and NaN stay.
+template <typename T>
+__device__ __forceinline__ float w4_span_step(float hi, float lo) {
+  const float span = hi - lo;
+  if (Elem<T>::kIsBf16 && !(span <= 3.4028235e38f)) return 2.0f * __fdiv_rn(0.5f * hi - 0.5f * lo, 15.0f);
+  return __fdiv_rn(span, 15.0f);
+}
+
 // Codes and scale of a group of G rows (largest magnitude to 7, or the range with zero to 15).
 // s is rounded to T first and the codes are taken against the rounded scale. A group whose scale
 // rounds to zero has code = zero point; one with a NaN or an infinity has a scale that is not
@@ -158,7 +167,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const __grid_
     }
     if (!in) continue;
     const float2 h = Elem<T>::unpack(hb), b = Elem<T>::unpack(lb);
-    uint32_t s01 = ZP ? Elem<T>::pack(__fdiv_rn(h.x - b.x, 15.0f), __fdiv_rn(h.y - b.y, 15.0f))
+    uint32_t s01 = ZP ? Elem<T>::pack(w4_span_step<T>(h.x, b.x), w4_span_step<T>(h.y, b.y))
                       : Elem<T>::pack(__fdiv_rn(h.x, 7.0f), __fdiv_rn(h.y, 7.0f));
     const float2 sv = Elem<T>::unpack(s01);
     const float s[2] = {sv.x, sv.y}, low[2] = {b.x, b.y};

@@ -172,6 +172,26 @@ def test_quantize_smallest_bf16_groups(cuda_dev, n, zeros):
             assert torch.equal(w4.zeros().cpu(), z)
 
 
+@pytest.mark.parametrize("n", [8, 7])
+def test_quantize_widest_bf16_range(cuda_dev, n):
+    """Groups whose range hi - lo is past fp32's largest number, (hi - lo) / 15 well within it."""
+    big = torch.finfo(torch.bfloat16).max
+    w = torch.linspace(-1, 1, 72 * n, dtype=torch.float64).view(72, n) * 3e38
+    w[0], w[1] = big, -big
+    w[2:4, 1] = torch.tensor([1.8e38, -1.75e38], dtype=torch.float64)
+    w = w.to(torch.bfloat16)
+    for group in (32, 64, 128):
+        w4 = cuda_ext.w4_quantize(w.to(cuda_dev), group=group, zero_points=True)
+        codes, scales, z = quantize_ref(w, group, True)
+        assert scales.isfinite().all()
+        assert torch.equal(w4.scales().cpu(), scales)
+        assert torch.equal(w4.codes().cpu(), codes)
+        assert torch.equal(w4.zeros().cpu(), z)
+    w[5, 0], w[6, 1], w[7, 2] = float("inf"), -float("inf"), float("nan")
+    sc = cuda_ext.w4_quantize(w.to(cuda_dev), group=128, zero_points=True).scales().cpu()
+    assert not sc[:, :3].isfinite().any() and sc[:, 3:].isfinite().all()
+
+
 @pytest.mark.parametrize("k,n", SHAPES)
 @pytest.mark.parametrize("zeros", [False, True])
 def test_pack_round_trip(cuda_dev, k, n, zeros):
