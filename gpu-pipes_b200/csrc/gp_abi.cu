@@ -719,7 +719,7 @@ static int w4_mlp(const gp_mlp_spec* s, int group, int zero_points, int64_t m, c
                     : static_cast<void*>(ws + (plan.buffers == 2 ? (i & 1) : 0) * plan.hidden);
     W4LinearArgs layer{l[i], s->dtype, m, in, packed[i], b != nullptr ? b[i] : nullptr,
                        last && normed ? GP_ACT_NONE : s->act[i], to, last && normed};
-    layer.exact = nl > 1;  // the layers' errors add up
+    layer.exact = true;  // the layers' errors add up, and a tail's come on top
     layer.x_planes = i > 0 ? plan.planes : 1;
     layer.out_planes = last ? 1 : plan.planes;
     rc = w4_linear(layer, stream);

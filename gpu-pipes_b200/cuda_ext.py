@@ -813,7 +813,8 @@ def w4_dequantize(w4) -> torch.Tensor:
 
 def w4_linear_out(x, w4, bias, out, act=L.ACT_NONE) -> None:
     """out [M, N] = act(x [M, K] W + bias) on 4-bit weights; x, bias (or None) and out have the
-    weights' type. Single tokens, decode batches, prompts."""
+    weights' type. Single tokens, decode batches, prompts. From 17 rows on each weight is rounded to 16
+    bits first; w4_mlp_out of the one layer rounds none."""
     if not isinstance(w4, W4Weight):
         raise RuntimeError("w4 must be a W4Weight")
     dev = _cuda_2d("x", x)

@@ -327,7 +327,8 @@ GP_API int gp_w4_dequantize_out(const gp_w4_spec* spec, const void* packed, void
 
 /* out [m, N] = act(x [m, K] W + bias) on packed weights, T; bias [N] or NULL; act a gp_act. From single
  * tokens to prompts: up to 16 rows the sums over each group are scaled in fp32 and no weight is rounded;
- * from 17 rows on each weight s (q - z) is rounded to T first, as gp_w4_dequantize_out gives it. A row of x
+ * from 17 rows on each weight s (q - z) is rounded to T first, as gp_w4_dequantize_out gives it (a chain of one
+ * layer, gp_w4_mlp_out, rounds none, at more time for prompts). A row of x
  * with an infinity (or, in bf16, with values whose sum over a group is one in fp32) may give NaN where the
  * sum is infinite (or very large). x 16-byte, out and bias 2-byte aligned. */
 GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, const void* packed,
@@ -336,7 +337,7 @@ GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const vo
 /* A chain of layers (gp_mlp_spec) on packed weights: widths of any multiple of 8 (the last one any
  * N without a tail), every activation and tail, no skip layer. Layer l is packed[l], a gp_w4_spec of
  * widths[l] x widths[l + 1], the group and zero_points given here and the spec's dtype. In a chain no weight
- * is rounded, at any m. The hidden activations of two layers are rounded to T; in longer chains they are
+ * is rounded, at any m and any number of layers, one included. The hidden activations of two layers are rounded to T; in longer chains they are
  * kept as two T (m below 2^30). The last layer goes into a LayerNorm tail in fp32. workspace: caller's,
  * 16-byte aligned, at least gp_w4_mlp_workspace_bytes(spec, m) long (0 bytes: NULL is fine), free for
  * other use once the call's work has run. gamma and beta 16-byte aligned. */

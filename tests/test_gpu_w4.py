@@ -432,6 +432,68 @@ def test_roundings_of_a_chain(cuda_dev, widths, m):
         assert rms(got - v) <= 1.1 * final * (2 ** 0.5 if len(layers) == 2 else 1.0) + rms(err), (widths, m, dtype)
 
 
+@pytest.mark.parametrize("tail", [L.TAIL_NONE, L.TAIL_LAYERNORM, L.TAIL_RESIDUAL_LN])
+@pytest.mark.parametrize("m", [9, 17, 37, 130])
+def test_roundings_of_a_chain_of_one_layer(cuda_dev, m, tail):
+    """One layer through the chain's entry point rounds no weight either: what is left is the final
+    rounding. As in test_roundings_of_a_chain, with a tenth for the sample (4,600 values or more); before a
+    tail the sum stays in fp32, and the norm's arithmetic is as mlp_ref derives it, without the term for
+    rounded weights that it has above 16 rows."""
+    k = 512
+    for dtype, group, zeros in ((torch.bfloat16, 128, False), (torch.float16, 32, True), (torch.bfloat16, 32, True)):
+        layer = make(k, k, dtype, group, zeros, 3)
+        w = weights64(*layer, group)
+        x = rows(m, k, dtype)
+        got = cuda_ext.w4_mlp(x, [cuda_ext.w4_pack(*layer, group=group)], [None], acts=[L.ACT_NONE], tail=tail)
+        v, x = x.double() @ w, x.double()
+        err = 2 * U32 * (2 * k / 16 + 96) * (x.abs() @ w.abs())
+        if tail:
+            c = 128 * U32
+            v = v + (x if tail == L.TAIL_RESIDUAL_LN else 0)
+            e = err + err.mean(1, keepdim=True) + c * (v.abs() + x.abs() + 2 * v.abs().mean(1, keepdim=True))
+            d = v - v.mean(1, keepdim=True)
+            rs = 1 / torch.sqrt(d.square().mean(1, keepdim=True) + 1e-5)
+            v = d * rs
+            err = e * rs + v.abs() * (2 * torch.sqrt(e.square().mean(1, keepdim=True)) * rs + c)
+        rms = lambda t: t.square().mean().sqrt().item()  # noqa: E731
+        assert rms(got.double() - v) <= 1.1 * rms(v.to(dtype).double() - v) + rms(err), (m, tail, dtype)
+
+
+@pytest.mark.parametrize("act", [L.ACT_SILU, L.ACT_GELU_TANH, L.ACT_SIGMOID])
+@pytest.mark.parametrize("tail", [L.TAIL_NONE, L.TAIL_RESIDUAL_LN])
+@pytest.mark.parametrize("m", [12, 33, 140])
+def test_roundings_of_a_chain_with_activations_and_tails(cuda_dev, act, tail, m):
+    """test_roundings_of_a_chain with activations, biases and tails (3,168 values or more): the residual,
+    the biases and the norm only add to what the errors are measured against."""
+    for dtype, group, zeros in ((torch.bfloat16, 64, True), (torch.bfloat16, 128, False), (torch.float16, 128, False)):
+        for widths in ((264, 520, 264), (264, 136, 392, 264)):
+            layers = [make(k, n, dtype, group, zeros, i) for i, (k, n) in enumerate(zip(widths[:-1], widths[1:]))]
+            ws = [cuda_ext.w4_pack(*layer, group=group) for layer in layers]
+            biases = [rows(1, n, dtype, 9)[0].contiguous() for n in widths[1:]]
+            x, nl = rows(m, widths[0], dtype), len(layers)
+            got = cuda_ext.w4_mlp(x, ws, biases, acts=[act] * (nl - 1) + [L.ACT_NONE], tail=tail)
+            v, err, x = x.double(), torch.zeros_like(x, dtype=torch.float64), x.double()
+            for i, layer in enumerate(layers):
+                w = weights64(*layer, group)
+                mag = v.abs() @ w.abs()
+                err = err @ w.abs() + (2 * U32 * (3 * w.shape[0] / 16 + 96) + 2 * half_step(dtype) ** 2) * mag
+                v = v @ w + biases[i].double()
+                err = err + U32 * (v.abs() + biases[i].double().abs())
+                if i + 1 < nl:
+                    err, v = 1.13 * err + 16 * U32 * (v.abs() + 1), act64(act, v)
+            if tail:
+                c = 128 * U32
+                v = v + x
+                e = err + err.mean(1, keepdim=True) + c * (v.abs() + x.abs() + 2 * v.abs().mean(1, keepdim=True))
+                d = v - v.mean(1, keepdim=True)
+                rs = 1 / torch.sqrt(d.square().mean(1, keepdim=True) + 1e-5)
+                v = d * rs
+                err = e * rs + v.abs() * (2 * torch.sqrt(e.square().mean(1, keepdim=True)) * rs + c)
+            rms = lambda t: t.square().mean().sqrt().item()  # noqa: E731
+            final = rms(v.to(dtype).double() - v)
+            assert rms(got.double() - v) <= 1.1 * final * (2 ** 0.5 if nl == 2 else 1.0) + rms(err), (widths, m, dtype)
+
+
 def test_bert_ffn_takes_packed_weights(cuda_dev):
     """The BERT-large block's entry point with 4-bit weights, against the same block on the 16-bit
     values that they stand for: the fused 16-bit chain has its own roundings (fp16 hidden
