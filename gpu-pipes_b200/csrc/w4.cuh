@@ -111,8 +111,30 @@ __device__ __forceinline__ uint32_t w4_load_word(uint32_t v) {
 // zero point and the code's offset away (both steps exact before the scale).
 //   half: 1024 + q minus 1024 + z; column 1 four bits higher: (1024 + 16 q) / 16 - (64 + z)
 //   bf16: 16 + q minus 16 + z
+// As two T (with `rest`) a weight past T's largest number is that number and the rest of it, infinite only past
+// twice the largest: the rounded product alone would be infinite and its rest minus infinity.
 template <typename T>
 struct W4Exact;
+
+// Whether 15 times one of two scales may round to infinity: only then need the products be limited. (Limiting
+// always: 46 -> 49 us at 64 rows of 4,096 -> 14,336 -> 4,096; a warp that looks first: 46.4.)
+template <typename T>
+__device__ __forceinline__ bool w4_large(uint32_t s01) {
+  constexpr uint32_t kMost = Elem<T>::kIsBf16 ? 0x7D88u : 0x6C43u;  // 1.0625 2^124, 4,364
+  const uint32_t a = s01 & 0x7FFF7FFFu;
+  return (a & 0xFFFFu) > kMost || (a >> 16) > kMost;
+}
+
+// a pair of T, each limited to T's largest number in magnitude; a NaN stays
+template <typename T>
+__device__ __forceinline__ uint32_t w4_limit(uint32_t a) {
+  uint32_t r;
+  if constexpr (Elem<T>::kIsBf16)
+    asm("min.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x7F7F7F7Fu));
+  else
+    asm("min.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x7BFF7BFFu));
+  return r;
+}
 
 template <>
 struct W4Exact<__half> {
@@ -129,9 +151,10 @@ struct W4Exact<__half> {
     }
   }
   // r[2 column + j]: rows (0, 1) (j = 0) and (2, 3) of the word, as tcgen05.st 16x256b takes them. rest: what
-  // each rounding took away, itself exact in T (s (q - z) has four bits more than T; only below T's
-  // smallest normal value is it rounded once more).
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* r, uint32_t* rest = nullptr) const {
+  // each rounding took away, itself exact in T (s (q - z) has four bits more than T) but for weights
+  // below T's smallest normal value or past its largest: there it may be rounded once more, by at most half a
+  // step of the weight in the second case. large: some scale of the group is w4_large.
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* r, uint32_t* rest = nullptr, bool large = false) const {
     const __half2 sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -139,10 +162,16 @@ struct W4Exact<__half> {
       const uint32_t lo = (v & 0x000F000Fu) | 0x64006400u, hi = (v & 0x00F000F0u) | 0x64006400u;
       const __half2 qa = __hadd2(*reinterpret_cast<const __half2*>(&lo), c[0]);
       const __half2 qb = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, c[1]);
-      const __half2 a = __hmul2(qa, s[0]), b = __hmul2(qb, s[1]);
+      __half2 a = __hmul2(qa, s[0]), b = __hmul2(qb, s[1]);
       r[i] = *reinterpret_cast<const uint32_t*>(&a);
       r[2 + i] = *reinterpret_cast<const uint32_t*>(&b);
       if (rest != nullptr) {
+        if (large) {
+          r[i] = w4_limit<__half>(r[i]);
+          r[2 + i] = w4_limit<__half>(r[2 + i]);
+          a = *reinterpret_cast<const __half2*>(&r[i]);
+          b = *reinterpret_cast<const __half2*>(&r[2 + i]);
+        }
         const __half2 ea = __hfma2(qa, s[0], __hneg2(a)), eb = __hfma2(qb, s[1], __hneg2(b));
         rest[i] = *reinterpret_cast<const uint32_t*>(&ea);
         rest[2 + i] = *reinterpret_cast<const uint32_t*>(&eb);
@@ -165,15 +194,19 @@ struct W4Exact<__nv_bfloat16> {
       c[0] = c[1] = __float2bfloat162_rn(-24.0f);
     }
   }
-  __device__ __forceinline__ void word(uint32_t w, uint32_t* r, uint32_t* rest = nullptr) const {
+  __device__ __forceinline__ void word(uint32_t w, uint32_t* r, uint32_t* rest = nullptr, bool large = false) const {
     uint32_t p[4];
     W4Deq<__nv_bfloat16>::pairs(w, p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // p[2 j + column], j: rows (0, 1) / (2, 3)
       const __nv_bfloat162 q = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&p[i]), c[i & 1]);
-      const __nv_bfloat162 a = __hmul2(q, s[i & 1]);
+      __nv_bfloat162 a = __hmul2(q, s[i & 1]);
       r[2 * (i & 1) + (i >> 1)] = *reinterpret_cast<const uint32_t*>(&a);
       if (rest != nullptr) {
+        if (large) {
+          r[2 * (i & 1) + (i >> 1)] = w4_limit<__nv_bfloat16>(r[2 * (i & 1) + (i >> 1)]);
+          a = *reinterpret_cast<const __nv_bfloat162*>(&r[2 * (i & 1) + (i >> 1)]);
+        }
         const __nv_bfloat162 e = __hfma2(q, s[i & 1], __hneg2(a));
         rest[2 * (i & 1) + (i >> 1)] = *reinterpret_cast<const uint32_t*>(&e);
       }

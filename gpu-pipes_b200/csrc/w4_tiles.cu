@@ -37,6 +37,8 @@
 #include "chain_registry.h"
 #include "w4.cuh"
 
+#include <type_traits>
+
 namespace gp {
 namespace {
 
@@ -321,15 +323,23 @@ __global__ void __launch_bounds__(tile_threads(GROUPS, EXACT), 1)
         w4_lds<4>(my_codes + at + i * kTurnCodes + part * 512, c);
         w4_lds<kUse>(my_scales + at + i * (128 * kUse), sw);
       }
-      W4Exact<T> dq;
+      auto words = [&](auto large) {
+        W4Exact<T> dq;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        constexpr int kPer = ZP ? 2 : 1;
-        const int u = (UNITS == 1 ? 0 : UNITS == 2 ? part : 2 * part + h) * kPer;
-        if (UNITS == 4 || h == 0) dq.set(sw[u], sw[u + kPer - 1], ZP);
-        dq.word(c[2 * h], r + 8 * h, rest == nullptr ? nullptr : rest + 8 * h);
-        dq.word(c[2 * h + 1], r + 8 * h + 4, rest == nullptr ? nullptr : rest + 8 * h + 4);
-      }
+        for (int h = 0; h < 2; ++h) {
+          constexpr int kPer = ZP ? 2 : 1;
+          const int u = (UNITS == 1 ? 0 : UNITS == 2 ? part : 2 * part + h) * kPer;
+          if (UNITS == 4 || h == 0) dq.set(sw[u], sw[u + kPer - 1], ZP);
+          dq.word(c[2 * h], r + 8 * h, rest == nullptr ? nullptr : rest + 8 * h, large);
+          dq.word(c[2 * h + 1], r + 8 * h + 4, rest == nullptr ? nullptr : rest + 8 * h + 4, large);
+        }
+      };
+      bool large = false;
+      if constexpr (EXACT)
+#pragma unroll
+        for (int w = 0; w < kUse; w += ZP ? 2 : 1) large |= w4_large<T>(sw[w]);
+      if (EXACT && __any_sync(0xffffffffu, large)) words(std::true_type{});
+      else words(std::false_type{});
     };
     // the TMEM stage is free: its last products have completed
     auto stage_free = [&](bool never_used) {

@@ -337,8 +337,10 @@ GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const vo
 /* A chain of layers (gp_mlp_spec) on packed weights: widths of any multiple of 8 (the last one any
  * N without a tail), every activation and tail, no skip layer. Layer l is packed[l], a gp_w4_spec of
  * widths[l] x widths[l + 1], the group and zero_points given here and the spec's dtype. In a chain no weight
- * is rounded, at any m and any number of layers, one included. The hidden activations of two layers are rounded to T; in longer chains they are
- * kept as two T (m below 2^30). The last layer goes into a LayerNorm tail in fp32. workspace: caller's,
+ * is rounded, at any m and any number of layers, one included (but for weights past T's largest number: from 17
+ * rows on such a weight may be rounded to T's 8 or 11 bits, and is infinite past twice that number). The hidden
+ * activations of two layers are rounded to T; in longer chains they are kept as two T (m below 2^30); either
+ * way one past T's largest number is infinite. The last layer goes into a LayerNorm tail in fp32. workspace: caller's,
  * 16-byte aligned, at least gp_w4_mlp_workspace_bytes(spec, m) long (0 bytes: NULL is fine), free for
  * other use once the call's work has run. gamma and beta 16-byte aligned. */
 GP_API int gp_w4_mlp_out(const gp_mlp_spec* spec, int group, int zero_points, int64_t m, const void* x,

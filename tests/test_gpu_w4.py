@@ -494,6 +494,40 @@ def test_roundings_of_a_chain_with_activations_and_tails(cuda_dev, act, tail, m)
             assert rms(got.double() - v) <= 1.1 * final * (2 ** 0.5 if nl == 2 else 1.0) + rms(err), (widths, m, dtype)
 
 
+@pytest.mark.parametrize("m", [5, 16, 17, 40, 150])
+@pytest.mark.parametrize("layers", [1, 2, 3])
+def test_chain_with_fp16_weights_past_the_largest_number(cuda_dev, m, layers):
+    """s (q - z) past 65,504 with scales that are finite: the sum is finite at any number of rows. The
+    first layer's weights are quantised ones (the largest fp16 number becomes 7 x 9,360 = 65,520, which
+    rounds to infinity) or packed ones up to 8 x 16,000; its products are small enough for the hidden
+    values to be finite. Past 65,504 the second of a weight's two parts is at most 65,504, so what its
+    rounding takes is at most 16: half_step times the weight, relative to at least 65,504."""
+    dtype, group = torch.float16, 64
+    g = torch.Generator().manual_seed(m)
+    k, n = 136, 72
+    big = (torch.randn(k, n, generator=g) * 2e4).clamp(-65504, 65504)
+    big[::9] = 65504.0 * torch.sign(big[::9])
+    w4 = cuda_ext.w4_quantize(big.to(dtype).to(cuda_dev), group=group)
+    quantised = (w4.codes(), w4.scales(), None)
+    assert weights64(*quantised, group).abs().max() > 65504
+    codes, scales, _ = make(k, n, dtype, group, False)
+    packed = (codes, (scales.float() / scales.float().max() * 16000).to(dtype), None)
+    rest = [make(72, 72, dtype, group, False, i) for i in range(1, layers)]
+    acts = [L.ACT_RELU] * (layers - 1) + [L.ACT_NONE]
+    x = (rows(m, k, dtype).double() * 2.0 ** -12).to(dtype)
+    for first in (quantised, packed):
+        chain = [first, *rest]
+        ws = [cuda_ext.w4_pack(*layer, group=group) for layer in chain]
+        got = cuda_ext.w4_mlp(x, ws, [None] * layers, acts=acts)
+        ref, bound = mlp_ref(x, chain, [None] * layers, acts, 0, None, None, 1e-5, group, dtype)
+        assert got.isfinite().all()
+        check(got, ref, bound, f"m={m}")
+        if first is quantised and layers == 1:  # every such weight is two fp16 numbers: exact
+            final = (ref.to(dtype).double() - ref).square().mean().sqrt()
+            sums = 2 * U32 * (3 * k / 16 + 96) * (x.double().abs() @ weights64(*first, group).abs())
+            assert (got.double() - ref).square().mean().sqrt() <= 1.1 * final + sums.square().mean().sqrt()
+
+
 def test_bert_ffn_takes_packed_weights(cuda_dev):
     """The BERT-large block's entry point with 4-bit weights, against the same block on the 16-bit
     values that they stand for: the fused 16-bit chain has its own roundings (fp16 hidden
