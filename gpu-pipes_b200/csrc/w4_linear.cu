@@ -7,11 +7,9 @@
 //     of W) and 8 or 16 rows of x on the other side; one to eight rows cost the same and the sums are
 //     fp32. (tcgen05 wants 16-bit weights in TMEM or shared memory, a store and a read per weight
 //     more: that form is w4_tiles.cu, for more rows.)
-//   - A code becomes an operand with one mask (w4.cuh): the operand is q plus a constant, scaled by a
-//     power of two. sum_k x (q - z) = sum_k x (q + c) - (c + z) sum_k x, and the second term starts
-//     the accumulator; the sums of x over each group are taken once per CTA. The group's scale
-//     multiplies the fp32 sum, so no weight is rounded. A first form that subtracted z from each
-//     weight and divided to find the group ran 348 instructions per 2,048 weights and 57 us at
+//   - A code becomes an operand q - z with one mask and one packed sum per two weights, both exact
+//     (w4.cuh). The group's scale multiplies the fp32 sum, so no weight is rounded. A first form that
+//     worked weight by weight and divided to find the group ran 348 instructions per 2,048 weights and 57 us at
 //     1 x 8,192 x 28,672 (fp16, groups of 128), where the bytes take 18.5.
 //
 //   - A CTA of 16 computing warps owns a slice of K (one of `ck` CTAs of a cluster does; ck = 1: all of
@@ -25,10 +23,10 @@
 //   - The codes of the next tiles are in flight while the sums of this one are joined by warps of
 //     their own, in shared memory and across a cluster through st.async, both in a fixed order:
 //     results do not depend on timing.
-// Measured (CUDA-graph replays over more weights than L2 holds): 1 x 8,192 x 28,672 fp16 26.7 us, 4.5
-// TB/s of 121 MB; 16 rows 46.9 us; 1 x 1,024 x 4,096 3.6 us. What is left at one row: about 3.5 us of
-// launch and first latency, 13 tiles on the busiest SM for 12.1 on average, and the integer pipe
-// (53 of its 88 cycles per block and SM).
+// Measured (CUDA-graph replays over more weights than L2 holds): 1 x 8,192 x 28,672 fp16 28.2 us, 4.3
+// TB/s of 121 MB; 16 rows 41.8 us; 1 x 1,024 x 4,096 bf16 3.3 us. What is left at one row: about 3.5 us of
+// launch and first latency, 13 tiles on the busiest SM for 12.1 on average, and latency between: no unit
+// is above half of its rate (issue 54%, integer pipe 43%).
 #include <climits>
 
 #include "../../include/gpipes.h"
@@ -137,8 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
   const int np = kWarps / a.ws;                               // tiles at a time
   const int outs = np * TT * 128;                             // sums of a tile group
   float* red = part + 2 * kWarps * kPart;                     // [2][outs], clusters only
-  float* xsum = red + (a.ck > 1 ? 2 * outs : 0);              // [slice * UNITS][8 TT]
-  uint8_t* zeros = reinterpret_cast<uint8_t*>(xsum + a.slice * UNITS * 8 * TT);
+  uint8_t* zeros = reinterpret_cast<uint8_t*>(red + (a.ck > 1 ? 2 * outs : 0));
   uint8_t* xs = zeros + kZeroBytes;                           // [rows][x_stride]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -215,45 +212,28 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
         }
     }
   } else {
-  // x rows of this CTA's slice (zero past K) and their sums over each group. Sixteen lanes hold a
-  // block of a row; absent rows have sums of zero and are read from the zeros.
+  // x rows of this CTA's slice (zero past K); absent rows are read from the zeros.
   constexpr int kStagers = 32 * (kWarps + kJoinWarps);
   if (threadIdx.x < kZeroBytes / 16) reinterpret_cast<uint4*>(zeros)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   {
     const int pieces = a.slice * 16;  // 16-byte pieces of a row
-    for (int i = threadIdx.x; i < (8 * TT - rows) * a.slice * UNITS; i += kStagers) {
-      const int dead = 8 * TT - rows;
-      xsum[i / dead * (8 * TT) + rows + i % dead] = 0.0f;
-    }
-    for (int i0 = 0; i0 < rows * pieces; i0 += kStagers) {
-      const int i = i0 + threadIdx.x;
+    for (int i = threadIdx.x; i < rows * pieces; i += kStagers) {
       const int r = i / pieces, c = i % pieces;
       const int k = b0 * kW4Block + c * 8;
       uint4 v = make_uint4(0, 0, 0, 0);
       const T* from = static_cast<const T*>(a.x) + (row0 + r) * a.l.k + k;
-      if (r < rows && k < a.l.k) v = *reinterpret_cast<const uint4*>(from);
-      if (r < rows) {  // rows 16 j + 4 t + i of a 32-row half where lane t reads them as 16 bytes, j by j
-        uint8_t* to = xs + r * a.x_stride + (c >> 2) * 64 + (c & 1) * 32 + ((c >> 1) & 1) * 8;
-        *reinterpret_cast<uint2*>(to) = make_uint2(v.x, v.y);
-        *reinterpret_cast<uint2*>(to + 16) = make_uint2(v.z, v.w);
-      }
-      float sum2 = 0.0f;
+      if (k < a.l.k) v = *reinterpret_cast<const uint4*>(from);
+      // rows 16 j + 4 t + i of a 32-row half where lane t reads them as 16 bytes, j by j
+      uint8_t* to = xs + r * a.x_stride + (c >> 2) * 64 + (c & 1) * 32 + ((c >> 1) & 1) * 8;
+      *reinterpret_cast<uint2*>(to) = make_uint2(v.x, v.y);
+      *reinterpret_cast<uint2*>(to + 16) = make_uint2(v.z, v.w);
       if constexpr (PLANES == 2) {
         uint4 u = make_uint4(0, 0, 0, 0);
-        if (r < rows && k < a.l.k) u = *reinterpret_cast<const uint4*>(from + a.m * a.l.k);
-        if (r < rows) {
-          uint8_t* to = xs + (rows + r) * a.x_stride + (c >> 2) * 64 + (c & 1) * 32 + ((c >> 1) & 1) * 8;
-          *reinterpret_cast<uint2*>(to) = make_uint2(u.x, u.y);
-          *reinterpret_cast<uint2*>(to + 16) = make_uint2(u.z, u.w);
-        }
-        const float2 e0 = Elem<T>::unpack(u.x), e1 = Elem<T>::unpack(u.y), e2 = Elem<T>::unpack(u.z), e3 = Elem<T>::unpack(u.w);
-        sum2 = ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+        if (k < a.l.k) u = *reinterpret_cast<const uint4*>(from + a.m * a.l.k);
+        to += rows * a.x_stride;
+        *reinterpret_cast<uint2*>(to) = make_uint2(u.x, u.y);
+        *reinterpret_cast<uint2*>(to + 16) = make_uint2(u.z, u.w);
       }
-      const float2 f0 = Elem<T>::unpack(v.x), f1 = Elem<T>::unpack(v.y), f2 = Elem<T>::unpack(v.z), f3 = Elem<T>::unpack(v.w);
-      float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y)) + sum2;
-#pragma unroll
-      for (int o = 1; o < 16 / UNITS; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (r < rows && c % (16 / UNITS) == 0) xsum[(c / (16 / UNITS)) * (8 * TT) + r] = sum;
     }
   }
   bar_sync(kBarFull);  // x is in place (this barrier's first use as a buffer's comes after)
@@ -359,41 +339,25 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
       xstep[i] = live ? kW4Block * 2 : 0;
       xsecond[i] = live ? rows * a.x_stride : 0;
     }
-    const uint32_t xsum0 = smem_u32(xsum) + (lead * UNITS * 8 * TT + 2 * t) * 4;
-    constexpr int kXsumBlock = UNITS * 8 * TT * 4;
     float acc[TT][4];
-    // a block: codes and scales at c and s, x rows at xa, their group sums at xg
-    auto block = [&](uint32_t c, uint32_t s, const uint32_t (&xa)[TT], uint32_t xg) {
+    // a block: codes and scales at c and s, x rows at xa
+    auto block = [&](uint32_t c, uint32_t s, const uint32_t (&xa)[TT]) {
       const uint4 cbuf[2] = {lds128(c), lds128(c + kW4BlockBytes / 2)};
       uint32_t sbuf[kWords];
       w4_lds<kWords>(s, sbuf);
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
         float sum[TT][4];
-        float2 z = make_float2(-8.0f - W4Deq<T>::kOffset, -8.0f - W4Deq<T>::kOffset);
-        if constexpr (ZP) {
-          z = Elem<T>::unpack(sbuf[2 * u + 1]);
-          z.x = -W4Deq<T>::kOffset - z.x;
-          z.y = -W4Deq<T>::kOffset - z.y;
-        }
-        z.x *= kUnit0;
-        z.y *= kUnit1;
+        W4Deq<T> dq;
+        dq.template set<ZP>(ZP ? sbuf[2 * u + 1] : 0u);
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
-          uint32_t v[2];
-          w4_lds<2>(xg + u * (8 * TT * 4) + i * 32, v);
-          const float2 xv = make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
-          sum[i][0] = z.x * xv.x;
-          sum[i][1] = z.x * xv.y;
-          sum[i][2] = z.y * xv.x;
-          sum[i][3] = z.y * xv.y;
-        }
+        for (int i = 0; i < TT; ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.0f;
 #pragma unroll
         for (int h = u * (4 / UNITS); h < (u + 1) * (4 / UNITS); ++h) {  // 32 rows at a time
           const uint4 cw = cbuf[h >> 1];
           uint32_t p0[4], p1[4];
-          W4Deq<T>::pairs((h & 1) ? cw.z : cw.x, p0);
-          W4Deq<T>::pairs((h & 1) ? cw.w : cw.y, p1);
+          dq.pairs((h & 1) ? cw.z : cw.x, p0);
+          dq.pairs((h & 1) ? cw.w : cw.y, p1);
 #pragma unroll
           for (int i = 0; i < TT; ++i) {
             const uint4 xv = lds128(xa[i] + h * 64);
@@ -424,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
     for (int it = 0, tile = cluster * np + slot_tile; it < a.iters; ++it, tile += tile_step) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-      uint32_t xa[TT], xg = xsum0;
+      uint32_t xa[TT];
 #pragma unroll
       for (int i = 0; i < TT; ++i) xa[i] = xa0[i];
       // blocks left for this warp from `lead` on, run by run; every warp takes part in every stage
@@ -441,14 +405,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
 #pragma unroll
         for (int b = 0; b < RUN; ++b) {
           if (b >= left) break;
-          block(cs + b * kW4BlockBytes, s + b * kScaleBytes, xb, xg + b * kXsumBlock);
+          block(cs + b * kW4BlockBytes, s + b * kScaleBytes, xb);
 #pragma unroll
           for (int i = 0; i < TT; ++i) xb[i] += xstep[i];
         }
         left -= stride;
 #pragma unroll
         for (int i = 0; i < TT; ++i) xa[i] += stride * xstep[i];
-        xg += stride * kXsumBlock;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&empty[stage]));
         cs += kStage;
@@ -476,11 +439,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_rows_kernel(const __grid_const
 
 int rows_x_stride(int slice) { return slice * (kW4Block * 2) + 64; }  // conflict-free: 64 past a multiple of 128
 
-// Shared memory of a CTA: rings, warps' sums, clusters' sums, group sums of x, zeros, x rows
+// Shared memory of a CTA: rings, warps' sums, clusters' sums, zeros, x rows
 // (`rows` times its planes)
 int64_t rows_smem(const W4Layout& l, int tt, int ck, int ws, int slice, int rows, int slots) {
   const int64_t outs = static_cast<int64_t>(kWarps / ws) * tt * 128;
-  return static_cast<int64_t>(kWarps) * slots * (kW4BlockBytes + l.scale_bytes()) + 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) + 32ll * slice * l.units * tt +
+  return static_cast<int64_t>(kWarps) * slots * (kW4BlockBytes + l.scale_bytes()) + 2ll * kWarps * tt * 8 * kPartStride * 4 + (ck > 1 ? 2 * outs * 4 : 0) +
          kZeroBytes + static_cast<int64_t>(rows) * rows_x_stride(slice);
 }
 

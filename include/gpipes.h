@@ -328,9 +328,9 @@ GP_API int gp_w4_dequantize_out(const gp_w4_spec* spec, const void* packed, void
 /* out [m, N] = act(x [m, K] W + bias) on packed weights, T; bias [N] or NULL; act a gp_act. From single
  * tokens to prompts: up to 16 rows the sums over each group are scaled in fp32 and no weight is rounded;
  * from 17 rows on each weight s (q - z) is rounded to T first, as gp_w4_dequantize_out gives it (a chain of one
- * layer, gp_w4_mlp_out, rounds none, at more time for prompts). A row of x
- * with an infinity (or, in bf16, with values whose sum over a group is one in fp32) may give NaN where the
- * sum is infinite (or very large). x 16-byte, out and bias 2-byte aligned. */
+ * layer, gp_w4_mlp_out, rounds none, at more time for prompts). An
+ * infinite x gives what the formula does. Up to 16 rows the sums of x (q - z) over each group have to stay within
+ * fp32's range (bf16 values past 2^117 may not). x 16-byte, out and bias 2-byte aligned. */
 GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, const void* packed,
                             const void* bias, void* out, void* stream);
 
@@ -340,7 +340,8 @@ GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const vo
  * is rounded, at any m and any number of layers, one included (but for weights past T's largest number: from 17
  * rows on such a weight may be rounded to T's 8 or 11 bits, and is infinite past twice that number). The hidden
  * activations of two layers are rounded to T; in longer chains they are kept as two T (m below 2^30); either
- * way one past T's largest number is infinite. The last layer goes into a LayerNorm tail in fp32. workspace: caller's,
+ * way one past T's largest number is infinite. From 17 rows on a row with an infinity, in x or in a hidden
+ * activation, becomes NaN. The last layer goes into a LayerNorm tail in fp32. workspace: caller's,
  * 16-byte aligned, at least gp_w4_mlp_workspace_bytes(spec, m) long (0 bytes: NULL is fine), free for
  * other use once the call's work has run. gamma and beta 16-byte aligned. */
 GP_API int gp_w4_mlp_out(const gp_mlp_spec* spec, int group, int zero_points, int64_t m, const void* x,

@@ -312,6 +312,52 @@ def test_linear_infinities_stay_in_their_row_and_column(cuda_dev):
         assert torch.equal(out[:, cols], clean[:, cols]) and out[:, 17].isnan().all()
 
 
+@pytest.mark.parametrize("m", [1, 3, 8, 9, 16, 17, 70])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_outliers_that_meet_zero_weights(cuda_dev, m, zeros):
+    """Values of x far above the rest whose weights are all zero (q = z) take nothing from the others'
+    sums, in a layer and in a chain: the bound has |x| |w| in it, not |x| and the codes."""
+    for dtype, big in ((torch.bfloat16, 2.0 ** 30), (torch.float16, 6e4)):
+        for group in (32, 128):
+            k, n = 1096, 200
+            codes, scales, z = make(k, n, dtype, group, zeros)
+            hot = torch.arange(5, k, 61, device=codes.device)
+            codes[hot] = torch.full_like(codes[hot], 8) if z is None else z[hot // group]
+            x = rows(m, k, dtype)
+            x[:, hot] = big
+            w4 = cuda_ext.w4_pack(codes, scales, z, group=group)
+            ref, err = linear_ref(x.double(), torch.zeros_like(x, dtype=torch.float64),
+                                  weights64(codes, scales, z, group), None, L.ACT_NONE, dtype)
+            if m > 16:  # tiny weights' rounding, here of weights that are not tiny
+                err = err - tiny(dtype) * x.double().abs().sum(1, keepdim=True)
+            check(cuda_ext.w4_linear(x, w4), ref, rounded(ref, err, dtype), f"m={m} {dtype}")
+            check(cuda_ext.w4_mlp(x, [w4], [None], acts=[L.ACT_NONE]), ref, rounded(ref, err, dtype), f"chain m={m} {dtype}")
+
+
+@pytest.mark.parametrize("m", [2, 8, 16, 20])
+def test_linear_infinite_rows_follow_the_definition(cuda_dev, m):
+    """An infinite x gives plus or minus infinity, or NaN where it meets a weight of zero or the other
+    infinity, at any number of rows. Large finite values stay finite where their products with q - z do
+    (64 times 2^119 times 24 would not)."""
+    for dtype in DTYPES:
+        for zeros in (False, True):
+            codes, scales, z = make(256, 96, dtype, 64, zeros)
+            x = rows(m, 256, dtype)
+            x[0, 5] = float("inf")
+            x[1, 250] = -float("inf")
+            w = weights64(codes, scales, z, 64)
+            got, ref = cuda_ext.w4_linear(x, cuda_ext.w4_pack(codes, scales, z, group=64)).double(), x.double() @ w
+            assert torch.equal(got[:2].nan_to_num(7.0, 1.0, -1.0), ref[:2].nan_to_num(7.0, 1.0, -1.0))
+            assert got[2:].isfinite().all()
+    x = rows(m, 256, torch.bfloat16)
+    x[0, :128] = 2.0 ** 119
+    codes, scales, z = make(256, 96, torch.bfloat16, 64, False)
+    scales = (scales.double() * 2.0 ** -100).to(torch.bfloat16)
+    ref, err = linear_ref(x.double(), torch.zeros_like(x, dtype=torch.float64), weights64(codes, scales, z, 64), None,
+                          L.ACT_NONE, torch.bfloat16)
+    check(cuda_ext.w4_linear(x, cuda_ext.w4_pack(codes, scales, z, group=64)), ref, rounded(ref, err, torch.bfloat16), f"m={m}")
+
+
 def test_linear_is_repeatable(cuda_dev):
     for m in (1, 12, 64):
         codes, scales, z = make(4096, 2000, torch.bfloat16, 128, True)
