@@ -85,6 +85,7 @@ _SPECS: dict = {}
 
 def _spec(widths, acts, tail, dt, ln_eps, skip_layer):
     """The chain description, built once per distinct chain (the struct is read-only to C)."""
+    ln_eps = float(ln_eps)  # a tensor would be kept by its identity
     key = (tuple(widths), tuple(acts), tail, dt, ln_eps, skip_layer)
     s = _SPECS.get(key)
     if s is None:
@@ -633,7 +634,8 @@ def block_norm_out(x, y, r, h, *, post=L.NORM_NONE, pre=L.NORM_NONE, gate=None, 
     of G: one row for each M / G consecutive rows. r is the new stream, h the next block's input;
     either may be None. x and r have one type (16-bit, or float32 for a stream kept in 32 bits), y
     may be 16-bit or float32, h, gate, gammas and betas are float16 or bfloat16, all the same (float32
-    ones are refused). r may be x or y and h may be x or y (in place) where the types match."""
+    ones are refused). r may be x or y and h may be x or y (in place) where the types match. Scales and
+    epsilons are numbers; one held in a tensor is read at the call."""
     first = x if x is not None else y
     if first is None or (r is None and h is None):
         raise RuntimeError("block_norm needs x or y, and r or h")
@@ -667,7 +669,8 @@ def block_norm_out(x, y, r, h, *, post=L.NORM_NONE, pre=L.NORM_NONE, gate=None, 
             raise RuntimeError(f"{m} rows are not a multiple of {groups} gate rows")
         gate_rows, gate_shape = m // groups if m else 0, (groups, width)
     _launch(dev, L.lib().gp_block_norm_out,
-            _norm_spec(width, dt, stream is f32, ydt is f32, post, pre, post_eps, pre_eps, x_scale, y_scale, gate_rows),
+            _norm_spec(width, dt, stream is f32, ydt is f32, post, pre, float(post_eps), float(pre_eps), float(x_scale),
+                       float(y_scale), gate_rows),
             m, None if x is None else _address("x", x, stream, shape, dev),
             None if y is None else _address("y", y, ydt, shape, dev),
             None if gate is None else _address("gate", gate, dtype, gate_shape, dev),
@@ -844,6 +847,7 @@ _W4_CHAINS: dict = {}
 
 def _w4_chain(m, widths, acts, tail, dtype, ln_eps):
     """The chain's description and the workspace bytes of m rows."""
+    ln_eps = float(ln_eps)  # a tensor would be kept by its identity
     key = (m, widths, acts, tail, dtype, ln_eps)
     c = _W4_CHAINS.get(key)
     if c is None:

@@ -238,3 +238,15 @@ def test_all_in_32_bits(cuda_dev):
         cuda_ext.block_norm(x, y, post=RMS, post_gamma=pg.float())
     with pytest.raises(RuntimeError, match="h must be float16 or bfloat16"):
         cuda_ext.block_norm_out(x, y, torch.empty_like(x), torch.empty_like(x), pre=RMS)
+
+
+def test_scales_as_tensors_are_read_at_the_call(cuda_dev):
+    """A scale or an epsilon held in a tensor counts with the value that it has at the call."""
+    x, y, *_ = _make(cuda_dev, 5, 64, torch.float16, torch.float16, torch.float16, 0)
+    scale, eps = torch.tensor(1.0), torch.tensor(1e-5)
+    for a, e in ((1.0, 1e-5), (0.25, 0.5), (-2.0, 4.0)):
+        scale.fill_(a)
+        eps.fill_(e)
+        got = cuda_ext.block_norm(x, y, post=RMS, pre=LAYER, x_scale=scale, y_scale=scale, post_eps=eps, pre_eps=eps)
+        want = cuda_ext.block_norm(x, y, post=RMS, pre=LAYER, x_scale=a, y_scale=a, post_eps=e, pre_eps=e)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -574,6 +574,15 @@ def test_chain_with_fp16_weights_past_the_largest_number(cuda_dev, m, layers):
             assert (got.double() - ref).square().mean().sqrt() <= 1.1 * final + sums.square().mean().sqrt()
 
 
+def test_chain_epsilon_as_a_tensor_is_read_at_the_call(cuda_dev):
+    w4 = cuda_ext.w4_pack(*make(64, 64, torch.float16, 64, False), group=64)
+    x, eps = rows(3, 64, torch.float16), torch.tensor(1e-5)
+    for e in (1e-5, 0.5, 8.0):
+        eps.fill_(e)
+        kw = dict(acts=[L.ACT_NONE], tail=L.TAIL_LAYERNORM)
+        assert torch.equal(cuda_ext.w4_mlp(x, [w4], [None], ln_eps=eps, **kw), cuda_ext.w4_mlp(x, [w4], [None], ln_eps=e, **kw))
+
+
 def test_bert_ffn_takes_packed_weights(cuda_dev):
     """The BERT-large block's entry point with 4-bit weights, against the same block on the 16-bit
     values that they stand for: the fused 16-bit chain has its own roundings (fp16 hidden

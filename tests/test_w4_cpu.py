@@ -173,3 +173,12 @@ def test_binding_refusals():
                                skip_layer=1)
     with pytest.raises(RuntimeError, match="match"):
         cuda_ext.w4_mlp_out(torch.zeros(1, 64), [w], [None], torch.zeros(1, 32), acts=[0, 0])
+
+
+def test_chain_descriptions_hold_the_value_of_an_epsilon():
+    """A tensor as the epsilon counts with its value at the call, in 16-bit and in 4-bit chains."""
+    eps = torch.tensor(1.0)
+    for value in (1.0, 0.5, 8.0):
+        eps.fill_(value)
+        assert cuda_ext._spec((64, 64), (0,), L.TAIL_LAYERNORM, L.GP_F16, eps, 0).ln_eps == value
+        assert cuda_ext._w4_chain(2, (64, 64), (0,), L.TAIL_LAYERNORM, torch.float16, eps)[0]._obj.ln_eps == value
