@@ -219,9 +219,11 @@ int launch_t(const BlockNormArgs& a, cudaStream_t stream) {
 
 // A row is one warp up to 1,024 columns (no barrier, eight rows in flight per CTA), one CTA above. The
 // CTA's size keeps two vectors per thread up to 4,096 columns, four above: a row's two reductions are
-// latency, which other CTAs on the SM cover, and more threads per row (512 x 2 instead of 256 x 4 at
-// 8,192 columns) leave fewer of them. Measured on 16-bit rows with a norm on both sides (TB/s of x, y, r, h):
-// 32,768 x 2,048 6.3 (256 x 1: 5.2), 16,384 x 4,096 6.8, 8,192 x 8,192 with gates 5.6 (512 x 2: 4.8).
+// latency, which other CTAs on the SM cover, and more threads per row leave fewer of them; fewer threads
+// leave single rows slower. Measured on bf16 rows with a norm on both sides (TB/s of x, y, r, h; the other
+// split in brackets): 32,768 x 2,048 6.3 (256 x 1: 5.4); 16,384 x 4,096 6.0 (128 x 4: 6.3) and one such row 2.8 us
+// (3.5); 8,192 x 8,192 5.9 (512 x 2: 5.8), in fp16 with gates 5.0 (5.4); 4,096 x 16,384 3.8. Above 16,384
+// columns 1,024 threads leave 64 registers for four vectors and some spill: 2,048 x 32,768 4.2, fp32 stream 3.7.
 template <typename T, typename X, typename Y>
 int launch_w(const BlockNormArgs& a, cudaStream_t s) {
   const int h = a.width;

@@ -615,9 +615,10 @@ int launch_w4_rows(const W4LinearArgs& in, cudaStream_t s, const DeviceInfo& dev
   return rc;
 }
 
-// Up to 16 rows the row kernel, from 17 on the tile kernel. Measured on either side of the border
-// (us, row / tile kernel; 9, 16 and 64 rows): 4,096 x 14,336 15.3 / 16.3, 16.7 / 16.4, 66 / 19;
-// 8,192 x 28,672 42 / 58, 43 / 58, 199 / 66; 1,024 x 4,096 4.4 / 5.5, 5.3 / 5.5, 20 / 7.
+// Up to 16 rows the row kernel, from 17 on the tile kernel. Measured on either side of the border (CUDA-graph
+// replays, fp16, groups of 128; us, row / tile kernel; 9, 16, 17 and 64 rows): 4,096 x 14,336 14.0 / 15.0, 16.3 / 15.0,
+// 29 / 15.2, 63 / 16.7; 8,192 x 28,672 39 / 54, 42 / 54, 82 / 55, 166 / 58; 1,024 x 4,096 4.1 / 5.3, 4.4 / 5.3, 7.4 / 5.8,
+// 17 / 6.7.
 int launch_w4_linear(const W4LinearArgs& a, cudaStream_t s, const DeviceInfo& dev) {
   return a.m <= kRowsMax ? launch_w4_rows(a, s, dev) : launch_w4_tiles(a, s, dev);
 }
