@@ -25,8 +25,8 @@
 //     results do not depend on timing.
 // Measured (CUDA-graph replays over more weights than L2 holds): 1 x 8,192 x 28,672 fp16 28.2 us, 4.3
 // TB/s of 121 MB; 16 rows 41.8 us; 1 x 1,024 x 4,096 bf16 3.3 us. What is left at one row: about 3.5 us of
-// launch and first latency, 13 tiles on the busiest SM for 12.1 on average, and latency between: no unit
-// is above half of its rate (issue 54%, integer pipe 43%).
+// launch and first latency, 13 tiles on the busiest SM for 12.1 on average, and latency between
+// (issue at 54%, the busiest pipe at 43%).
 #include <climits>
 
 #include "../../include/gpipes.h"

@@ -328,9 +328,9 @@ GP_API int gp_w4_dequantize_out(const gp_w4_spec* spec, const void* packed, void
 /* out [m, N] = act(x [m, K] W + bias) on packed weights, T; bias [N] or NULL; act a gp_act. From single
  * tokens to prompts: up to 16 rows the sums over each group are scaled in fp32 and no weight is rounded;
  * from 17 rows on each weight s (q - z) is rounded to T first, as gp_w4_dequantize_out gives it (a chain of one
- * layer, gp_w4_mlp_out, rounds none, at more time for prompts). An
- * infinite x gives what the formula does. Up to 16 rows the sums of x (q - z) over each group have to stay within
- * fp32's range (bf16 values past 2^117 may not). x 16-byte, out and bias 2-byte aligned. */
+ * layer, gp_w4_mlp_out, rounds none, at more time for prompts). An infinite x gives what the formula does. Up
+ * to 16 rows the sums of x (q - z) over each group have to stay within fp32's range (bf16 values past 2^117 may
+ * not). x 16-byte, out and bias 2-byte aligned. */
 GP_API int gp_w4_linear_out(const gp_w4_spec* spec, int64_t m, int act, const void* x, const void* packed,
                             const void* bias, void* out, void* stream);
 
